@@ -14,13 +14,13 @@ from . import _lib  # noqa: F401
 from ._lib import DSV41Error, lib_path  # noqa: F401
 
 __all__ = ["dequant", "moe", "engram", "linear", "act_quant", "gemm", "ep", "release", "convert",
-           "DSV41Error", "lib_path"]
+           "lora", "DSV41Error", "lib_path"]
 
 
 def __getattr__(name):
     # submodules load lazily so that importing the package never touches CUDA
     if name in ("dequant", "moe", "engram", "linear", "act_quant", "gemm", "ep", "release",
-                "convert"):
+                "convert", "lora"):
         import importlib
         return importlib.import_module(f"{__name__}.{name}")
     raise AttributeError(name)

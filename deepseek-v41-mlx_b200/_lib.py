@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import threading
+from contextlib import nullcontext
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB_NAME = "libdsv41q.so"
@@ -76,6 +77,15 @@ PROTOTYPES = {
     "dsv41_moe_route_workspace_size": (_SZ, [_I64, _I64, _I64]),
     "dsv41_moe_route": (_I, [_P, _I64, _I64, _P, _P, _I64, _I, _I, _F, _I, _F, _P, _P, _P, _SZ,
                              _P]),
+    "dsv41_moe_logits": (_I, [_P, _I64, _I64, _P, _I64, _P, _P, _SZ, _P]),
+    "dsv41_moe_balance_workspace_size": (_SZ, [_I64, _I64]),
+    "dsv41_moe_balance": (_I, [_P, _I, _I64, _I64, _P, _I, _P, _I64, _P, _I, _F, _P, _P, _I, _F,
+                               _P, _P, _P, _P, _SZ, _P]),
+    "dsv41_lora_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I]),
+    "dsv41_lora_forward": (_I, [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _P, _P, _I, _P, _P,
+                                _P, _SZ, _P]),
+    "dsv41_lora_backward": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _I,
+                                 _P, _I, _P, _P, _P, _SZ, _P]),
     "dsv41_moe_decode_workspace_size": (_SZ, [C.POINTER(MoeConfig), _I64]),
     "dsv41_moe_decode_pack_size": (_SZ, [C.POINTER(MoeConfig)]),
     "dsv41_ep_create": (_I, [_I, _I, _I64, _I, _I64, C.POINTER(_P)]),
@@ -201,6 +211,12 @@ def ptr(t) -> int:
 
 def stream_of(t) -> int:
     return torch().cuda.current_stream(t.device).cuda_stream
+
+
+def on(device):
+    """Context in which ``device`` is the current device (nothing to do when it already is)."""
+    t = torch()
+    return nullcontext() if t.cuda.current_device() == device.index else t.cuda.device(device)
 
 
 def dtype_code(dt) -> int:

@@ -14,6 +14,8 @@
 #include "aqgemm.cuh"
 #include "a16gemm.cuh"
 #include "gemv_m1.cuh"
+#include "lora.cuh"
+#include "balance.cuh"
 
 #include <mutex>
 
@@ -675,6 +677,206 @@ extern "C" int dsv41_moe_route(const void *x, int64_t T, int64_t D, const void *
   return route_impl(x, T, D, gate_w, bias, E, topk, score_func, gate_temp, norm_topk_prob,
                     route_scale, weights, indices, reinterpret_cast<float *>(workspace),
                     STREAM(stream));
+}
+
+extern "C" size_t dsv41_moe_balance_workspace_size(int64_t T, int64_t S) {
+  return align_up(size_t(S > 0 ? S : 0) * 4, 256) + align_up(size_t(T > 0 ? T : 0) * 4, 256) + 256;
+}
+
+extern "C" int dsv41_moe_balance(const void *logits, int dtype, int64_t T, int64_t E,
+                                 const int32_t *indices, int topk, const int32_t *offsets,
+                                 int64_t S, const uint8_t *mask, int score_func, float gate_temp,
+                                 const float *grad_loss, const float *dweights,
+                                 int norm_topk_prob, float route_scale, float *loss,
+                                 int32_t *counts, void *dlogits, void *workspace,
+                                 size_t workspace_bytes, void *stream) {
+  DSV41_REQUIRE(dtype == DSV41_F32 || dtype == DSV41_BF16, DSV41_ERR_BAD_DTYPE,
+                "logits must be F32 or BF16");
+  DSV41_REQUIRE(T >= 0 && T <= INT32_MAX, DSV41_ERR_BAD_SHAPE, "0 <= T < 2^31");
+  DSV41_REQUIRE(E > 0 && E <= 1024, DSV41_ERR_BAD_SHAPE, "1 <= E <= 1024");
+  DSV41_REQUIRE(S >= 0 && S < INT32_MAX, DSV41_ERR_BAD_SHAPE, "0 <= S < 2^31 - 1");
+  DSV41_REQUIRE(topk >= 1 && topk <= 64 && topk <= E, DSV41_ERR_BAD_ARG, "1 <= topk <= min(64, E)");
+  DSV41_REQUIRE(score_func >= 0 && score_func <= 2, DSV41_ERR_BAD_ARG, "unknown score_func");
+  DSV41_REQUIRE(gate_temp > 0.0f, DSV41_ERR_BAD_ARG, "gate_temp must be positive");
+  DSV41_REQUIRE(offsets || S == 1, DSV41_ERR_BAD_ARG, "without offsets there is one sequence");
+  DSV41_REQUIRE(T == 0 || dlogits || (!grad_loss && !dweights), DSV41_ERR_BAD_ARG,
+                "grad_loss and dweights need dlogits");
+  DSV41_REQUIRE(S == 0 || (loss && counts), DSV41_ERR_BAD_ARG, "NULL pointer");
+  DSV41_REQUIRE(T == 0 || (logits && indices), DSV41_ERR_BAD_ARG, "NULL pointer");
+  DSV41_REQUIRE(workspace && workspace_bytes >= dsv41_moe_balance_workspace_size(T, S),
+                DSV41_ERR_WORKSPACE, "workspace too small");
+  WsCarve ws{static_cast<uint8_t *>(workspace), workspace_bytes, 0};
+  int *live = ws.take<int>(S);
+  float *tok_dot = ws.take<float>(T);
+  cudaStream_t st = STREAM(stream);
+  if (S > 0) {
+    DSV41_LAUNCH(cudaMemsetAsync(live, 0, S * 4, st), "balance memset");
+    DSV41_LAUNCH(cudaMemsetAsync(counts, 0, S * E * 4, st), "balance memset");
+  }
+  if (T > 0) {
+    { ProfScope prof("balance_count", st);
+    k_balance_count<<<unsigned(ceil_div(T, 256)), 256, 0, st>>>(indices, T, topk, int(E), offsets,
+                                                                int(S), mask, counts, live); }
+    DSV41_CHECK_LAUNCH("balance_count");
+    ProfScope prof("balance_row", st);
+    const unsigned th = unsigned(ceil_div(E, 32) * 32);
+    if (dtype == DSV41_F32)
+      k_balance_row<float><<<unsigned(T), th, 0, st>>>(
+          static_cast<const float *>(logits), T, int(E), indices, topk, offsets, int(S), mask,
+          score_func, gate_temp, grad_loss, dweights, norm_topk_prob, route_scale, counts, live,
+          tok_dot, static_cast<float *>(dlogits));
+    else
+      k_balance_row<__nv_bfloat16><<<unsigned(T), th, 0, st>>>(
+          static_cast<const __nv_bfloat16 *>(logits), T, int(E), indices, topk, offsets, int(S),
+          mask, score_func, gate_temp, grad_loss, dweights, norm_topk_prob, route_scale, counts,
+          live, tok_dot, static_cast<__nv_bfloat16 *>(dlogits));
+    DSV41_CHECK_LAUNCH("balance_row");
+  }
+  if (S > 0) {
+    ProfScope prof("balance_loss", st);
+    k_balance_loss<<<unsigned(S), 256, 0, st>>>(tok_dot, T, int(E), topk, offsets, live, loss);
+    DSV41_CHECK_LAUNCH("balance_loss");
+  }
+  return DSV41_OK;
+}
+
+extern "C" int dsv41_moe_logits(const void *x, int64_t T, int64_t D, const void *gate_w, int64_t E,
+                                float *logits, void *workspace, size_t workspace_bytes,
+                                void *stream) {
+  int rc = route_check(T, D, E, 1, 0);
+  if (rc) return rc;
+  if (T == 0) return DSV41_OK;
+  DSV41_REQUIRE(x && gate_w && logits, DSV41_ERR_BAD_ARG, "NULL pointer");
+  DSV41_REQUIRE(workspace && workspace_bytes >= dsv41_moe_route_workspace_size(T, D, E),
+                DSV41_ERR_WORKSPACE, "workspace too small");
+  DSV41_REQUIRE(aligned(x, 16) && aligned(gate_w, 16), DSV41_ERR_MISALIGNED,
+                "x and gate_w must be 16-byte aligned");
+  const int nks = router_nks(T, D, E);
+  float *partial = nks > 1 ? static_cast<float *>(workspace) : logits;
+  const int64_t warps = ceil_div(E, 16) * ceil_div(T, 8) * nks;
+  cudaStream_t st = STREAM(stream);
+  { ProfScope prof("router_scores", st);
+  DSV41_LAUNCH(launch_pdl(k_router_scores, dim3(unsigned(ceil_div(warps * 32, 128))), dim3(128), 0,
+                          st, static_cast<const __nv_bfloat16 *>(x), T, D,
+                          static_cast<const __nv_bfloat16 *>(gate_w), E, nks, partial),
+               "router_scores"); }
+  if (nks > 1) {
+    ProfScope prof("router_sum", st);
+    k_router_sum<<<unsigned(ceil_div(T * E, 256)), 256, 0, st>>>(partial, nks, T * E, logits);
+    DSV41_CHECK_LAUNCH("router_sum");
+  }
+  return DSV41_OK;
+}
+
+// ======================================================================= adapters
+
+namespace {
+
+int lora_check(int64_t T, int64_t K, int64_t N, int64_t n, int64_t R) {
+  DSV41_REQUIRE(T >= 0 && T <= INT32_MAX && K > 0 && K % 8 == 0 && N > 0, DSV41_ERR_BAD_SHAPE,
+                "0 <= T < 2^31, K a positive multiple of 8, N positive");
+  DSV41_REQUIRE(n > 0 && n <= 8192, DSV41_ERR_BAD_SHAPE, "1 <= adapters <= 8192");
+  DSV41_REQUIRE(R > 0 && R <= 128 && R % 8 == 0, DSV41_ERR_UNSUPPORTED,
+                "the rank must be a multiple of 8 up to 128");
+  return DSV41_OK;
+}
+
+template <typename OT>
+void lora_expand_launch(const float *h, int64_t T, int64_t N, const void *w, int64_t wc,
+                        int64_t wr, int64_t n, int R, const int32_t *ids, const float *scaling,
+                        const void *base, void *y, cudaStream_t st) {
+  k_lora_expand<OT><<<unsigned(ceil_div(T * N, 256)), 256, 0, st>>>(
+      h, T, N, static_cast<const __nv_bfloat16 *>(w), wc, wr, n, R, ids, scaling,
+      static_cast<const OT *>(base), static_cast<OT *>(y));
+}
+
+}  // namespace
+
+extern "C" size_t dsv41_lora_workspace_size(int64_t T, int64_t K, int64_t N, int64_t n, int64_t R,
+                                            int backward) {
+  return align_up(size_t(T > 0 && R > 0 ? T * R : 0) * 4, 256) + 256;
+}
+
+extern "C" int dsv41_lora_forward(const void *x, int64_t T, int64_t K, const void *a,
+                                  const void *b, int64_t n, int64_t R, int64_t N,
+                                  const float *scaling, const int32_t *ids, const void *base,
+                                  int out_dtype, void *y, float *h_out, void *workspace,
+                                  size_t workspace_bytes, void *stream) {
+  int rc = lora_check(T, K, N, n, R);
+  if (rc) return rc;
+  DSV41_REQUIRE(out_dtype == DSV41_F32 || out_dtype == DSV41_BF16, DSV41_ERR_BAD_DTYPE,
+                "out_dtype must be F32 or BF16");
+  if (T == 0) return DSV41_OK;
+  DSV41_REQUIRE(x && a && b && ids && y, DSV41_ERR_BAD_ARG, "NULL pointer");
+  DSV41_REQUIRE(aligned(x, 16) && aligned(a, 16) && aligned(b, 16), DSV41_ERR_MISALIGNED,
+                "x, a and b must be 16-byte aligned");
+  DSV41_REQUIRE(workspace && workspace_bytes >= dsv41_lora_workspace_size(T, K, N, n, R, 0),
+                DSV41_ERR_WORKSPACE, "workspace too small");
+  cudaStream_t st = STREAM(stream);
+  float *h = h_out ? h_out : static_cast<float *>(workspace);
+  { ProfScope prof("lora_shrink", st);
+  k_lora_shrink<<<unsigned(ceil_div(T * R * 32, 256)), 256, 0, st>>>(
+      static_cast<const __nv_bfloat16 *>(x), T, K, static_cast<const __nv_bfloat16 *>(a), K, 1, n,
+      int(R), ids, nullptr, h); }
+  DSV41_CHECK_LAUNCH("lora_shrink");
+  ProfScope prof("lora_expand", st);
+  if (out_dtype == DSV41_F32)
+    lora_expand_launch<float>(h, T, N, b, R, 1, n, int(R), ids, scaling, base, y, st);
+  else
+    lora_expand_launch<__nv_bfloat16>(h, T, N, b, R, 1, n, int(R), ids, scaling, base, y, st);
+  DSV41_CHECK_LAUNCH("lora_expand");
+  return DSV41_OK;
+}
+
+extern "C" int dsv41_lora_backward(const void *dy, const void *x, const float *h, const void *a,
+                                   const void *b, int64_t T, int64_t K, int64_t N, int64_t n,
+                                   int64_t R, const float *scaling, const int32_t *ids,
+                                   const void *dx_base, int dx_dtype, void *dx, int grad_dtype,
+                                   void *da, void *db, void *workspace, size_t workspace_bytes,
+                                   void *stream) {
+  int rc = lora_check(T, K, N, n, R);
+  if (rc) return rc;
+  DSV41_REQUIRE((dx_dtype == DSV41_F32 || dx_dtype == DSV41_BF16) &&
+                    (grad_dtype == DSV41_F32 || grad_dtype == DSV41_BF16),
+                DSV41_ERR_BAD_DTYPE, "dx_dtype and grad_dtype must be F32 or BF16");
+  DSV41_REQUIRE(da && db, DSV41_ERR_BAD_ARG, "NULL pointer");
+  DSV41_REQUIRE(T == 0 || (dy && x && h && a && b && ids && dx), DSV41_ERR_BAD_ARG,
+                "NULL pointer");
+  DSV41_REQUIRE(aligned(x, 16) && aligned(a, 16) && aligned(b, 16) && aligned(dy, 16),
+                DSV41_ERR_MISALIGNED, "dy, x, a and b must be 16-byte aligned");
+  DSV41_REQUIRE(workspace && workspace_bytes >= dsv41_lora_workspace_size(T, K, N, n, R, 1),
+                DSV41_ERR_WORKSPACE, "workspace too small");
+  cudaStream_t st = STREAM(stream);
+  float *g = static_cast<float *>(workspace);
+  const __nv_bfloat16 *dyb = static_cast<const __nv_bfloat16 *>(dy),
+                      *xb = static_cast<const __nv_bfloat16 *>(x);
+  if (T > 0) {
+    { ProfScope prof("lora_shrink", st);
+    k_lora_shrink<<<unsigned(ceil_div(T * R * 32, 256)), 256, 0, st>>>(
+        dyb, T, N, static_cast<const __nv_bfloat16 *>(b), 1, R, n, int(R), ids, scaling, g); }
+    DSV41_CHECK_LAUNCH("lora_shrink");
+    ProfScope prof("lora_expand", st);
+    if (dx_dtype == DSV41_F32)
+      lora_expand_launch<float>(g, T, K, a, 1, K, n, int(R), ids, nullptr, dx_base, dx, st);
+    else
+      lora_expand_launch<__nv_bfloat16>(g, T, K, a, 1, K, n, int(R), ids, nullptr, dx_base, dx, st);
+    DSV41_CHECK_LAUNCH("lora_expand");
+  }
+  ProfScope prof("lora_wgrad", st);
+  const unsigned ba = unsigned(ceil_div(n * R * K, 256)), bb = unsigned(ceil_div(n * R * N, 256));
+  if (grad_dtype == DSV41_F32) {
+    k_lora_wgrad<float><<<ba, 256, 0, st>>>(g, xb, T, K, n, int(R), ids, nullptr, K, 1,
+                                            static_cast<float *>(da));
+    k_lora_wgrad<float><<<bb, 256, 0, st>>>(h, dyb, T, N, n, int(R), ids, scaling, 1, R,
+                                            static_cast<float *>(db));
+  } else {
+    k_lora_wgrad<__nv_bfloat16><<<ba, 256, 0, st>>>(g, xb, T, K, n, int(R), ids, nullptr, K, 1,
+                                                    static_cast<__nv_bfloat16 *>(da));
+    k_lora_wgrad<__nv_bfloat16><<<bb, 256, 0, st>>>(h, dyb, T, N, n, int(R), ids, scaling, 1, R,
+                                                    static_cast<__nv_bfloat16 *>(db));
+  }
+  DSV41_CHECK_LAUNCH("lora_wgrad");
+  return DSV41_OK;
 }
 
 // ======================================================================= MoE decode

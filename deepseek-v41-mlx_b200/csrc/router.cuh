@@ -60,6 +60,16 @@ __global__ void __launch_bounds__(128) k_router_scores(const __nv_bfloat16 *__re
   }
 }
 
+// out[e] = sum of the K splits' partial products, in split order
+__global__ void k_router_sum(const float *__restrict__ partial, int nks, int64_t n,
+                             float *__restrict__ out) {
+  const int64_t e = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+  if (e >= n) return;
+  float s = 0.0f;
+  for (int ks = 0; ks < nks; ++ks) s += partial[ks * n + e];
+  out[e] = s;
+}
+
 struct ArgMax {
   float v;
   int i;

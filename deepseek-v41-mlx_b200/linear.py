@@ -97,14 +97,26 @@ def linear_affine(x, wq, scales, biases, bits=4, group_size=64, out_dtype=None):
     return y.reshape(tuple(xt.shape[:-1]) + (N,))
 
 
+def _with_lora(y, x, lora, ids):
+    """The adapters' part (``lora.LoRA``) added to a projection's output in place, in fp32 on the
+    output as rounded to its dtype."""
+    if lora is None:
+        return y
+    return lora(x, ids, base=y, out=y)
+
+
 class FP8Linear:
-    """Release fp8 linear: weight e4m3 [out, in], scale ue8m0 [ceil(out/32), ceil(in/32)]."""
+    """Release fp8 linear: weight e4m3 [out, in], scale ue8m0 [ceil(out/32), ceil(in/32)].
+
+    With ``lora`` (a ``lora.LoRA`` bank) and ``lora_ids`` (int32, the adapter of each row of x,
+    negative for none) the rows' adapters are added; the other layers take them the same way."""
 
     def __init__(self, weight, scale):
         self.weight, self.scale = weight, scale
 
-    def __call__(self, x, out_dtype=None):
-        return linear_fp8(x, self.weight, self.scale, out_dtype)
+    def __call__(self, x, out_dtype=None, lora=None, lora_ids=None):
+        y = linear_fp8(x, self.weight, self.scale, out_dtype)
+        return _with_lora(y, x, lora, lora_ids)
 
 
 class FP4Linear:
@@ -113,8 +125,9 @@ class FP4Linear:
     def __init__(self, weight, scale):
         self.weight, self.scale = weight, scale
 
-    def __call__(self, x, out_dtype=None):
-        return linear_fp4(x, self.weight, self.scale, out_dtype)
+    def __call__(self, x, out_dtype=None, lora=None, lora_ids=None):
+        y = linear_fp4(x, self.weight, self.scale, out_dtype)
+        return _with_lora(y, x, lora, lora_ids)
 
 
 class QuantizedLinear:
@@ -124,6 +137,7 @@ class QuantizedLinear:
         self.weight, self.scales, self.biases = weight, scales, biases
         self.group_size, self.bits = group_size, bits
 
-    def __call__(self, x, out_dtype=None):
-        return linear_affine(x, self.weight, self.scales, self.biases, self.bits,
-                             self.group_size, out_dtype)
+    def __call__(self, x, out_dtype=None, lora=None, lora_ids=None):
+        y = linear_affine(x, self.weight, self.scales, self.biases, self.bits,
+                          self.group_size, out_dtype)
+        return _with_lora(y, x, lora, lora_ids)

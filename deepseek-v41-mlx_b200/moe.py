@@ -83,6 +83,102 @@ class Gate:
         return weights.reshape(shp), indices.reshape(shp)
 
 
+    def logits(self, x):
+        """The router's products x @ weight.T as float32 [..., E], before gate_temp and the
+        score function: the input of ``balance_loss``."""
+        t = _torch()
+        xt = L.cuda_tensor(x, "x")
+        if xt.dtype != t.bfloat16:
+            xt = xt.to(t.bfloat16)
+        w = L.cuda_tensor(self.weight, "gate.weight").to(t.bfloat16)
+        E, D = w.shape
+        T = xt.numel() // D
+        if xt.shape[-1] != D or w.device != xt.device:
+            raise ValueError(f"x must be [..., {D}] on the weight's device")
+        out = t.empty(tuple(xt.shape[:-1]) + (E,), dtype=t.float32, device=xt.device)
+        with L.on(xt.device):
+            ws = L.workspace(L.load().dsv41_moe_route_workspace_size(T, D, E), xt.device)
+            L.call("dsv41_moe_logits", L.ptr(xt), T, D, L.ptr(w), E, L.ptr(out), L.ptr(ws),
+                   ws.numel(), L.stream_of(xt))
+        return out
+
+    def balance_loss(self, logits, indices, offsets=None, mask=None, grad_loss=None,
+                     dweights=None):
+        """``balance_loss`` with this router's score function, temperature and scale."""
+        return balance_loss(logits, indices, offsets, mask, self.score_func, self.gate_temp,
+                            grad_loss, dweights, self.norm_topk_prob, self.route_scale)
+
+
+def balance_loss(logits, indices, offsets=None, mask=None, score_func="sqrtsoftplus",
+                 gate_temp=1.0, grad_loss=None, dweights=None, norm_topk_prob=True,
+                 route_scale=1.0):
+    """The router's training pass: (loss [S], counts int32 [S, E], dlogits or None).
+
+    logits [..., E] float32 or bf16 (``Gate.logits``), indices [..., topk] int32 the chosen
+    experts (negative: no choice).  ``offsets`` int32 [S + 1] bounds the sequences in the
+    flattened tokens (None: one sequence of all); tokens outside them and tokens whose ``mask``
+    [...] is 0 / False count nowhere and get zero gradients.  With p the scores normalised over
+    all experts and c the sequence's choices of each expert (the counts),
+
+        loss[q] = E / (topk m^2) * sum_t sum_e c[e] p[t, e]      m = the sequence's live tokens
+
+    which is 1 for a balanced router with equal scores.  ``dlogits`` (given ``grad_loss``, a
+    number or float32 [S], or ``dweights``, float32 [..., topk]) is the gradient of
+    sum(grad_loss * loss) with the counts held constant, plus that of sum(dweights * weights)
+    for the routing weights that ``Gate`` gives for these logits and indices."""
+    t = _torch()
+    z = L.cuda_tensor(logits, "logits")
+    if z.dtype not in (t.float32, t.bfloat16):
+        raise ValueError("logits must be float32 or bfloat16")
+    dev, E = z.device, z.shape[-1]
+    if E == 0:
+        raise ValueError("logits must have at least one expert")
+    T = z.numel() // E
+
+    def arg(v, name, dtypes, rows, cols=None):
+        v = L.cuda_tensor(v, name)
+        if v.dtype not in dtypes:
+            raise ValueError(f"{name} must be {dtypes[0]}")
+        if v.device != dev:
+            raise ValueError(f"{name} is on {v.device}, logits on {dev}")
+        if v.numel() != rows * (cols or 1) or (cols and v.shape[-1] != cols):
+            raise ValueError(f"{name} has shape {tuple(v.shape)}, not one row a token"
+                             if cols else f"{name} must have {rows} values")
+        return v
+
+    topk = indices.shape[-1]
+    idx = arg(indices, "indices", (t.int32, t.int64), T, topk)
+    if idx.dtype != t.int32:
+        idx = idx.clamp(-1, 0x7FFFFFFF).to(t.int32)
+    S = 1
+    if offsets is not None:
+        S = offsets.numel() - 1
+        if S < 0:
+            raise ValueError("offsets must hold S + 1 values")
+        offsets = arg(offsets, "offsets", (t.int32,), S + 1)
+    if mask is not None:
+        mask = L.u8(arg(mask, "mask", (t.bool, t.uint8), T))
+    if grad_loss is not None:
+        if not hasattr(grad_loss, "numel"):
+            grad_loss = t.full((S,), float(grad_loss), dtype=t.float32, device=dev)
+        grad_loss = arg(grad_loss, "grad_loss", (t.float32,), S)
+    if dweights is not None:
+        dweights = arg(dweights, "dweights", (t.float32,), T, topk)
+    if score_func not in L.SCORE_FUNCS:
+        raise ValueError(f"unknown score_func {score_func!r}")
+    loss = t.empty((S,), dtype=t.float32, device=dev)
+    counts = t.empty((S, E), dtype=t.int32, device=dev)
+    dz = t.empty_like(z) if grad_loss is not None or dweights is not None else None
+    with L.on(dev):
+        nb = L.load().dsv41_moe_balance_workspace_size(T, S)
+        ws = L.workspace(nb, dev)
+        L.call("dsv41_moe_balance", L.ptr(z), L.dtype_code(z.dtype), T, E, L.ptr(idx), topk,
+               L.ptr(offsets), S, L.ptr(mask), L.SCORE_FUNCS[score_func], float(gate_temp),
+               L.ptr(grad_loss), L.ptr(dweights), int(norm_topk_prob), float(route_scale),
+               L.ptr(loss), L.ptr(counts), L.ptr(dz), L.ptr(ws), nb, L.stream_of(z))
+    return loss, counts, dz
+
+
 class _Proj:
     """One stacked projection (weight + scales)."""
 

@@ -189,6 +189,36 @@ int dsv41_gemv_affine(const void *x, int64_t M, int64_t K, const uint32_t *wq,
                       int out_dtype, void *y, void *workspace, size_t workspace_bytes,
                       void *stream);
 
+/* ---- low-rank adapters of many requests beside a shared projection (no reference
+ * counterpart: the reference runs one set of weights for everyone).  x bf16 [T, K]; a bf16
+ * [n, R, K], b bf16 [n, N, R], scaling f32 [n] (NULL: 1); ids int32 [T], the adapter of each
+ * token (negative: none).  With i = ids[t]:
+ *   h[t] = x[t] . a[i]^T          y[t] = base[t] + scaling[i] * (h[t] . b[i]^T)
+ * base (may be NULL, may be y itself) and y [T, N] of out_dtype (F32 or BF16); rows without an
+ * adapter get base (zeros when it is NULL).  h_out, if not NULL, receives h f32 [T, R] (zero
+ * rows without an adapter) for the backward pass.  Sums are fp32, h is not rounded below 16
+ * bits of mantissa, y is rounded once.  K a multiple of 8, R a multiple of 8 up to 128, n <=
+ * 8192, N any; x, a, b 16-byte aligned.  An id at or past n counts as none and raises bit 1 of
+ * dsv41_device_status.
+ *
+ * dsv41_lora_backward: from dy bf16 [T, N], x and h of the forward pass, with g[t] =
+ * scaling[i] * (dy[t] . b[i]):
+ *   dx[t] = dx_base[t] + g[t] . a[i]    da[i] = sum_t g[t]^T x[t]
+ *   db[i] = scaling[i] sum_t dy[t]^T h[t]
+ * dx_base (may be NULL, may be dx) and dx [T, K] of dx_dtype; da [n, R, K] and db [n, N, R] of
+ * grad_dtype, written whole (zeros for an adapter without tokens).  The same bits every time. */
+size_t dsv41_lora_workspace_size(int64_t T, int64_t K, int64_t N, int64_t n, int64_t R,
+                                 int backward);
+int dsv41_lora_forward(const void *x, int64_t T, int64_t K, const void *a, const void *b,
+                       int64_t n, int64_t R, int64_t N, const float *scaling, const int32_t *ids,
+                       const void *base, int out_dtype, void *y, float *h_out, void *workspace,
+                       size_t workspace_bytes, void *stream);
+int dsv41_lora_backward(const void *dy, const void *x, const float *h, const void *a,
+                        const void *b, int64_t T, int64_t K, int64_t N, int64_t n, int64_t R,
+                        const float *scaling, const int32_t *ids, const void *dx_base,
+                        int dx_dtype, void *dx, int grad_dtype, void *da, void *db,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- a8: router (deepseek_v41_mlx/moe.py:58-74; upstream
  * docs/reference/model.py:809-827).  x bf16 [T, D], w bf16 [E, D], bias f32
  * [E] (may be NULL) -> weights f32 [T, topk], indices int32 [T, topk], in
@@ -198,6 +228,34 @@ int dsv41_moe_route(const void *x, int64_t T, int64_t D, const void *gate_w, con
                     int64_t E, int topk, int score_func, float gate_temp, int norm_topk_prob,
                     float route_scale, float *weights, int32_t *indices, void *workspace,
                     size_t workspace_bytes, void *stream);
+/* The router's logits alone, before gate_temp and the score function (the products at
+ * deepseek_v41_mlx/moe.py:59): x bf16 [T, D], w bf16 [E, D] -> logits f32 [T, E].  Workspace
+ * as dsv41_moe_route. */
+int dsv41_moe_logits(const void *x, int64_t T, int64_t D, const void *gate_w, int64_t E,
+                     float *logits, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- the router's training pass (no reference counterpart: the reference only runs the
+ * router).  logits [T, E] of dtype (F32 or BF16), before gate_temp; indices int32 [T, topk],
+ * the chosen experts (negative: no choice); offsets int32 [S + 1], ascending: sequence q is
+ * tokens [offsets[q], offsets[q+1]) (NULL: one sequence of all T tokens, S = 1); mask u8 [T] or
+ * NULL (0: the token is padding).  With s the scores of dsv41_moe_route, p = s / (sum s +
+ * 1e-20), counts[q][e] the choices of expert e in sequence q and m its unmasked tokens:
+ *   loss[q] = E / (topk m^2) sum_t sum_e counts[q][e] p[t][e]     (0 where m = 0)
+ * dlogits (NULL: none) [T, E] of the logits' type receives the gradient to the logits of
+ * sum_q grad_loss[q] loss[q] (counts held constant; grad_loss f32 [S], NULL: left out) plus
+ * sum dweights * w over the unmasked tokens (dweights f32 [T, topk], NULL: left out), w the
+ * routing weights of dsv41_moe_route for these logits and indices.  Masked tokens and tokens of
+ * no sequence count nowhere, whatever they hold, and get zero gradients.  A row whose scores
+ * are all zero (logits of -inf) adds nothing and gets a zero gradient from the loss.  loss f32
+ * [S], counts int32 [S, E].  1 <= E <= 1024, 1 <= topk <= min(64, E).  An index at or past E
+ * counts as no choice and raises bit 1 of dsv41_device_status.  The same bits every time. */
+size_t dsv41_moe_balance_workspace_size(int64_t T, int64_t S);
+int dsv41_moe_balance(const void *logits, int dtype, int64_t T, int64_t E, const int32_t *indices,
+                      int topk, const int32_t *offsets, int64_t S, const uint8_t *mask,
+                      int score_func, float gate_temp, const float *grad_loss,
+                      const float *dweights, int norm_topk_prob, float route_scale, float *loss,
+                      int32_t *counts, void *dlogits, void *workspace, size_t workspace_bytes,
+                      void *stream);
 
 /* ---- a9..a11: MoE layer at decode (deepseek_v41_mlx/moe.py:105-112 with
  * SwitchGLU :101-102, ClampedSwiGLU :30-43, SharedExpert :77-93).
