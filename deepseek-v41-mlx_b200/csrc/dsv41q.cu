@@ -17,6 +17,7 @@
 #include "lora.cuh"
 #include "balance.cuh"
 
+#include <algorithm>
 #include <mutex>
 
 using namespace dsv41;
@@ -773,28 +774,176 @@ extern "C" int dsv41_moe_logits(const void *x, int64_t T, int64_t D, const void 
 namespace {
 
 int lora_check(int64_t T, int64_t K, int64_t N, int64_t n, int64_t R) {
-  DSV41_REQUIRE(T >= 0 && T <= INT32_MAX && K > 0 && K % 8 == 0 && N > 0, DSV41_ERR_BAD_SHAPE,
-                "0 <= T < 2^31, K a positive multiple of 8, N positive");
+  DSV41_REQUIRE(T >= 0 && T <= (int64_t(1) << 30) && K > 0 && K % 8 == 0 && N > 0,
+                DSV41_ERR_BAD_SHAPE, "0 <= T <= 2^30, K a positive multiple of 8, N positive");
+  DSV41_REQUIRE(K < (int64_t(1) << 31) && N < (int64_t(1) << 31), DSV41_ERR_BAD_SHAPE,
+                "K and N must be below 2^31");
   DSV41_REQUIRE(n > 0 && n <= 8192, DSV41_ERR_BAD_SHAPE, "1 <= adapters <= 8192");
   DSV41_REQUIRE(R > 0 && R <= 128 && R % 8 == 0, DSV41_ERR_UNSUPPORTED,
                 "the rank must be a multiple of 8 up to 128");
   return DSV41_OK;
 }
 
+int lora_rp(int64_t R) { return int((R + 15) / 16 * 16); }
+
+// the most tiles that T tokens on n adapters (and none) can make
+int64_t lora_max_tiles(int64_t T, int64_t n) { return T / LR_TILE + std::min(n + 1, T); }
+
+// wgrad: stages of the ring, CTAs an SM and the grid.  Three stages that fit twice into an SM
+// run as two CTAs; otherwise one CTA takes up to four.
+struct LoraWgradShape {
+  int stages, grid;
+  size_t smem;
+  uint32_t u_bytes;
+};
+LoraWgradShape lora_wgrad_shape(int64_t T, int64_t K, int64_t N, int64_t n, int64_t R,
+                                int grad_dtype) {
+  LoraWgradShape s;
+  const int Rp = lora_rp(R), ns = grad_dtype == DSV41_F32 ? 3 : 2;
+  s.u_bytes = uint32_t(Rp / 8) * LG_MN_LD;
+  const size_t stage = LG_X_BYTES + size_t(ns) * s.u_bytes;
+  const bool two = 3 * stage + 1024 <= 113 * 1024;
+  s.stages = two ? 3 : int(std::min<size_t>(4, (225 * 1024 - 1024) / stage));
+  s.smem = s.stages * stage + 1024;
+  const int64_t work = (T / LR_KB + std::min(n, T)) * (ceil_div(K, LG_COLS) + ceil_div(N, LG_COLS));
+  s.grid = int(std::max<int64_t>(1, std::min<int64_t>(work, int64_t(num_sms()) * (two ? 2 : 1))));
+  return s;
+}
+
+struct LoraWs {
+  LoraPlan plan;
+  float *h, *part;
+  bool ok;
+  size_t used;
+};
+LoraWs lora_carve(void *ws, size_t cap, int64_t T, int64_t K, int64_t N, int64_t n, int64_t R,
+                  bool backward) {
+  WsCarve c{static_cast<uint8_t *>(ws), cap, 0};
+  LoraWs w;
+  w.plan.perm = c.take<int>(T);
+  w.plan.tiles = c.take<int2>(lora_max_tiles(T, n));
+  w.plan.n_tiles = c.take<int>(1);
+  w.plan.off = c.take<int>(n + 2);
+  w.plan.stages = c.take<int>(n + 1);
+  w.h = c.take<float>(T * R);
+  w.plan.tickets = nullptr;
+  w.plan.n_tickets = 0;
+  w.part = nullptr;
+  if (backward) {
+    // the larger of the two grids (bf16 and fp32 gradients)
+    const int grid = std::max(lora_wgrad_shape(T, K, N, n, R, DSV41_BF16).grid,
+                              lora_wgrad_shape(T, K, N, n, R, DSV41_F32).grid);
+    w.plan.tickets = c.take<int>(grid);
+    w.plan.n_tickets = grid;
+    w.part = c.take<float>(size_t(2) * grid * lora_rp(R) * LG_COLS);
+  }
+  w.ok = c.ok;
+  w.used = align_up(c.off, 256);
+  return w;
+}
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsigned cluster, unsigned block,
+                           size_t smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {cluster, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+int lora_plan_launch(const int32_t *ids, int64_t T, int64_t n, const LoraPlan &plan,
+                     cudaStream_t st) {
+  const size_t smem = size_t(3) * (n + 1) * 4;
+  DSV41_LAUNCH(cudaFuncSetAttribute(k_lora_plan, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    int(smem)), "lora_plan");
+  const unsigned C = unsigned(std::min<int64_t>(8, ceil_div(T, 1024)));
+  ProfScope prof("lora_plan", st);
+  DSV41_LAUNCH(launch_cluster(k_lora_plan, C, C, 1024, smem, st, ids, int(T), int(n), plan),
+               "lora_plan");
+  return DSV41_OK;
+}
+
+template <bool WMN, bool VEC, int S>
+cudaError_t lora_shrink_go(const LoraShrink &a, unsigned clusters, unsigned C, cudaStream_t st) {
+  const size_t smem = size_t(S) * (LS_X_BYTES + a.w_bytes) + 1024;
+  cudaError_t e = cudaFuncSetAttribute(k_lora_shrink<WMN, VEC, S>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e != cudaSuccess) return e;
+  return launch_cluster(k_lora_shrink<WMN, VEC, S>, clusters * C, C, LS_THREADS, smem, st, a);
+}
+
+// The contraction is split over the CTAs of a cluster as far as the tiles leave SMs free (two
+// CTAs an SM); stages are as many as fit twice into an SM.
+template <bool WMN, bool VEC>
+int lora_shrink_launch(LoraShrink a, int64_t T, cudaStream_t st) {
+  const int64_t slots = 2 * num_sms(), nkb = ceil_div(a.K, LR_KB);
+  unsigned C = 8;
+  while (C > 1 && (ceil_div(T, LR_TILE) * C > slots || C > nkb)) C >>= 1;
+  const unsigned clusters = unsigned(std::min<int64_t>(lora_max_tiles(T, a.n), slots / C));
+  a.w_bytes = WMN ? uint32_t(a.Rp / 8) * LS_MN_LD : uint32_t(a.Rp) * 128;
+  ProfScope prof("lora_shrink", st);
+  if (a.Rp <= 32) DSV41_LAUNCH((lora_shrink_go<WMN, VEC, 5>(a, clusters, C, st)), "lora_shrink");
+  else if (a.Rp <= 64) DSV41_LAUNCH((lora_shrink_go<WMN, VEC, 4>(a, clusters, C, st)), "lora_shrink");
+  else DSV41_LAUNCH((lora_shrink_go<WMN, VEC, 3>(a, clusters, C, st)), "lora_shrink");
+  return DSV41_OK;
+}
+
+template <bool WMN, typename OT, int KJ>
+cudaError_t lora_expand_go(const LoraExpand &a, unsigned grid, cudaStream_t st) {
+  const int smem = (sizeof(OT) == 4 ? 3 : 2) * KJ * LR_TILE * 4 * 8;
+  cudaError_t e = cudaFuncSetAttribute(k_lora_expand<WMN, OT, KJ>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  k_lora_expand<WMN, OT, KJ><<<grid, 256, smem, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <bool WMN, typename OT>
+int lora_expand_launch(LoraExpand a, int64_t T, cudaStream_t st) {
+  a.ncb = int(ceil_div(a.N, 256));
+  const int64_t tiles = ceil_div(T, LR_TILE), slots = 4 * num_sms();
+  a.cpu = int(std::max<int64_t>(1, std::min<int64_t>(8, tiles * a.ncb / (4 * slots))));
+  a.vec = a.N * sizeof(OT) % 16 == 0 && aligned(a.base, 16) && aligned(a.y, 16);
+  const unsigned grid = unsigned(std::min<int64_t>(
+      lora_max_tiles(T, a.n) * ceil_div(a.ncb, a.cpu), slots));
+  ProfScope prof("lora_expand", st);
+  cudaError_t e;
+  if (a.R <= 16) e = lora_expand_go<WMN, OT, 1>(a, grid, st);
+  else if (a.R <= 32) e = lora_expand_go<WMN, OT, 2>(a, grid, st);
+  else if (a.R <= 64) e = lora_expand_go<WMN, OT, 4>(a, grid, st);
+  else e = lora_expand_go<WMN, OT, 8>(a, grid, st);
+  return cuda_status(e, "lora_expand");
+}
+
+template <typename OT, int S>
+cudaError_t lora_wgrad_go(const LoraWgrad &a, const LoraWgradShape &sh, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(k_lora_wgrad<OT, S>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, int(sh.smem));
+  if (e != cudaSuccess) return e;
+  k_lora_wgrad<OT, S><<<unsigned(sh.grid), LG_THREADS, sh.smem, st>>>(a);
+  return cudaGetLastError();
+}
+
 template <typename OT>
-void lora_expand_launch(const float *h, int64_t T, int64_t N, const void *w, int64_t wc,
-                        int64_t wr, int64_t n, int R, const int32_t *ids, const float *scaling,
-                        const void *base, void *y, cudaStream_t st) {
-  k_lora_expand<OT><<<unsigned(ceil_div(T * N, 256)), 256, 0, st>>>(
-      h, T, N, static_cast<const __nv_bfloat16 *>(w), wc, wr, n, R, ids, scaling,
-      static_cast<const OT *>(base), static_cast<OT *>(y));
+cudaError_t lora_wgrad_launch(const LoraWgrad &a, const LoraWgradShape &sh, cudaStream_t st) {
+  if (sh.stages == 4) return lora_wgrad_go<OT, 4>(a, sh, st);
+  if (sh.stages == 3) return lora_wgrad_go<OT, 3>(a, sh, st);
+  return lora_wgrad_go<OT, 2>(a, sh, st);
 }
 
 }  // namespace
 
 extern "C" size_t dsv41_lora_workspace_size(int64_t T, int64_t K, int64_t N, int64_t n, int64_t R,
                                             int backward) {
-  return align_up(size_t(T > 0 && R > 0 ? T * R : 0) * 4, 256) + 256;
+  if (T < 0 || K <= 0 || N <= 0 || n <= 0 || R <= 0) return 256;
+  return lora_carve(nullptr, ~size_t(0), T, K, N, n, R, backward != 0).used;
 }
 
 extern "C" int dsv41_lora_forward(const void *x, int64_t T, int64_t K, const void *a,
@@ -808,24 +957,23 @@ extern "C" int dsv41_lora_forward(const void *x, int64_t T, int64_t K, const voi
                 "out_dtype must be F32 or BF16");
   if (T == 0) return DSV41_OK;
   DSV41_REQUIRE(x && a && b && ids && y, DSV41_ERR_BAD_ARG, "NULL pointer");
-  DSV41_REQUIRE(aligned(x, 16) && aligned(a, 16) && aligned(b, 16), DSV41_ERR_MISALIGNED,
-                "x, a and b must be 16-byte aligned");
-  DSV41_REQUIRE(workspace && workspace_bytes >= dsv41_lora_workspace_size(T, K, N, n, R, 0),
-                DSV41_ERR_WORKSPACE, "workspace too small");
+  DSV41_REQUIRE(aligned(x, 16) && aligned(a, 16) && aligned(b, 16) && aligned(h_out, 16),
+                DSV41_ERR_MISALIGNED, "x, a, b and h_out must be 16-byte aligned");
+  LoraWs w = lora_carve(workspace, workspace_bytes, T, K, N, n, R, false);
+  DSV41_REQUIRE(workspace && w.ok, DSV41_ERR_WORKSPACE, "workspace too small");
+  DSV41_REQUIRE(aligned(workspace, 16), DSV41_ERR_MISALIGNED, "workspace must be 16-byte aligned");
   cudaStream_t st = STREAM(stream);
-  float *h = h_out ? h_out : static_cast<float *>(workspace);
-  { ProfScope prof("lora_shrink", st);
-  k_lora_shrink<<<unsigned(ceil_div(T * R * 32, 256)), 256, 0, st>>>(
-      static_cast<const __nv_bfloat16 *>(x), T, K, static_cast<const __nv_bfloat16 *>(a), K, 1, n,
-      int(R), ids, nullptr, h); }
-  DSV41_CHECK_LAUNCH("lora_shrink");
-  ProfScope prof("lora_expand", st);
-  if (out_dtype == DSV41_F32)
-    lora_expand_launch<float>(h, T, N, b, R, 1, n, int(R), ids, scaling, base, y, st);
-  else
-    lora_expand_launch<__nv_bfloat16>(h, T, N, b, R, 1, n, int(R), ids, scaling, base, y, st);
-  DSV41_CHECK_LAUNCH("lora_expand");
-  return DSV41_OK;
+  float *h = h_out ? h_out : w.h;
+  rc = lora_plan_launch(ids, T, n, w.plan, st);
+  if (rc) return rc;
+  const LoraShrink s{static_cast<const __nv_bfloat16 *>(x), K, static_cast<const __nv_bfloat16 *>(a),
+                     int(R), lora_rp(R), int(n), nullptr, h, w.plan, 0};
+  rc = lora_shrink_launch<false, true>(s, T, st);
+  if (rc) return rc;
+  const LoraExpand e{h, static_cast<const __nv_bfloat16 *>(b), N, int(R), int(n), scaling, base, y,
+                     w.plan, 0, 0, 0};
+  return out_dtype == DSV41_F32 ? lora_expand_launch<false, float>(e, T, st)
+                                : lora_expand_launch<false, __nv_bfloat16>(e, T, st);
 }
 
 extern "C" int dsv41_lora_backward(const void *dy, const void *x, const float *h, const void *a,
@@ -842,41 +990,46 @@ extern "C" int dsv41_lora_backward(const void *dy, const void *x, const float *h
   DSV41_REQUIRE(da && db, DSV41_ERR_BAD_ARG, "NULL pointer");
   DSV41_REQUIRE(T == 0 || (dy && x && h && a && b && ids && dx), DSV41_ERR_BAD_ARG,
                 "NULL pointer");
-  DSV41_REQUIRE(aligned(x, 16) && aligned(a, 16) && aligned(b, 16) && aligned(dy, 16),
-                DSV41_ERR_MISALIGNED, "dy, x, a and b must be 16-byte aligned");
-  DSV41_REQUIRE(workspace && workspace_bytes >= dsv41_lora_workspace_size(T, K, N, n, R, 1),
-                DSV41_ERR_WORKSPACE, "workspace too small");
+  DSV41_REQUIRE(aligned(x, 16) && aligned(a, 16) && aligned(b, 16) && aligned(dy, 16) &&
+                    aligned(h, 16) && aligned(da, 16) && aligned(db, 16),
+                DSV41_ERR_MISALIGNED, "dy, x, h, a, b, da and db must be 16-byte aligned");
   cudaStream_t st = STREAM(stream);
-  float *g = static_cast<float *>(workspace);
+  if (T == 0) {
+    const size_t e = grad_dtype == DSV41_F32 ? 4 : 2;
+    DSV41_LAUNCH(cudaMemsetAsync(da, 0, n * R * K * e, st), "lora memset");
+    DSV41_LAUNCH(cudaMemsetAsync(db, 0, n * R * N * e, st), "lora memset");
+    return DSV41_OK;
+  }
+  LoraWs w = lora_carve(workspace, workspace_bytes, T, K, N, n, R, true);
+  DSV41_REQUIRE(workspace && w.ok, DSV41_ERR_WORKSPACE, "workspace too small");
+  DSV41_REQUIRE(aligned(workspace, 16), DSV41_ERR_MISALIGNED, "workspace must be 16-byte aligned");
+  rc = lora_plan_launch(ids, T, n, w.plan, st);
+  if (rc) return rc;
   const __nv_bfloat16 *dyb = static_cast<const __nv_bfloat16 *>(dy),
                       *xb = static_cast<const __nv_bfloat16 *>(x);
-  if (T > 0) {
-    { ProfScope prof("lora_shrink", st);
-    k_lora_shrink<<<unsigned(ceil_div(T * R * 32, 256)), 256, 0, st>>>(
-        dyb, T, N, static_cast<const __nv_bfloat16 *>(b), 1, R, n, int(R), ids, scaling, g); }
-    DSV41_CHECK_LAUNCH("lora_shrink");
-    ProfScope prof("lora_expand", st);
-    if (dx_dtype == DSV41_F32)
-      lora_expand_launch<float>(g, T, K, a, 1, K, n, int(R), ids, nullptr, dx_base, dx, st);
-    else
-      lora_expand_launch<__nv_bfloat16>(g, T, K, a, 1, K, n, int(R), ids, nullptr, dx_base, dx, st);
-    DSV41_CHECK_LAUNCH("lora_expand");
-  }
+  const LoraShrink s{dyb, N, static_cast<const __nv_bfloat16 *>(b), int(R), lora_rp(R), int(n),
+                     scaling, w.h, w.plan, 0};
+  rc = N % 8 == 0 ? lora_shrink_launch<true, true>(s, T, st) : lora_shrink_launch<true, false>(s, T, st);
+  if (rc) return rc;
+  const LoraExpand e{w.h, static_cast<const __nv_bfloat16 *>(a), K, int(R), int(n), nullptr, dx_base,
+                     dx, w.plan, 0, 0, 0};
+  rc = dx_dtype == DSV41_F32 ? lora_expand_launch<true, float>(e, T, st)
+                             : lora_expand_launch<true, __nv_bfloat16>(e, T, st);
+  if (rc) return rc;
+  const LoraWgradShape sh = lora_wgrad_shape(T, K, N, n, R, grad_dtype);
+  LoraWgrad g{};
+  g.side[0] = LoraGradSide{xb, w.h, K, int(ceil_div(K, LG_COLS)), nullptr, da, 1, 1};
+  g.side[1] = LoraGradSide{dyb, h, N, int(ceil_div(N, LG_COLS)), scaling, db, 0, N % 8 == 0};
+  g.R = int(R);
+  g.Rp = lora_rp(R);
+  g.n = int(n);
+  g.plan = w.plan;
+  g.part = w.part;
+  g.u_bytes = sh.u_bytes;
   ProfScope prof("lora_wgrad", st);
-  const unsigned ba = unsigned(ceil_div(n * R * K, 256)), bb = unsigned(ceil_div(n * R * N, 256));
-  if (grad_dtype == DSV41_F32) {
-    k_lora_wgrad<float><<<ba, 256, 0, st>>>(g, xb, T, K, n, int(R), ids, nullptr, K, 1,
-                                            static_cast<float *>(da));
-    k_lora_wgrad<float><<<bb, 256, 0, st>>>(h, dyb, T, N, n, int(R), ids, scaling, 1, R,
-                                            static_cast<float *>(db));
-  } else {
-    k_lora_wgrad<__nv_bfloat16><<<ba, 256, 0, st>>>(g, xb, T, K, n, int(R), ids, nullptr, K, 1,
-                                                    static_cast<__nv_bfloat16 *>(da));
-    k_lora_wgrad<__nv_bfloat16><<<bb, 256, 0, st>>>(h, dyb, T, N, n, int(R), ids, scaling, 1, R,
-                                                    static_cast<__nv_bfloat16 *>(db));
-  }
-  DSV41_CHECK_LAUNCH("lora_wgrad");
-  return DSV41_OK;
+  const cudaError_t ge = grad_dtype == DSV41_F32 ? lora_wgrad_launch<float>(g, sh, st)
+                                                 : lora_wgrad_launch<__nv_bfloat16>(g, sh, st);
+  return cuda_status(ge, "lora_wgrad");
 }
 
 // ======================================================================= MoE decode

@@ -198,7 +198,7 @@ int dsv41_gemv_affine(const void *x, int64_t M, int64_t K, const uint32_t *wq,
  * adapter get base (zeros when it is NULL).  h_out, if not NULL, receives h f32 [T, R] (zero
  * rows without an adapter) for the backward pass.  Sums are fp32, h is not rounded below 16
  * bits of mantissa, y is rounded once.  K a multiple of 8, R a multiple of 8 up to 128, n <=
- * 8192, N any; x, a, b 16-byte aligned.  An id at or past n counts as none and raises bit 1 of
+ * 8192, T <= 2^30, N any; every tensor but y and the base 16-byte aligned, and the workspace.  An id at or past n counts as none and raises bit 1 of
  * dsv41_device_status.
  *
  * dsv41_lora_backward: from dy bf16 [T, N], x and h of the forward pass, with g[t] =
