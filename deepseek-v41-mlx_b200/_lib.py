@@ -78,7 +78,7 @@ PROTOTYPES = {
     "dsv41_moe_route": (_I, [_P, _I64, _I64, _P, _P, _I64, _I, _I, _F, _I, _F, _P, _P, _P, _SZ,
                              _P]),
     "dsv41_moe_logits": (_I, [_P, _I64, _I64, _P, _I64, _P, _P, _SZ, _P]),
-    "dsv41_moe_balance_workspace_size": (_SZ, [_I64, _I64]),
+    "dsv41_moe_balance_workspace_size": (_SZ, [_I64, _I64, _I64]),
     "dsv41_moe_balance": (_I, [_P, _I, _I64, _I64, _P, _I, _P, _I64, _P, _I, _F, _P, _P, _I, _F,
                                _P, _P, _P, _P, _SZ, _P]),
     "dsv41_lora_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I]),
@@ -183,9 +183,15 @@ def call(name: str, *args):
 
 # ---------------------------------------------------------------- torch glue --
 
+_torch = None
+
+
 def torch():
-    import torch as _t
-    return _t
+    global _torch
+    if _torch is None:
+        import torch as _t
+        _torch = _t
+    return _torch
 
 
 def as_tensor(a):
@@ -210,6 +216,10 @@ def ptr(t) -> int:
 
 
 def stream_of(t) -> int:
+    """The current stream of t's device, as an integer."""
+    raw = getattr(torch()._C, "_cuda_getCurrentRawStream", None)   # no Stream object is built
+    if raw is not None:
+        return raw(t.device.index)
     return torch().cuda.current_stream(t.device).cuda_stream
 
 

@@ -18,6 +18,7 @@
 #include "balance.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 
 using namespace dsv41;
@@ -327,6 +328,53 @@ struct WsCarve {
     return p;
   }
 };
+
+// Allow a kernel its dynamic shared memory, once per kernel, size and device: the attribute call
+// costs the host about as much as a launch.  (The default of 48 KB covers the static part too, so
+// that smaller requests need no call.)
+template <typename... KArgs>
+cudaError_t max_dynamic_smem(void (*kernel)(KArgs...), size_t bytes) {
+  if (bytes <= 40 * 1024) return cudaSuccess;
+  struct Entry {
+    std::atomic<const void *> fn;
+    std::atomic<size_t> bytes[16];
+  };
+  static Entry seen[64];                 // one table per kernel signature
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const void *f = reinterpret_cast<const void *>(kernel);
+  Entry *slot = nullptr;
+  if (dev < 16)
+    for (Entry &s : seen) {
+      const void *have = s.fn.load(std::memory_order_acquire);
+      if (!have && s.fn.compare_exchange_strong(have, f)) have = f;
+      if (have == f) {
+        slot = &s;
+        break;
+      }
+    }
+  if (slot && slot->bytes[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+  e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  if (e == cudaSuccess && slot) slot->bytes[dev].store(bytes, std::memory_order_release);
+  return e;
+}
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsigned cluster, unsigned block,
+                           size_t smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {cluster, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 constexpr int QG_MAX_SPLIT = 16;
 
@@ -680,8 +728,57 @@ extern "C" int dsv41_moe_route(const void *x, int64_t T, int64_t D, const void *
                     STREAM(stream));
 }
 
-extern "C" size_t dsv41_moe_balance_workspace_size(int64_t T, int64_t S) {
-  return align_up(size_t(S > 0 ? S : 0) * 4, 256) + align_up(size_t(T > 0 ? T : 0) * 4, 256) + 256;
+namespace {
+
+constexpr int64_t BL_SMALL_T = 512;
+
+// One launch does the whole pass (k_balance_small): no workspace.
+bool balance_is_small(int64_t T, int64_t E, int64_t S) {
+  return T > 0 && T <= BL_SMALL_T && S * E <= BL_SMALL_INTS;
+}
+// Tokens of a warp's run: two CTAs an SM share the tokens in one wave.
+int64_t balance_run(int64_t T) { return std::max<int64_t>(1, ceil_div(T, 2 * num_sms() * BL_WARPS)); }
+
+struct BalShape {
+  unsigned grid, cluster;      // cluster: 0 for the several-launch form
+  size_t smem;
+};
+
+template <typename IT, int NV, int VEC, bool GRAD>
+cudaError_t balance_go(const BalArgs &p, const BalShape &sh, cudaStream_t st) {
+  if (sh.cluster) {
+    cudaError_t e = max_dynamic_smem(k_balance_small<IT, NV, VEC, GRAD>, sh.smem);
+    if (e != cudaSuccess) return e;
+    return launch_cluster(k_balance_small<IT, NV, VEC, GRAD>, sh.grid, sh.cluster, 32 * BL_WARPS,
+                          sh.smem, st, p);
+  }
+  k_balance<IT, NV, VEC, GRAD><<<sh.grid, 32 * BL_WARPS, sh.smem, st>>>(p);
+  return cudaGetLastError();
+}
+template <typename IT, int NV, int VEC>
+cudaError_t balance_grad(const BalArgs &p, const BalShape &sh, cudaStream_t st) {
+  return p.dlogits ? balance_go<IT, NV, VEC, true>(p, sh, st) : balance_go<IT, NV, VEC, false>(p, sh, st);
+}
+// Rows of E % 4 == 0 values move in pieces of four, others one by one.
+template <typename IT>
+cudaError_t balance_rows(const BalArgs &p, const BalShape &sh, cudaStream_t st) {
+  const bool vec = p.E % 4 == 0 && aligned(p.logits, 4 * sizeof(IT)) && aligned(p.dlogits, 4 * sizeof(IT));
+  if (!vec)
+    return p.E <= 256 ? balance_grad<IT, 8, 1>(p, sh, st) : balance_grad<IT, 32, 1>(p, sh, st);
+  switch ((p.E + 127) / 128) {
+    case 1: return balance_grad<IT, 1, 4>(p, sh, st);
+    case 2: return balance_grad<IT, 2, 4>(p, sh, st);
+    case 3: return balance_grad<IT, 3, 4>(p, sh, st);
+    case 4: return balance_grad<IT, 4, 4>(p, sh, st);
+    default: return balance_grad<IT, 8, 4>(p, sh, st);
+  }
+}
+
+}  // namespace
+
+extern "C" size_t dsv41_moe_balance_workspace_size(int64_t T, int64_t E, int64_t S) {
+  if (T < 0 || E <= 0 || S < 0 || balance_is_small(T, E, S)) return 0;
+  return align_up(size_t(S + 1) * 4, 256) + size_t(ceil_div(T, balance_run(T)) + S) * 8 + 256;
 }
 
 extern "C" int dsv41_moe_balance(const void *logits, int dtype, int64_t T, int64_t E,
@@ -693,9 +790,9 @@ extern "C" int dsv41_moe_balance(const void *logits, int dtype, int64_t T, int64
                                  size_t workspace_bytes, void *stream) {
   DSV41_REQUIRE(dtype == DSV41_F32 || dtype == DSV41_BF16, DSV41_ERR_BAD_DTYPE,
                 "logits must be F32 or BF16");
-  DSV41_REQUIRE(T >= 0 && T <= INT32_MAX, DSV41_ERR_BAD_SHAPE, "0 <= T < 2^31");
+  DSV41_REQUIRE(T >= 0 && T <= (int64_t(1) << 30), DSV41_ERR_BAD_SHAPE, "0 <= T <= 2^30");
   DSV41_REQUIRE(E > 0 && E <= 1024, DSV41_ERR_BAD_SHAPE, "1 <= E <= 1024");
-  DSV41_REQUIRE(S >= 0 && S < INT32_MAX, DSV41_ERR_BAD_SHAPE, "0 <= S < 2^31 - 1");
+  DSV41_REQUIRE(S >= 0 && S <= (int64_t(1) << 30), DSV41_ERR_BAD_SHAPE, "0 <= S <= 2^30");
   DSV41_REQUIRE(topk >= 1 && topk <= 64 && topk <= E, DSV41_ERR_BAD_ARG, "1 <= topk <= min(64, E)");
   DSV41_REQUIRE(score_func >= 0 && score_func <= 2, DSV41_ERR_BAD_ARG, "unknown score_func");
   DSV41_REQUIRE(gate_temp > 0.0f, DSV41_ERR_BAD_ARG, "gate_temp must be positive");
@@ -704,41 +801,48 @@ extern "C" int dsv41_moe_balance(const void *logits, int dtype, int64_t T, int64
                 "grad_loss and dweights need dlogits");
   DSV41_REQUIRE(S == 0 || (loss && counts), DSV41_ERR_BAD_ARG, "NULL pointer");
   DSV41_REQUIRE(T == 0 || (logits && indices), DSV41_ERR_BAD_ARG, "NULL pointer");
-  DSV41_REQUIRE(workspace && workspace_bytes >= dsv41_moe_balance_workspace_size(T, S),
-                DSV41_ERR_WORKSPACE, "workspace too small");
-  WsCarve ws{static_cast<uint8_t *>(workspace), workspace_bytes, 0};
-  int *live = ws.take<int>(S);
-  float *tok_dot = ws.take<float>(T);
   cudaStream_t st = STREAM(stream);
-  if (S > 0) {
-    DSV41_LAUNCH(cudaMemsetAsync(live, 0, S * 4, st), "balance memset");
-    DSV41_LAUNCH(cudaMemsetAsync(counts, 0, S * E * 4, st), "balance memset");
+  if (T == 0) {
+    if (S > 0) {
+      DSV41_LAUNCH(cudaMemsetAsync(loss, 0, S * 4, st), "balance memset");
+      DSV41_LAUNCH(cudaMemsetAsync(counts, 0, S * E * 4, st), "balance memset");
+    }
+    return DSV41_OK;
   }
-  if (T > 0) {
-    { ProfScope prof("balance_count", st);
-    k_balance_count<<<unsigned(ceil_div(T, 256)), 256, 0, st>>>(indices, T, topk, int(E), offsets,
-                                                                int(S), mask, counts, live); }
-    DSV41_CHECK_LAUNCH("balance_count");
-    ProfScope prof("balance_row", st);
-    const unsigned th = unsigned(ceil_div(E, 32) * 32);
-    if (dtype == DSV41_F32)
-      k_balance_row<float><<<unsigned(T), th, 0, st>>>(
-          static_cast<const float *>(logits), T, int(E), indices, topk, offsets, int(S), mask,
-          score_func, gate_temp, grad_loss, dweights, norm_topk_prob, route_scale, counts, live,
-          tok_dot, static_cast<float *>(dlogits));
-    else
-      k_balance_row<__nv_bfloat16><<<unsigned(T), th, 0, st>>>(
-          static_cast<const __nv_bfloat16 *>(logits), T, int(E), indices, topk, offsets, int(S),
-          mask, score_func, gate_temp, grad_loss, dweights, norm_topk_prob, route_scale, counts,
-          live, tok_dot, static_cast<__nv_bfloat16 *>(dlogits));
-    DSV41_CHECK_LAUNCH("balance_row");
+  BalArgs p{logits, T, int(E), topk, int(S), score_func, indices, offsets, mask, 1.0f / gate_temp,
+            grad_loss, dweights, norm_topk_prob, route_scale, loss, counts, dlogits, nullptr,
+            nullptr, 0};
+  BalShape sh{};
+  const size_t add = dweights ? size_t(BL_WARPS) * E * 4 : 0;
+  if (balance_is_small(T, E, S)) {
+    sh.cluster = sh.grid = unsigned(std::min<int64_t>(8, ceil_div(T, BL_WARPS)));
+    sh.smem = size_t(S * E + S + T) * 4 + add;
+  } else {
+    DSV41_REQUIRE(workspace && workspace_bytes >= dsv41_moe_balance_workspace_size(T, E, S),
+                  DSV41_ERR_WORKSPACE, "workspace too small");
+    DSV41_REQUIRE(aligned(workspace, 8), DSV41_ERR_MISALIGNED, "workspace must be 8-byte aligned");
+    WsCarve ws{static_cast<uint8_t *>(workspace), workspace_bytes, 0};
+    p.live = ws.take<int>(S + 1);
+    p.run = int(balance_run(T));
+    p.part = ws.take<double>(ceil_div(T, p.run) + S);
+    sh.grid = unsigned(ceil_div(ceil_div(T, p.run), BL_WARPS));
+    sh.smem = add;
+    const int64_t n = S * E + S;
+    ProfScope prof("balance_count", st);
+    if (n <= BL_COUNT_INTS) {
+      DSV41_LAUNCH(max_dynamic_smem(k_balance_count, n * 4), "balance_count");
+      DSV41_LAUNCH(launch_cluster(k_balance_count, 8, 8, 1024, size_t(n) * 4, st, p),
+                   "balance_count");
+    } else {
+      DSV41_LAUNCH(cudaMemsetAsync(p.live, 0, (S + 1) * 4, st), "balance memset");
+      DSV41_LAUNCH(cudaMemsetAsync(counts, 0, S * E * 4, st), "balance memset");
+      k_balance_count_global<<<unsigned(ceil_div(T, 256)), 256, 0, st>>>(p);
+      DSV41_CHECK_LAUNCH("balance_count");
+    }
   }
-  if (S > 0) {
-    ProfScope prof("balance_loss", st);
-    k_balance_loss<<<unsigned(S), 256, 0, st>>>(tok_dot, T, int(E), topk, offsets, live, loss);
-    DSV41_CHECK_LAUNCH("balance_loss");
-  }
-  return DSV41_OK;
+  ProfScope prof("balance", st);
+  return cuda_status(dtype == DSV41_F32 ? balance_rows<float>(p, sh, st)
+                                        : balance_rows<__nv_bfloat16>(p, sh, st), "balance");
 }
 
 extern "C" int dsv41_moe_logits(const void *x, int64_t T, int64_t D, const void *gate_w, int64_t E,
@@ -842,27 +946,10 @@ LoraWs lora_carve(void *ws, size_t cap, int64_t T, int64_t K, int64_t N, int64_t
   return w;
 }
 
-template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsigned cluster, unsigned block,
-                           size_t smem, cudaStream_t st, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim = {cluster, 1, 1};
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 int lora_plan_launch(const int32_t *ids, int64_t T, int64_t n, const LoraPlan &plan,
                      cudaStream_t st) {
   const size_t smem = size_t(3) * (n + 1) * 4;
-  DSV41_LAUNCH(cudaFuncSetAttribute(k_lora_plan, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    int(smem)), "lora_plan");
+  DSV41_LAUNCH(max_dynamic_smem(k_lora_plan, smem), "lora_plan");
   const unsigned C = unsigned(std::min<int64_t>(8, ceil_div(T, 1024)));
   ProfScope prof("lora_plan", st);
   DSV41_LAUNCH(launch_cluster(k_lora_plan, C, C, 1024, smem, st, ids, int(T), int(n), plan),
@@ -870,11 +957,24 @@ int lora_plan_launch(const int32_t *ids, int64_t T, int64_t n, const LoraPlan &p
   return DSV41_OK;
 }
 
+// Up to this many tokens a forward call is one launch (k_lora_decode).
+constexpr int64_t LORA_DECODE_T = 64;
+
+template <typename OT>
+cudaError_t lora_decode_launch(const LoraDecode &p, int64_t T, cudaStream_t st) {
+  const unsigned C = 8;
+  const unsigned grid = unsigned(T) * C;
+  if (p.R <= 8) return launch_cluster(k_lora_decode<OT, 1, 1>, grid, C, LD_THREADS, 0, st, p);
+  if (p.R <= 16) return launch_cluster(k_lora_decode<OT, 2, 2>, grid, C, LD_THREADS, 0, st, p);
+  if (p.R <= 32) return launch_cluster(k_lora_decode<OT, 4, 4>, grid, C, LD_THREADS, 0, st, p);
+  if (p.R <= 64) return launch_cluster(k_lora_decode<OT, 8, 8>, grid, C, LD_THREADS, 0, st, p);
+  return launch_cluster(k_lora_decode<OT, 16, 16>, grid, C, LD_THREADS, 0, st, p);
+}
+
 template <bool WMN, bool VEC, int S>
 cudaError_t lora_shrink_go(const LoraShrink &a, unsigned clusters, unsigned C, cudaStream_t st) {
   const size_t smem = size_t(S) * (LS_X_BYTES + a.w_bytes) + 1024;
-  cudaError_t e = cudaFuncSetAttribute(k_lora_shrink<WMN, VEC, S>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  cudaError_t e = max_dynamic_smem(k_lora_shrink<WMN, VEC, S>, smem);
   if (e != cudaSuccess) return e;
   return launch_cluster(k_lora_shrink<WMN, VEC, S>, clusters * C, C, LS_THREADS, smem, st, a);
 }
@@ -898,8 +998,7 @@ int lora_shrink_launch(LoraShrink a, int64_t T, cudaStream_t st) {
 template <bool WMN, typename OT, int KJ>
 cudaError_t lora_expand_go(const LoraExpand &a, unsigned grid, cudaStream_t st) {
   const int smem = (sizeof(OT) == 4 ? 3 : 2) * KJ * LR_TILE * 4 * 8;
-  cudaError_t e = cudaFuncSetAttribute(k_lora_expand<WMN, OT, KJ>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = max_dynamic_smem(k_lora_expand<WMN, OT, KJ>, smem);
   if (e != cudaSuccess) return e;
   k_lora_expand<WMN, OT, KJ><<<grid, 256, smem, st>>>(a);
   return cudaGetLastError();
@@ -924,8 +1023,7 @@ int lora_expand_launch(LoraExpand a, int64_t T, cudaStream_t st) {
 
 template <typename OT, int S>
 cudaError_t lora_wgrad_go(const LoraWgrad &a, const LoraWgradShape &sh, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(k_lora_wgrad<OT, S>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, int(sh.smem));
+  cudaError_t e = max_dynamic_smem(k_lora_wgrad<OT, S>, sh.smem);
   if (e != cudaSuccess) return e;
   k_lora_wgrad<OT, S><<<unsigned(sh.grid), LG_THREADS, sh.smem, st>>>(a);
   return cudaGetLastError();
@@ -942,7 +1040,8 @@ cudaError_t lora_wgrad_launch(const LoraWgrad &a, const LoraWgradShape &sh, cuda
 
 extern "C" size_t dsv41_lora_workspace_size(int64_t T, int64_t K, int64_t N, int64_t n, int64_t R,
                                             int backward) {
-  if (T < 0 || K <= 0 || N <= 0 || n <= 0 || R <= 0) return 256;
+  if (T < 0 || K <= 0 || N <= 0 || n <= 0 || R <= 0) return 0;
+  if (T == 0 || (!backward && T <= LORA_DECODE_T)) return 0;
   return lora_carve(nullptr, ~size_t(0), T, K, N, n, R, backward != 0).used;
 }
 
@@ -959,6 +1058,15 @@ extern "C" int dsv41_lora_forward(const void *x, int64_t T, int64_t K, const voi
   DSV41_REQUIRE(x && a && b && ids && y, DSV41_ERR_BAD_ARG, "NULL pointer");
   DSV41_REQUIRE(aligned(x, 16) && aligned(a, 16) && aligned(b, 16) && aligned(h_out, 16),
                 DSV41_ERR_MISALIGNED, "x, a, b and h_out must be 16-byte aligned");
+  if (T <= LORA_DECODE_T) {
+    const LoraDecode d{static_cast<const __nv_bfloat16 *>(x), static_cast<const __nv_bfloat16 *>(a),
+                       static_cast<const __nv_bfloat16 *>(b), K, N, int(R), int(n), scaling, ids,
+                       base, y, h_out};
+    ProfScope prof("lora_decode", STREAM(stream));
+    return cuda_status(out_dtype == DSV41_F32 ? lora_decode_launch<float>(d, T, STREAM(stream))
+                                              : lora_decode_launch<__nv_bfloat16>(d, T, STREAM(stream)),
+                       "lora_decode");
+  }
   LoraWs w = lora_carve(workspace, workspace_bytes, T, K, N, n, R, false);
   DSV41_REQUIRE(workspace && w.ok, DSV41_ERR_WORKSPACE, "workspace too small");
   DSV41_REQUIRE(aligned(workspace, 16), DSV41_ERR_MISALIGNED, "workspace must be 16-byte aligned");

@@ -30,12 +30,6 @@ namespace dsv41 {
 constexpr int LR_TILE = 128;        // token rows of a tile
 constexpr int LR_KB = 64;           // contraction length of a stage
 
-__device__ __forceinline__ uint32_t cluster_nctas() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-
 // ------------------------------------------------------------------ plan
 struct LoraPlan {
   int *perm;       // [T] token of sorted position p
@@ -79,12 +73,6 @@ __device__ __forceinline__ void block_scan3(int (&v)[3], int (&tot)[3], int (*ws
     const int before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
     if (warp) v[i] += before;
   }
-}
-
-__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
 }
 
 // One cluster of 1024-thread CTAs, each on a contiguous slice of the tokens: histogram in
@@ -401,6 +389,122 @@ __global__ void __launch_bounds__(LS_THREADS, 2) k_lora_shrink(const LoraShrink 
     tc_fence_after();
     tmem_dealloc(tmem, cols);
   }
+}
+
+// ------------------------------------------------------------------ few tokens
+struct LoraDecode {
+  const __nv_bfloat16 *x, *a, *b;
+  int64_t K, N;
+  int R, n;
+  const float *scaling;
+  const int32_t *ids;
+  const void *base;
+  void *y;
+  float *h;                    // NULL: not kept
+};
+
+// 8 bf16 products added to acc
+__device__ __forceinline__ float dot8(uint4 u, uint4 v, float acc) {
+  const uint32_t a[4] = {u.x, u.y, u.z, u.w}, b[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    acc = fmaf(__uint_as_float(a[i] << 16), __uint_as_float(b[i] << 16), acc);
+    acc = fmaf(__uint_as_float(a[i] & 0xFFFF0000u), __uint_as_float(b[i] & 0xFFFF0000u), acc);
+  }
+  return acc;
+}
+
+constexpr int LD_THREADS = 256, LD_WARPS = 8;
+
+// Both products of a token in one launch, no plan: a cluster per token.  Each CTA takes a slice
+// of K (its warps R / 8 ranks each), the partial h meet in distributed shared memory in rank
+// order, then each CTA takes a slice of the columns, a row of B per group of LPR lanes.  The
+// first rows of B are requested before the cluster meets.  Bound by the latency of one pass
+// over an adapter (360 KB at K 7168, N 4096, R 16), which tokens on the same adapter find in L2.
+// RW: ranks a warp; LPR: lanes a row of B, the power of two at or above R / 8.
+template <typename OT, int RW, int LPR>
+__global__ void __launch_bounds__(LD_THREADS) k_lora_decode(const LoraDecode p) {
+  constexpr int COLS = LD_THREADS / LPR;            // columns a pass
+  constexpr int PF = 8;                             // passes requested ahead
+  __shared__ float part[LD_WARPS * RW];
+  __shared__ float hs[LD_WARPS * RW];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int C = int(cluster_nctas()), rank = int(cluster_rank());
+  const int64_t t = cluster_id_x();
+  const OT *base = static_cast<const OT *>(p.base);
+  OT *y = static_cast<OT *>(p.y) + t * p.N;
+  const int i = lora_bin(p.ids[t], p.n);
+  const int64_t c0 = p.N * rank / C, c1 = p.N * (rank + 1) / C;
+  if (i == p.n) {                                   // uniform over the cluster
+    for (int64_t c = c0 + tid; c < c1; c += LD_THREADS)
+      y[c] = base ? base[t * p.N + c] : OT(0.0f);
+    if (p.h && rank == 0)
+      for (int r = tid; r < p.R; r += LD_THREADS) p.h[t * p.R + r] = 0.0f;
+    return;
+  }
+  const uint4 z = make_uint4(0, 0, 0, 0);
+  const int ln = tid % LPR, cg = tid / LPR;
+  const __nv_bfloat16 *bi = p.b + int64_t(i) * p.N * p.R + ln * 8;
+  uint4 bv[PF];
+#pragma unroll
+  for (int u = 0; u < PF; ++u) {
+    const int64_t c = c0 + u * COLS + cg;
+    bv[u] = (c < c1 && ln * 8 < p.R) ? __ldg(reinterpret_cast<const uint4 *>(bi + c * p.R)) : z;
+  }
+  {
+    const int64_t nk = p.K >> 3, k0 = nk * rank / C, k1 = nk * (rank + 1) / C;
+    const uint4 *xr = reinterpret_cast<const uint4 *>(p.x + t * p.K);
+    const uint4 *ar = reinterpret_cast<const uint4 *>(p.a + int64_t(i) * p.R * p.K);
+    float acc[RW] = {};
+#pragma unroll 2
+    for (int64_t k = k0 + lane; k < k1; k += 32) {
+      const uint4 xv = __ldg(xr + k);
+      uint4 av[RW];
+#pragma unroll
+      for (int r = 0; r < RW; ++r)
+        av[r] = warp * RW + r < p.R ? __ldg(ar + (warp * RW + r) * nk + k) : z;
+#pragma unroll
+      for (int r = 0; r < RW; ++r) acc[r] = dot8(xv, av[r], acc[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
+      if (lane == 0) part[warp * RW + r] = acc[r];
+    }
+  }
+  cluster_sync();
+  if (tid < LD_WARPS * RW) {
+    float s = 0.0f;
+    for (int q = 0; q < C; ++q)
+      s += __int_as_float(ld_cluster_s32(mapa_rank(part + tid, q)));
+    if (p.h && rank == 0 && tid < p.R) p.h[t * p.R + tid] = s;
+    hs[tid] = tid < p.R ? s * (p.scaling ? p.scaling[i] : 1.0f) : 0.0f;
+  }
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");      // part has been read
+  float hv[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) hv[e] = ln * 8 + e < p.R ? hs[ln * 8 + e] : 0.0f;
+  for (int64_t cb = c0; cb < c1; cb += PF * COLS) {
+#pragma unroll
+    for (int u = 0; u < PF; ++u) {
+      const int64_t c = cb + u * COLS + cg;
+      const uint32_t w[4] = {bv[u].x, bv[u].y, bv[u].z, bv[u].w};
+      float s = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s = fmaf(hv[2 * e], __uint_as_float(w[e] << 16), s);
+        s = fmaf(hv[2 * e + 1], __uint_as_float(w[e] & 0xFFFF0000u), s);
+      }
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (ln == 0 && c < c1) y[c] = OT((base ? float(base[t * p.N + c]) : 0.0f) + s);
+      const int64_t cn = c + PF * COLS;
+      bv[u] = (cn < c1 && ln * 8 < p.R) ? __ldg(reinterpret_cast<const uint4 *>(bi + cn * p.R)) : z;
+    }
+  }
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // ------------------------------------------------------------------ expand

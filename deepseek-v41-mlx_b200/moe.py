@@ -135,44 +135,44 @@ def balance_loss(logits, indices, offsets=None, mask=None, score_func="sqrtsoftp
         raise ValueError("logits must have at least one expert")
     T = z.numel() // E
 
-    def arg(v, name, dtypes, rows, cols=None):
+    def arg(v, name, dtype, count, cols=0):
         v = L.cuda_tensor(v, name)
-        if v.dtype not in dtypes:
-            raise ValueError(f"{name} must be {dtypes[0]}")
+        if v.dtype != dtype:
+            raise ValueError(f"{name} must be {dtype}, not {v.dtype}")
         if v.device != dev:
             raise ValueError(f"{name} is on {v.device}, logits on {dev}")
-        if v.numel() != rows * (cols or 1) or (cols and v.shape[-1] != cols):
-            raise ValueError(f"{name} has shape {tuple(v.shape)}, not one row a token"
-                             if cols else f"{name} must have {rows} values")
+        if v.numel() != count or (cols and v.shape[-1] != cols):
+            raise ValueError(f"{name} has shape {tuple(v.shape)} for {T} tokens")
         return v
 
     topk = indices.shape[-1]
-    idx = arg(indices, "indices", (t.int32, t.int64), T, topk)
-    if idx.dtype != t.int32:
-        idx = idx.clamp(-1, 0x7FFFFFFF).to(t.int32)
+    if indices.dtype == t.int64:         # ids that int32 cannot hold are no expert's
+        indices = indices.clamp(-1, 0x7FFFFFFF).to(t.int32)
+    idx = arg(indices, "indices", t.int32, T * topk, topk)
     S = 1
     if offsets is not None:
         S = offsets.numel() - 1
         if S < 0:
             raise ValueError("offsets must hold S + 1 values")
-        offsets = arg(offsets, "offsets", (t.int32,), S + 1)
+        offsets = arg(offsets, "offsets", t.int32, S + 1)
     if mask is not None:
-        mask = L.u8(arg(mask, "mask", (t.bool, t.uint8), T))
+        mask = arg(mask, "mask", t.bool if mask.dtype == t.bool else t.uint8, T)
     if grad_loss is not None:
         if not hasattr(grad_loss, "numel"):
             grad_loss = t.full((S,), float(grad_loss), dtype=t.float32, device=dev)
-        grad_loss = arg(grad_loss, "grad_loss", (t.float32,), S)
+        grad_loss = arg(grad_loss, "grad_loss", t.float32, S)
     if dweights is not None:
-        dweights = arg(dweights, "dweights", (t.float32,), T, topk)
+        dweights = arg(dweights, "dweights", t.float32, T * topk, topk)
     if score_func not in L.SCORE_FUNCS:
         raise ValueError(f"unknown score_func {score_func!r}")
     loss = t.empty((S,), dtype=t.float32, device=dev)
     counts = t.empty((S, E), dtype=t.int32, device=dev)
     dz = t.empty_like(z) if grad_loss is not None or dweights is not None else None
     with L.on(dev):
-        nb = L.load().dsv41_moe_balance_workspace_size(T, S)
-        ws = L.workspace(nb, dev)
-        L.call("dsv41_moe_balance", L.ptr(z), L.dtype_code(z.dtype), T, E, L.ptr(idx), topk,
+        nb = L.load().dsv41_moe_balance_workspace_size(T, E, S)
+        ws = L.workspace(nb, dev) if nb else None
+        code = L.F32 if z.dtype == t.float32 else L.BF16
+        L.call("dsv41_moe_balance", L.ptr(z), code, T, E, L.ptr(idx), topk,
                L.ptr(offsets), S, L.ptr(mask), L.SCORE_FUNCS[score_func], float(gate_temp),
                L.ptr(grad_loss), L.ptr(dweights), int(norm_topk_prob), float(route_scale),
                L.ptr(loss), L.ptr(counts), L.ptr(dz), L.ptr(ws), nb, L.stream_of(z))

@@ -206,7 +206,8 @@ int dsv41_gemv_affine(const void *x, int64_t M, int64_t K, const uint32_t *wq,
  *   dx[t] = dx_base[t] + g[t] . a[i]    da[i] = sum_t g[t]^T x[t]
  *   db[i] = scaling[i] sum_t dy[t]^T h[t]
  * dx_base (may be NULL, may be dx) and dx [T, K] of dx_dtype; da [n, R, K] and db [n, N, R] of
- * grad_dtype, written whole (zeros for an adapter without tokens).  The same bits every time. */
+ * grad_dtype, written whole (zeros for an adapter without tokens).  The same bits every time.
+ * The workspace may be NULL where its size is 0 (forward calls of few tokens: one launch). */
 size_t dsv41_lora_workspace_size(int64_t T, int64_t K, int64_t N, int64_t n, int64_t R,
                                  int backward);
 int dsv41_lora_forward(const void *x, int64_t T, int64_t K, const void *a, const void *b,
@@ -248,8 +249,9 @@ int dsv41_moe_logits(const void *x, int64_t T, int64_t D, const void *gate_w, in
  * no sequence count nowhere, whatever they hold, and get zero gradients.  A row whose scores
  * are all zero (logits of -inf) adds nothing and gets a zero gradient from the loss.  loss f32
  * [S], counts int32 [S, E].  1 <= E <= 1024, 1 <= topk <= min(64, E).  An index at or past E
- * counts as no choice and raises bit 1 of dsv41_device_status.  The same bits every time. */
-size_t dsv41_moe_balance_workspace_size(int64_t T, int64_t S);
+ * counts as no choice and raises bit 1 of dsv41_device_status.  The same bits every time.  T, S <= 2^30.
+ * The workspace (8-byte aligned) may be NULL where its size is 0. */
+size_t dsv41_moe_balance_workspace_size(int64_t T, int64_t E, int64_t S);
 int dsv41_moe_balance(const void *logits, int dtype, int64_t T, int64_t E, const int32_t *indices,
                       int topk, const int32_t *offsets, int64_t S, const uint8_t *mask,
                       int score_func, float gate_temp, const float *grad_loss,

@@ -17,7 +17,7 @@ def test_lora_forward_refuses_before_any_device_work():
     assert _fwd(R=12) == L.UNSUPPORTED and _fwd(R=136) == L.UNSUPPORTED
     assert _fwd(out=L.F16) == L.BAD_DTYPE
     assert _fwd(x=None) == L.BAD_ARG and _fwd(x=24) == L.MISALIGNED
-    assert _fwd() == L.WORKSPACE
+    assert _fwd(T=5000) == L.WORKSPACE
     assert _fwd(T=0) == L.OK
 
 
@@ -42,7 +42,7 @@ def test_balance_refuses_before_any_device_work():
     assert _bal(E=1025) == L.BAD_SHAPE and _bal(E=0) == L.BAD_SHAPE and _bal(T=-1) == L.BAD_SHAPE
     assert _bal(k=9) == L.BAD_ARG and _bal(k=0) == L.BAD_ARG and _bal(score=3) == L.BAD_ARG
     assert _bal(temp=0.0) == L.BAD_ARG and _bal(S=2) == L.BAD_ARG and _bal(gl=16) == L.BAD_ARG
-    assert _bal(p=None) == L.BAD_ARG and _bal() == L.WORKSPACE
+    assert _bal(p=None) == L.BAD_ARG and _bal(T=5000) == L.WORKSPACE
 
 
 def test_workspaces_stay_proportionate():
@@ -54,7 +54,7 @@ def test_workspaces_stay_proportionate():
             g = lib.dsv41_lora_workspace_size(T, 7168, 4096, n, 64, 1)
             assert f <= T * (64 * 4 + 64) + n * 64 + (1 << 20)
             assert g <= f + 2 * 2 * 148 * 64 * 256 * 4 + (1 << 20)
-    assert lib.dsv41_moe_balance_workspace_size(65536, 16) <= 65536 * 8 + 4096
+    assert lib.dsv41_moe_balance_workspace_size(65536, 384, 16) <= 65536 * 8 + 4096
 
 
 def test_cpu_tensors_are_refused():
