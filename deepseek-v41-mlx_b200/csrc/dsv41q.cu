@@ -893,8 +893,9 @@ int lora_rp(int64_t R) { return int((R + 15) / 16 * 16); }
 // the most tiles that T tokens on n adapters (and none) can make
 int64_t lora_max_tiles(int64_t T, int64_t n) { return T / LR_TILE + std::min(n + 1, T); }
 
-// wgrad: stages of the ring, CTAs an SM and the grid.  Three stages that fit twice into an SM
-// run as two CTAs; otherwise one CTA takes up to four.
+// wgrad: stages of the ring, CTAs an SM and the grid.  Four or five stages that fit twice into
+// an SM run as two CTAs (one's joins and stores behind the other's loads); larger ones as one
+// CTA of up to six.
 struct LoraWgradShape {
   int stages, grid;
   size_t smem;
@@ -906,8 +907,9 @@ LoraWgradShape lora_wgrad_shape(int64_t T, int64_t K, int64_t N, int64_t n, int6
   const int Rp = lora_rp(R), ns = grad_dtype == DSV41_F32 ? 3 : 2;
   s.u_bytes = uint32_t(Rp / 8) * LG_MN_LD;
   const size_t stage = LG_X_BYTES + size_t(ns) * s.u_bytes;
-  const bool two = 3 * stage + 1024 <= 113 * 1024;
-  s.stages = two ? 3 : int(std::min<size_t>(4, (225 * 1024 - 1024) / stage));
+  const int twice = int((112 * 1024 - 1024) / stage), once = int((224 * 1024 - 1024) / stage);
+  const bool two = twice >= 4;
+  s.stages = two ? std::min(twice, 5) : std::min(once, 6);
   s.smem = s.stages * stage + 1024;
   const int64_t work = (T / LR_KB + std::min(n, T)) * (ceil_div(K, LG_COLS) + ceil_div(N, LG_COLS));
   s.grid = int(std::max<int64_t>(1, std::min<int64_t>(work, int64_t(num_sms()) * (two ? 2 : 1))));
@@ -916,30 +918,31 @@ LoraWgradShape lora_wgrad_shape(int64_t T, int64_t K, int64_t N, int64_t n, int6
 
 struct LoraWs {
   LoraPlan plan;
-  float *h, *part;
+  __nv_bfloat16 *parts, *h_parts;
+  int64_t plane;
+  float *sums;
   bool ok;
   size_t used;
 };
 LoraWs lora_carve(void *ws, size_t cap, int64_t T, int64_t K, int64_t N, int64_t n, int64_t R,
                   bool backward) {
   WsCarve c{static_cast<uint8_t *>(ws), cap, 0};
-  LoraWs w;
+  LoraWs w{};
   w.plan.perm = c.take<int>(T);
-  w.plan.tiles = c.take<int2>(lora_max_tiles(T, n));
-  w.plan.n_tiles = c.take<int>(1);
+  w.plan.tiles = c.take<int4>(lora_max_tiles(T, n));
+  w.plan.head = c.take<int>(2);
   w.plan.off = c.take<int>(n + 2);
   w.plan.stages = c.take<int>(n + 1);
-  w.h = c.take<float>(T * R);
-  w.plan.tickets = nullptr;
-  w.plan.n_tickets = 0;
-  w.part = nullptr;
+  w.plane = T * lora_rp(R);
+  w.parts = c.take<__nv_bfloat16>(LR_PARTS * w.plane);
   if (backward) {
+    w.h_parts = c.take<__nv_bfloat16>(LR_PARTS * w.plane);
     // the larger of the two grids (bf16 and fp32 gradients)
     const int grid = std::max(lora_wgrad_shape(T, K, N, n, R, DSV41_BF16).grid,
                               lora_wgrad_shape(T, K, N, n, R, DSV41_F32).grid);
     w.plan.tickets = c.take<int>(grid);
     w.plan.n_tickets = grid;
-    w.part = c.take<float>(size_t(2) * grid * lora_rp(R) * LG_COLS);
+    w.sums = c.take<float>(size_t(2) * grid * lora_rp(R) * LG_COLS);
   }
   w.ok = c.ok;
   w.used = align_up(c.off, 256);
@@ -948,9 +951,9 @@ LoraWs lora_carve(void *ws, size_t cap, int64_t T, int64_t K, int64_t N, int64_t
 
 int lora_plan_launch(const int32_t *ids, int64_t T, int64_t n, const LoraPlan &plan,
                      cudaStream_t st) {
-  const size_t smem = size_t(3) * (n + 1) * 4;
+  const size_t smem = size_t(4) * (n + 1) * 4;
   DSV41_LAUNCH(max_dynamic_smem(k_lora_plan, smem), "lora_plan");
-  const unsigned C = unsigned(std::min<int64_t>(8, ceil_div(T, 1024)));
+  const unsigned C = unsigned(std::min<int64_t>(LP_MAX_CTAS, ceil_div(T, 1024)));
   ProfScope prof("lora_plan", st);
   DSV41_LAUNCH(launch_cluster(k_lora_plan, C, C, 1024, smem, st, ids, int(T), int(n), plan),
                "lora_plan");
@@ -995,29 +998,25 @@ int lora_shrink_launch(LoraShrink a, int64_t T, cudaStream_t st) {
   return DSV41_OK;
 }
 
-template <bool WMN, typename OT, int KJ>
-cudaError_t lora_expand_go(const LoraExpand &a, unsigned grid, cudaStream_t st) {
-  const int smem = (sizeof(OT) == 4 ? 3 : 2) * KJ * LR_TILE * 4 * 8;
-  cudaError_t e = max_dynamic_smem(k_lora_expand<WMN, OT, KJ>, smem);
-  if (e != cudaSuccess) return e;
-  k_lora_expand<WMN, OT, KJ><<<grid, 256, smem, st>>>(a);
-  return cudaGetLastError();
-}
-
+// Work items of up to 16 column blocks, about three for each CTA that runs at once.
 template <bool WMN, typename OT>
 int lora_expand_launch(LoraExpand a, int64_t T, cudaStream_t st) {
-  a.ncb = int(ceil_div(a.N, 256));
-  const int64_t tiles = ceil_div(T, LR_TILE), slots = 4 * num_sms();
-  a.cpu = int(std::max<int64_t>(1, std::min<int64_t>(8, tiles * a.ncb / (4 * slots))));
+  a.Rp = lora_rp(a.R);
+  a.a_bytes = uint32_t((sizeof(OT) == 4 ? 3 : 2) * (a.Rp / 8)) * LE_LD;
+  a.w_bytes = WMN ? uint32_t(LE_COLS / 8) * (a.Rp * 16 + 16) : uint32_t(a.Rp / 8) * LE_LD;
+  const size_t smem = a.a_bytes + 2 * a.w_bytes + LE_EPI_BYTES;
+  const int64_t slots = int64_t(num_sms()) * (smem <= 112 * 1024 ? 2 : 1);
+  a.ncb = int(ceil_div(a.N, LE_COLS));
+  a.cpu = int(std::max<int64_t>(1, std::min<int64_t>(16, ceil_div(T, LR_TILE) * a.ncb / (3 * slots))));
   a.vec = a.N * sizeof(OT) % 16 == 0 && aligned(a.base, 16) && aligned(a.y, 16);
   const unsigned grid = unsigned(std::min<int64_t>(
       lora_max_tiles(T, a.n) * ceil_div(a.ncb, a.cpu), slots));
   ProfScope prof("lora_expand", st);
-  cudaError_t e;
-  if (a.R <= 16) e = lora_expand_go<WMN, OT, 1>(a, grid, st);
-  else if (a.R <= 32) e = lora_expand_go<WMN, OT, 2>(a, grid, st);
-  else if (a.R <= 64) e = lora_expand_go<WMN, OT, 4>(a, grid, st);
-  else e = lora_expand_go<WMN, OT, 8>(a, grid, st);
+  cudaError_t e = max_dynamic_smem(k_lora_expand<WMN, OT>, smem);
+  if (e == cudaSuccess) {
+    k_lora_expand<WMN, OT><<<grid, LE_THREADS, smem, st>>>(a);
+    e = cudaGetLastError();
+  }
   return cuda_status(e, "lora_expand");
 }
 
@@ -1031,9 +1030,12 @@ cudaError_t lora_wgrad_go(const LoraWgrad &a, const LoraWgradShape &sh, cudaStre
 
 template <typename OT>
 cudaError_t lora_wgrad_launch(const LoraWgrad &a, const LoraWgradShape &sh, cudaStream_t st) {
-  if (sh.stages == 4) return lora_wgrad_go<OT, 4>(a, sh, st);
-  if (sh.stages == 3) return lora_wgrad_go<OT, 3>(a, sh, st);
-  return lora_wgrad_go<OT, 2>(a, sh, st);
+  switch (sh.stages) {
+    case 6: return lora_wgrad_go<OT, 6>(a, sh, st);
+    case 5: return lora_wgrad_go<OT, 5>(a, sh, st);
+    case 4: return lora_wgrad_go<OT, 4>(a, sh, st);
+    default: return lora_wgrad_go<OT, 3>(a, sh, st);
+  }
 }
 
 }  // namespace
@@ -1071,15 +1073,32 @@ extern "C" int dsv41_lora_forward(const void *x, int64_t T, int64_t K, const voi
   DSV41_REQUIRE(workspace && w.ok, DSV41_ERR_WORKSPACE, "workspace too small");
   DSV41_REQUIRE(aligned(workspace, 16), DSV41_ERR_MISALIGNED, "workspace must be 16-byte aligned");
   cudaStream_t st = STREAM(stream);
-  float *h = h_out ? h_out : w.h;
   rc = lora_plan_launch(ids, T, n, w.plan, st);
   if (rc) return rc;
-  const LoraShrink s{static_cast<const __nv_bfloat16 *>(x), K, static_cast<const __nv_bfloat16 *>(a),
-                     int(R), lora_rp(R), int(n), nullptr, h, w.plan, 0};
+  LoraShrink s{};
+  s.x = static_cast<const __nv_bfloat16 *>(x);
+  s.K = K;
+  s.w = static_cast<const __nv_bfloat16 *>(a);
+  s.R = int(R);
+  s.Rp = lora_rp(R);
+  s.n = int(n);
+  s.scaling = scaling;
+  s.out = h_out;
+  s.parts = w.parts;
+  s.plane = w.plane;
+  s.plan = w.plan;
   rc = lora_shrink_launch<false, true>(s, T, st);
   if (rc) return rc;
-  const LoraExpand e{h, static_cast<const __nv_bfloat16 *>(b), N, int(R), int(n), scaling, base, y,
-                     w.plan, 0, 0, 0};
+  LoraExpand e{};
+  e.parts = w.parts;
+  e.plane = w.plane;
+  e.w = static_cast<const __nv_bfloat16 *>(b);
+  e.N = N;
+  e.R = int(R);
+  e.n = int(n);
+  e.base = base;
+  e.y = y;
+  e.plan = w.plan;
   return out_dtype == DSV41_F32 ? lora_expand_launch<false, float>(e, T, st)
                                 : lora_expand_launch<false, __nv_bfloat16>(e, T, st);
 }
@@ -1115,24 +1134,44 @@ extern "C" int dsv41_lora_backward(const void *dy, const void *x, const float *h
   if (rc) return rc;
   const __nv_bfloat16 *dyb = static_cast<const __nv_bfloat16 *>(dy),
                       *xb = static_cast<const __nv_bfloat16 *>(x);
-  const LoraShrink s{dyb, N, static_cast<const __nv_bfloat16 *>(b), int(R), lora_rp(R), int(n),
-                     scaling, w.h, w.plan, 0};
+  LoraShrink s{};
+  s.x = dyb;
+  s.K = N;
+  s.w = static_cast<const __nv_bfloat16 *>(b);
+  s.R = int(R);
+  s.Rp = lora_rp(R);
+  s.n = int(n);
+  s.scaling = scaling;
+  s.parts = w.parts;
+  s.h = h;
+  s.h_parts = w.h_parts;
+  s.plane = w.plane;
+  s.plan = w.plan;
   rc = N % 8 == 0 ? lora_shrink_launch<true, true>(s, T, st) : lora_shrink_launch<true, false>(s, T, st);
   if (rc) return rc;
-  const LoraExpand e{w.h, static_cast<const __nv_bfloat16 *>(a), K, int(R), int(n), nullptr, dx_base,
-                     dx, w.plan, 0, 0, 0};
+  LoraExpand e{};
+  e.parts = w.parts;
+  e.plane = w.plane;
+  e.w = static_cast<const __nv_bfloat16 *>(a);
+  e.N = K;
+  e.R = int(R);
+  e.n = int(n);
+  e.base = dx_base;
+  e.y = dx;
+  e.plan = w.plan;
   rc = dx_dtype == DSV41_F32 ? lora_expand_launch<true, float>(e, T, st)
                              : lora_expand_launch<true, __nv_bfloat16>(e, T, st);
   if (rc) return rc;
   const LoraWgradShape sh = lora_wgrad_shape(T, K, N, n, R, grad_dtype);
   LoraWgrad g{};
-  g.side[0] = LoraGradSide{xb, w.h, K, int(ceil_div(K, LG_COLS)), nullptr, da, 1, 1};
-  g.side[1] = LoraGradSide{dyb, h, N, int(ceil_div(N, LG_COLS)), scaling, db, 0, N % 8 == 0};
+  g.side[0] = LoraGradSide{xb, w.parts, K, int(ceil_div(K, LG_COLS)), da, 1, 1};
+  g.side[1] = LoraGradSide{dyb, w.h_parts, N, int(ceil_div(N, LG_COLS)), db, 0, N % 8 == 0};
   g.R = int(R);
   g.Rp = lora_rp(R);
   g.n = int(n);
+  g.plane = w.plane;
   g.plan = w.plan;
-  g.part = w.part;
+  g.part = w.sums;
   g.u_bytes = sh.u_bytes;
   ProfScope prof("lora_wgrad", st);
   const cudaError_t ge = grad_dtype == DSV41_F32 ? lora_wgrad_launch<float>(g, sh, st)

@@ -13,10 +13,10 @@
 //   expand  [tokens x R] . [R x long]         k_lora_expand   (y, dx)
 //   wgrad   [long x tokens] . [tokens x R]    k_lora_wgrad    (dA, dB)
 // Every one streams a long activation matrix once against a small operand, so the bound is
-// HBM.  All sums are fp32; h and g stay fp32 in memory.  Where h or g is an operand of a
-// bf16 tensor-core product it goes in as a sum of bf16 parts (v = p0 + p1 + ..., each the
-// rounding of what the earlier ones leave): two parts keep 17 bits or more, below the rounding of a
-// bf16 result, three keep all 24 for an fp32 result.
+// HBM.  All sums are fp32.  Where h or g is an operand of a bf16 tensor-core product it goes in
+// as a sum of bf16 parts (v = p0 + p1 + ..., each the rounding of what the earlier ones leave):
+// two parts keep 17 bits or more, below the rounding of a bf16 result, three keep all 24 for an
+// fp32 result.  Shrink writes the parts, in sorted order, for both consumers.
 //
 // k_lora_plan sorts the tokens by adapter first (a stable counting sort), so that a tile of
 // 128 token rows belongs to one adapter; tokens without one come last.
@@ -33,8 +33,8 @@ constexpr int LR_KB = 64;           // contraction length of a stage
 // ------------------------------------------------------------------ plan
 struct LoraPlan {
   int *perm;       // [T] token of sorted position p
-  int2 *tiles;     // {adapter (n: none), tile of that adapter}
-  int *n_tiles;    // [1]
+  int4 *tiles;     // {adapter (n: none), first position, rows, 0}
+  int *head;       // [2] tiles, adapters with tokens
   int *off;        // [n + 2] first position of each adapter (n: none), then T
   int *stages;     // [n + 1] 64-token stages of the adapters before this one (wgrad's work)
   int *tickets;    // zeroed here: wgrad's joins
@@ -77,88 +77,99 @@ __device__ __forceinline__ void block_scan3(int (&v)[3], int (&tot)[3], int (*ws
 
 // One cluster of 1024-thread CTAs, each on a contiguous slice of the tokens: histogram in
 // shared memory, the other CTAs' histograms over distributed shared memory, one scan over the
-// adapters, then the stable scatter (warps of a 1024-token batch in order).  One launch of
-// about 4-6 us up to 8192 tokens; sorting in global memory would take three.
+// adapters, then the stable scatter (warps of a 1024-token batch in order).  One launch; sorting
+// through global memory would take three.
+constexpr int LP_MAX_CTAS = 8;
 __global__ void __launch_bounds__(1024, 1)
     k_lora_plan(const int32_t *__restrict__ ids, int T, int n, LoraPlan p) {
-  extern __shared__ int lp_smem[];
-  int *cnt = lp_smem, *pos = cnt + (n + 1), *tile0 = pos + (n + 1);   // [n + 1] each
+  extern __shared__ int lp_smem[];                                    // [n + 1] each
+  int *cnt = lp_smem, *pos = cnt + (n + 1), *tile0 = pos + (n + 1), *first = tile0 + (n + 1);
   __shared__ int wsum[32][3];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = gridDim.x, rank = blockIdx.x;
   const int per = (((T + C - 1) / C) + 1023) & ~1023;
-  const int t0 = min(int64_t(rank) * per, int64_t(T)), t1 = min(int64_t(t0) + per, int64_t(T));
+  const int t0 = int(min(int64_t(rank) * per, int64_t(T)));
+  const int t1 = int(min(int64_t(t0) + per, int64_t(T)));
   for (int i = tid; i <= n; i += 1024) cnt[i] = 0;
   __syncthreads();
-  for (int t = t0 + tid; t < t1; t += 1024) atomicAdd(&cnt[lora_bin(ids[t], n)], 1);
+  for (int b0 = t0; b0 < t1; b0 += 1024) {
+    const int bin = b0 + tid < t1 ? lora_bin(ids[b0 + tid], n) : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, bin);         // runs: one add a warp
+    if (bin >= 0 && lane == __ffs(same) - 1) atomicAdd(&cnt[bin], __popc(same));
+  }
   cluster_sync();
-  int run[3] = {0, 0, 0};                       // tokens, tiles, stages before this batch
+  int run[3] = {0, 0, 0}, used = 0;             // tokens, tiles, stages before this batch
   for (int b0 = 0; b0 <= n; b0 += 1024) {
     const int b = b0 + tid;
     int total = 0, before = 0;
-    if (b <= n)
-      for (int c = 0; c < C; ++c) {
-        const int v = ld_cluster_s32(mapa_rank(&cnt[b], c));
-        if (c < rank) before += v;
-        total += v;
+    if (b <= n) {
+      int v[LP_MAX_CTAS];                       // all requests in flight at once
+#pragma unroll
+      for (int c = 0; c < LP_MAX_CTAS; ++c) v[c] = c < C ? ld_cluster_s32(mapa_rank(&cnt[b], c)) : 0;
+#pragma unroll
+      for (int c = 0; c < LP_MAX_CTAS; ++c) {
+        if (c < rank) before += v[c];
+        total += v[c];
       }
+    }
     const int nt = (total + LR_TILE - 1) / LR_TILE, ns = (total + LR_KB - 1) / LR_KB;
     int v[3] = {total, nt, ns}, tot[3];
     block_scan3(v, tot, wsum);
     if (b <= n) {
-      const int first = run[0] + v[0] - total;
-      pos[b] = first + before;
+      first[b] = run[0] + v[0] - total;
+      pos[b] = first[b] + before;
       tile0[b] = run[1] + v[1] - nt;
       if (rank == 0) {
-        p.off[b] = first;
+        p.off[b] = first[b];
         p.stages[b] = run[2] + v[2] - ns;
         if (b == n) p.off[n + 1] = T;
       }
     }
+    used += __syncthreads_count(b < n && total > 0);
     for (int i = 0; i < 3; ++i) run[i] += tot[i];
   }
-  cluster_sync();                               // everyone has read the histograms
   for (int i = rank * 1024 + tid; i < p.n_tickets; i += C * 1024) p.tickets[i] = 0;
-  if (rank == 0 && tid == 0) *p.n_tiles = run[1];
-  // scatter: batches of 1024 tokens, their warps one after another
-  for (int b0 = t0; b0 < t1; b0 += 1024) {
-    const int t = b0 + tid;
-    const int bin = t < t1 ? lora_bin(ids[t], n) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, bin);
-    const int before = __popc(same & ((1u << lane) - 1));
-    const int warps = min(32, (t1 - b0 + 31) >> 5);
-    int start = 0;
-    for (int w = 0; w < warps; ++w) {
-      if (w == warp && before == 0 && bin >= 0) {
-        start = pos[bin];
-        pos[bin] = start + __popc(same);
-      }
-      __syncthreads();
-    }
-    start = __shfl_sync(0xffffffffu, start, __ffs(same) - 1);
-    if (bin >= 0) p.perm[start + before] = t;
+  if (rank == 0 && tid == 0) {
+    p.head[0] = run[1];
+    p.head[1] = used;
   }
-  // tiles: adapter by binary search over the first tiles
+  // tiles: the adapter by binary search over the first tiles
   for (int i = rank * 1024 + tid; i < run[1]; i += C * 1024) {
-    int lo = 0, hi = n;                         // last b with tile0[b] <= i (and tiles of its own)
+    int lo = 0, hi = n;                         // last b with tile0[b] <= i
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (tile0[mid] <= i) lo = mid;
       else hi = mid - 1;
     }
-    p.tiles[i] = make_int2(lo, i - tile0[lo]);
+    const int p0 = first[lo] + (i - tile0[lo]) * LR_TILE;
+    p.tiles[i] = make_int4(lo, p0, min(LR_TILE, (lo == n ? T : first[lo + 1]) - p0), 0);
   }
-}
-
-// The rows of tile i: adapter, first sorted position, row count.
-struct LoraTile {
-  int adapter, p0, rows;
-};
-__device__ __forceinline__ LoraTile lora_tile(const LoraPlan &p, int i) {
-  const int2 v = p.tiles[i];
-  const int a = p.off[v.x], b = p.off[v.x + 1];
-  const int p0 = a + v.y * LR_TILE;
-  return LoraTile{v.x, p0, min(LR_TILE, b - p0)};
+  // scatter: batches of 1024 tokens, their warps one after another
+  for (int b0 = t0; b0 < t1; b0 += 1024) {
+    const int t = b0 + tid, bin0 = lora_bin(ids[b0], n);
+    const int bin = t < t1 ? lora_bin(ids[t], n) : -1;
+    if (__syncthreads_and(bin < 0 || bin == bin0)) {                  // a run on one adapter
+      if (bin >= 0) p.perm[pos[bin0] + tid] = t;
+      __syncthreads();
+      if (tid == 0) pos[bin0] += min(1024, t1 - b0);
+    } else {
+      const unsigned same = __match_any_sync(0xffffffffu, bin);
+      const int before = __popc(same & ((1u << lane) - 1));
+      const int warps = min(32, (t1 - b0 + 31) >> 5);
+      int start = 0;
+      for (int w = 0; w < warps; ++w) {
+        if (w == warp && before == 0 && bin >= 0) {
+          start = pos[bin];
+          pos[bin] = start + __popc(same);
+        }
+        __syncthreads();
+      }
+      start = __shfl_sync(0xffffffffu, start, __ffs(same) - 1);
+      if (bin >= 0) p.perm[start + before] = t;
+    }
+    __syncthreads();
+  }
+  cluster_sync();                               // the others have read this histogram
 }
 
 // ------------------------------------------------------------------ operand staging
@@ -179,24 +190,54 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32
                "r"(src_bytes)
                : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
+// the same, asking L2 for the 256 bytes around it: rows are walked 128 bytes a stage
+__device__ __forceinline__ void cp_async16_256(uint32_t dst, const void *src, uint32_t src_bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(src_bytes)
+               : "memory");
 }
-template <int N> __device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void cp_async_wait_all() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+// This thread's part of a stage is on its way: its arrival on `full` follows its copies.  The
+// MMA warp fences the proxies once it has seen the barrier.  Element stores are fenced and released
+// by the thread itself.
+template <bool VEC> __device__ __forceinline__ void stage_arrive(uint64_t *full) {
+  if constexpr (VEC) {
+    cp_async_arrive_noinc(full);
+  } else {
+    cp_async_wait_all();
+    fence_proxy_async_smem();
+    mbar_arrive(full);
+  }
 }
 __device__ __forceinline__ void st_shared16(uint32_t dst, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y),
                "r"(v.z), "r"(v.w)
                : "memory");
 }
+// Items e = tid + 128 i of a [major][minor] grid, without a division an item.
+struct GridWalk {
+  int major, minor, dmajor, dminor, n;
+  __device__ __forceinline__ GridWalk(int e, int n_minor)
+      : major(e / n_minor), minor(e % n_minor), dmajor(128 / n_minor), dminor(128 % n_minor),
+        n(n_minor) {}
+  __device__ __forceinline__ void next() {
+    major += dmajor;
+    minor += dminor;
+    if (minor >= n) {
+      minor -= n;
+      ++major;
+    }
+  }
+};
 // Eight bf16 values of a row to shared memory, zeros past `valid` of them (valid <= 0: none is
 // read).  VEC: the row is 16-byte aligned and valid is 0 or >= 8 (one asynchronous copy);
 // otherwise (rows of a length that is no multiple of 8) element loads.
 template <bool VEC>
 __device__ __forceinline__ void stage8(uint32_t dst, const __nv_bfloat16 *src, int64_t valid) {
   if constexpr (VEC) {
-    cp_async16(dst, src, valid > 0 ? 16u : 0u);
+    cp_async16_256(dst, src, valid > 0 ? 16u : 0u);
   } else {
     uint32_t w[4] = {0, 0, 0, 0};
     const uint16_t *s = reinterpret_cast<const uint16_t *>(src);
@@ -207,14 +248,45 @@ __device__ __forceinline__ void stage8(uint32_t dst, const __nv_bfloat16 *src, i
   }
 }
 
+// v as bf16 parts; the rest after each part is exact in fp32 (and zero after an infinity or NaN).
+template <int NS>
+__device__ __forceinline__ void split_bf16(float v, uint16_t (&p)[NS]) {
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    p[i] = f2bf_bits(v);
+    v = (p[i] & 0x7F80) == 0x7F80 ? 0.0f : v - bf_bits2f(p[i]);
+  }
+}
+
+// Four values times sc to their parts: LR_PARTS planes of [T][Rp], `plane` apart.
+constexpr int LR_PARTS = 3;
+__device__ __forceinline__ void store_parts(__nv_bfloat16 *dst, int64_t plane, float4 v, float sc) {
+  uint16_t p[4][LR_PARTS];
+  split_bf16<LR_PARTS>(v.x * sc, p[0]);
+  split_bf16<LR_PARTS>(v.y * sc, p[1]);
+  split_bf16<LR_PARTS>(v.z * sc, p[2]);
+  split_bf16<LR_PARTS>(v.w * sc, p[3]);
+#pragma unroll
+  for (int i = 0; i < LR_PARTS; ++i)
+    *reinterpret_cast<uint2 *>(dst + i * plane) = make_uint2(
+        uint32_t(p[0][i]) | (uint32_t(p[1][i]) << 16), uint32_t(p[2][i]) | (uint32_t(p[3][i]) << 16));
+}
+
 // ------------------------------------------------------------------ shrink
+struct LoraTile {
+  int adapter, p0, rows;       // n: none; first sorted position; rows <= LR_TILE
+};
 struct LoraShrink {
   const __nv_bfloat16 *x;      // [T, K]
   int64_t K;                   // contraction length
   const __nv_bfloat16 *w;      // [n][R][K], or [n][K][R] (WMN)
   int R, Rp, n;                // Rp: R rounded up to 16
   const float *scaling;        // NULL: 1
-  float *out;                  // [T, R]
+  float *out;                  // [T, R] the product as it is, or NULL
+  __nv_bfloat16 *parts;        // [LR_PARTS][T][Rp] the product times scaling, sorted order
+  const float *h;              // [T, R] or NULL: a second value to scale and split the same way
+  __nv_bfloat16 *h_parts;
+  int64_t plane;               // T * Rp
   LoraPlan plan;
   uint32_t w_bytes;            // staged bytes of w in a stage
 };
@@ -242,7 +314,7 @@ __global__ void __launch_bounds__(LS_THREADS, 2) k_lora_shrink(const LoraShrink 
   const uint32_t cols = a.Rp <= 32 ? 32u : a.Rp <= 64 ? 64u : 128u;
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 4);
+      mbar_init(&full[s], 128);
       mbar_init(&empty[s], 1);
     }
     mbar_init(&acc_full, 1);
@@ -258,13 +330,14 @@ __global__ void __launch_bounds__(LS_THREADS, 2) k_lora_shrink(const LoraShrink 
   const uint32_t tmem = tmem_slot;
   const int nkb = int((a.K + LR_KB - 1) / LR_KB);
   const int kb0 = int(int64_t(nkb) * rank / C), kb1 = int(int64_t(nkb) * (rank + 1) / C);
-  const int ntiles = *a.plan.n_tiles;
+  const int ntiles = a.plan.head[0];
   int it = 0, done = 0;                   // stages and tiles so far (barrier parities)
   bool ok = true;                         // no wait of this thread has run out
   for (int i = int(cluster_id_x()); i < ntiles; i += int(ncluster_x())) {
-    const LoraTile tl = lora_tile(a.plan, i);
+    const int4 tv = a.plan.tiles[i];
+    const LoraTile tl{tv.x, tv.y, tv.z};
     if (tl.adapter == a.n) {              // no adapter: h = 0
-      if (rank == 0)
+      if (rank == 0 && a.out)
         for (int e = tid; e < tl.rows * a.R; e += LS_THREADS)
           a.out[int64_t(a.plan.perm[tl.p0 + e / a.R]) * a.R + e % a.R] = 0.0f;
       continue;
@@ -278,6 +351,8 @@ __global__ void __launch_bounds__(LS_THREADS, 2) k_lora_shrink(const LoraShrink 
 #pragma unroll
       for (int j = 0; j < 8; ++j) tok[j] = rows_s[r0 + 16 * j];
       const __nv_bfloat16 *wi = a.w + int64_t(tl.adapter) * a.R * a.K;
+      const GridWalk w0(tid, a.Rp >> 3);             // WMN: 8-wide groups of r, contraction rows
+      const uint32_t swz = uint32_t(c ^ (r0 & 7)) << 4;
       int jt = it;
       for (int kb = kb0; kb < kb1 && ok; ++kb, ++jt) {
         const int s = jt % S;
@@ -286,7 +361,7 @@ __global__ void __launch_bounds__(LS_THREADS, 2) k_lora_shrink(const LoraShrink 
           break;
         }
         const int64_t k = int64_t(kb) * LR_KB + c * 8;
-        const uint32_t dx = sx + s * LS_X_BYTES + r0 * 128 + ((c ^ (r0 & 7)) << 4);
+        const uint32_t dx = sx + s * LS_X_BYTES + r0 * 128 + swz;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           stage8<VEC>(dx + j * 2048, tok[j] < 0 ? a.x : a.x + int64_t(tok[j]) * a.K + k,
@@ -294,30 +369,20 @@ __global__ void __launch_bounds__(LS_THREADS, 2) k_lora_shrink(const LoraShrink 
         const uint32_t dw = sw + s * a.w_bytes;
         if constexpr (!WMN) {
           for (int r = r0; r < a.Rp; r += 16)
-            cp_async16(dw + r * 128 + ((c ^ (r & 7)) << 4), r < a.R && k < a.K ? wi + r * a.K + k : wi,
+            cp_async16(dw + r * 128 + swz, r < a.R && k < a.K ? wi + r * a.K + k : wi,
                        r < a.R && k < a.K ? 16u : 0u);
         } else {
-          const int rc = a.Rp >> 3;
-          for (int e = tid; e < rc * LR_KB; e += 128) {
-            const int g = e % rc, kk = e / rc;
-            const int64_t kr = int64_t(kb) * LR_KB + kk;
-            const bool in = g * 8 < a.R && kr < a.K;
-            cp_async16(dw + g * LS_MN_LD + kk * 16, in ? wi + kr * a.R + g * 8 : wi, in ? 16u : 0u);
+          const __nv_bfloat16 *wk = wi + int64_t(kb) * LR_KB * a.R;
+          const int rows = int(min(int64_t(LR_KB), a.K - int64_t(kb) * LR_KB));
+#pragma unroll 4
+          for (GridWalk w = w0; w.major < LR_KB; w.next()) {
+            const bool in = w.minor * 8 < a.R && w.major < rows;
+            cp_async16(dw + w.minor * LS_MN_LD + w.major * 16,
+                       in ? wk + w.major * a.R + w.minor * 8 : wi, in ? 16u : 0u);
           }
         }
-        cp_async_commit();
-        if (kb - kb0 >= S - 2) {                     // the stage issued S - 2 ago has landed
-          cp_async_wait<S - 2>();
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[(jt - (S - 2)) % S]);
-        }
+        stage_arrive<VEC>(&full[s]);
       }
-      cp_async_wait<0>();
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0 && ok)
-        for (int e = max(it, jt - (S - 2)); e < jt; ++e) mbar_arrive(&full[e % S]);
     } else {
       // ------------------------------------------------------------ MMA issuer
       const uint32_t id = idesc_lora(a.Rp, 0, WMN ? 1 : 0);
@@ -327,6 +392,7 @@ __global__ void __launch_bounds__(LS_THREADS, 2) k_lora_shrink(const LoraShrink 
           ok = false;
           break;
         }
+        fence_proxy_async_smem();
         tc_fence_after();
         const uint64_t da = sdesc_sw128(sx + s * LS_X_BYTES);
         const uint32_t bw = sw + s * a.w_bytes;
@@ -362,27 +428,38 @@ __global__ void __launch_bounds__(LS_THREADS, 2) k_lora_shrink(const LoraShrink 
     cluster_sync();
     tc_fence_after();
     const float sc = a.scaling ? a.scaling[tl.adapter] : 1.0f;
-    const int q4 = a.R >> 2, row_a = LR_TILE * rank / C, row_b = LR_TILE * (rank + 1) / C;
+    const int q4 = a.Rp >> 2, row_a = LR_TILE * rank / C, row_b = LR_TILE * (rank + 1) / C;
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int e = tid; e < (row_b - row_a) * q4; e += LS_THREADS) {
       const int row = row_a + e / q4, c4 = (e % q4) * 4;
       if (row >= tl.rows) break;
-      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int q = 0; q < C; ++q) {
-        float4 v;
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                     : "r"(mapa_rank(red + row * ld + c4, q))
-                     : "memory");
-        s.x += v.x;
-        s.y += v.y;
-        s.z += v.z;
-        s.w += v.w;
+      const bool in = c4 < a.R;                    // the padding of Rp: zeros
+      const int64_t tok = rows_s[row], at = int64_t(tl.p0 + row) * a.Rp + c4;
+      float4 v[8], s = zero;                       // all requests in flight, added in rank order
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        v[q] = zero;
+        if (in && q < C)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[q].x), "=f"(v[q].y), "=f"(v[q].z), "=f"(v[q].w)
+                       : "r"(mapa_rank(red + row * ld + c4, q))
+                       : "memory");
       }
-      *reinterpret_cast<float4 *>(a.out + int64_t(rows_s[row]) * a.R + c4) =
-          make_float4(s.x * sc, s.y * sc, s.z * sc, s.w * sc);
+      const float4 h = in && a.h ? __ldg(reinterpret_cast<const float4 *>(a.h + tok * a.R + c4)) : zero;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        s.x += v[q].x;
+        s.y += v[q].y;
+        s.z += v[q].z;
+        s.w += v[q].w;
+      }
+      if (a.out && in) *reinterpret_cast<float4 *>(a.out + tok * a.R + c4) = s;
+      store_parts(a.parts + at, a.plane, s, sc);
+      if (a.h) store_parts(a.h_parts + at, a.plane, h, sc);
     }
     cluster_sync();                       // before the stages are written again
   }
+  cp_async_wait_all();
   tc_fence_before();
   __syncthreads();
   if (warp == 4) {
@@ -509,206 +586,265 @@ __global__ void __launch_bounds__(LD_THREADS) k_lora_decode(const LoraDecode p) 
 
 // ------------------------------------------------------------------ expand
 struct LoraExpand {
-  const float *h;              // [T, R]
+  const __nv_bfloat16 *parts;  // [LR_PARTS][T][Rp] h times scaling, sorted order
+  int64_t plane;
   const __nv_bfloat16 *w;      // [n][N][R], or [n][R][N] (WMN)
   int64_t N;
-  int R, n;
-  const float *scaling;        // NULL: 1
+  int R, Rp, n;
   const void *base;            // [T, N] or NULL
   void *y;                     // [T, N]
   LoraPlan plan;
-  int ncb, cpu;                // 256-column blocks, and how many of them a work item takes
+  int ncb, cpu;                // 128-column blocks, and how many of them a work item takes
   int vec;                     // rows of base and y are 16-byte aligned
+  uint32_t a_bytes, w_bytes;   // staged bytes of the parts and of a column block of W
 };
 
-// v as bf16 parts; the rest after each part is exact in fp32 (and zero after an infinity or NaN).
-template <int NS>
-__device__ __forceinline__ void split_bf16(float v, uint16_t (&p)[NS]) {
-#pragma unroll
-  for (int i = 0; i < NS; ++i) {
-    p[i] = f2bf_bits(v);
-    v = (p[i] & 0x7F80) == 0x7F80 ? 0.0f : v - bf_bits2f(p[i]);
-  }
-}
+constexpr int LE_COLS = 128;
+constexpr int LE_THREADS = 13 * 32;
+constexpr int LE_LD = 128 * 16 + 16;              // bytes between 8-wide k groups of 128 rows
+constexpr int LE_EPI_LD = 36;                     // floats of a transposition row
+constexpr int LE_EPI_BYTES = 8 * 32 * LE_EPI_LD * 4;
 
-// A CTA of 8 warps takes a tile's 128 token rows and 256 output columns at a time, a warp 32
-// columns: the warp's piece of W stays in registers for all 128 rows (mma.sync m16n8k16), the
-// split rows of h are in shared memory.  Output columns are dealt to the MMA's n indices so
-// that a lane's four accumulator pairs are 8 neighbouring columns (and k indices so that a
-// lane's operand values are 4 neighbouring r): base and y move as 16-byte pieces straight from
-// registers, no transposition.  KJ = ceil(R / 16) rounded up to 1, 2, 4 or 8.
-template <bool WMN, typename OT, int KJ>
-__global__ void __launch_bounds__(256) k_lora_expand(const LoraExpand a) {
+// D[128 tokens x 128 columns] in TMEM (tcgen05.mma kind::f16, double-buffered): the tile's
+// parts are the A operand, contraction NS * Rp, staged once for a work item's column blocks; a
+// block of W is the B operand, double-buffered, in its own order in memory (rows of r for B,
+// columns contiguous for A: the MMA takes either).  Warps 0-3 stage, 4 issues the MMAs, 5-12
+// read TMEM, turn 32 x 32 pieces through shared memory and move base and y in 64- or 128-byte
+// pieces of a row.  mma.sync with its accumulators stored straight from registers took 185 us
+// at T 8192, N 14336, R 32 (two CTAs an SM at 122 registers, too few loads in flight).
+template <bool WMN, typename OT>
+__global__ void __launch_bounds__(LE_THREADS, 2) k_lora_expand(const LoraExpand a) {
   constexpr int NS = sizeof(OT) == 4 ? 3 : 2;
-  extern __shared__ uint2 le_h[];                 // [NS][KJ][128 rows][4 lanes] pairs of bf16x2
-  __shared__ int rows_s[LR_TILE];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const OT *base = static_cast<const OT *>(a.base);
-  OT *y = static_cast<OT *>(a.y);
-  const int per_tile = (a.ncb + a.cpu - 1) / a.cpu;
-  const int64_t items = int64_t(*a.plan.n_tiles) * per_tile;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const LoraTile tl = lora_tile(a.plan, int(item / per_tile));
-    const bool live = tl.adapter < a.n;
-    const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
-    __syncthreads();
-    if (tid < LR_TILE) rows_s[tid] = tid < tl.rows ? a.plan.perm[tl.p0 + tid] : -1;
-    __syncthreads();
-    if (live) {
-      const float sc = a.scaling ? a.scaling[tl.adapter] : 1.0f;
-      for (int e = tid; e < KJ * LR_TILE * 4; e += 256) {
-        const int row = (e >> 2) / KJ, r = ((e >> 2) % KJ) * 16 + (e & 3) * 4;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (rows_s[row] >= 0 && r < a.R)
-          v = *reinterpret_cast<const float4 *>(a.h + int64_t(rows_s[row]) * a.R + r);
-        uint16_t p0[NS], p1[NS], p2[NS], p3[NS];
-        split_bf16<NS>(v.x * sc, p0);
-        split_bf16<NS>(v.y * sc, p1);
-        split_bf16<NS>(v.z * sc, p2);
-        split_bf16<NS>(v.w * sc, p3);
+  extern __shared__ __align__(128) uint8_t le_smem[];
+  const uint32_t sa = smem_u32(le_smem), sw = sa + a.a_bytes;
+  float *epi = reinterpret_cast<float *>(le_smem + a.a_bytes + 2 * a.w_bytes);
+  __shared__ uint64_t a_empty, w_full[2], w_empty[2], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    mbar_init(&a_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&w_full[i], 128);
+      mbar_init(&w_empty[i], 1);
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 8);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(&tmem_slot, 2 * LE_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int per_tile = (a.ncb + a.cpu - 1) / a.cpu, rg = a.Rp >> 3;
+  const int64_t items = int64_t(a.plan.head[0]) * per_tile;
+  bool ok = true;
+  int blk = 0, live = 0;                          // column blocks and live items so far
+  if (warp < 4) {
+    // -------------------------------------------------------------- staging
+    const GridWalk w0(tid, rg);
+    for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      const int4 tl = a.plan.tiles[item / per_tile];
+      if (tl.x >= a.n) continue;
+      const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
+      const __nv_bfloat16 *wi = a.w + int64_t(tl.x) * a.R * a.N;
+      if (!(ok = mbar_wait(&a_empty, (uint32_t(live) & 1u) ^ 1u))) break;
+      ++live;
+      const __nv_bfloat16 *pt = a.parts + int64_t(tl.y) * a.Rp;
+#pragma unroll 2
+      for (GridWalk w = w0; w.major < LR_TILE; w.next()) {
+        const bool in = w.major < tl.z;
+        const __nv_bfloat16 *src = in ? pt + w.major * a.Rp + w.minor * 8 : a.parts;
 #pragma unroll
         for (int i = 0; i < NS; ++i)
-          le_h[((i * KJ + (r >> 4)) * LR_TILE + row) * 4 + (e & 3)] = make_uint2(
-              uint32_t(p0[i]) | (uint32_t(p1[i]) << 16), uint32_t(p2[i]) | (uint32_t(p3[i]) << 16));
+          cp_async16(sa + uint32_t(i * rg + w.minor) * LE_LD + w.major * 16,
+                     src + (in ? i * a.plane : 0), in ? 16u : 0u);
       }
-    }
-    __syncthreads();
-    for (int cb = cb0; cb < cb1; ++cb) {
-      const int64_t c0 = int64_t(cb) * 256 + warp * 32;
-      if (c0 >= a.N) break;
-      // W of this warp's 32 columns: b[j][q] = the k16 step j of n index g = column
-      // c0 + 8 (g >> 1) + 2 q + (g & 1), values r = 16 j + 4 t .. + 3
-      uint2 b[KJ][4];
-#pragma unroll
-      for (int j = 0; j < KJ; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) b[j][q] = make_uint2(0u, 0u);
-      if (live) {
+      for (int cb = cb0; cb < cb1 && ok; ++cb, ++blk) {
+        const int b = blk & 1;
+        if (!(ok = mbar_wait(&w_empty[b], (uint32_t(blk >> 1) & 1u) ^ 1u))) break;
+        const int64_t c0 = int64_t(cb) * LE_COLS;
+        const uint32_t dw = sw + b * a.w_bytes;
         if constexpr (!WMN) {
-          const __nv_bfloat16 *wi = a.w + int64_t(tl.adapter) * a.R * a.N;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int64_t col = c0 + 8 * (g >> 1) + 2 * q + (g & 1);
-#pragma unroll
-            for (int j = 0; j < KJ; ++j)
-              if (col < a.N && 16 * j + 4 * t < a.R)
-                b[j][q] = __ldg(reinterpret_cast<const uint2 *>(wi + col * a.R + 16 * j + 4 * t));
+          const __nv_bfloat16 *wc = wi + c0 * a.R;
+          const int n_cols = int(min(int64_t(LE_COLS), a.N - c0));
+#pragma unroll 4
+          for (GridWalk w = w0; w.major < LE_COLS; w.next()) {
+            const bool in = w.major < n_cols && w.minor * 8 < a.R;
+            cp_async16(dw + uint32_t(w.minor) * LE_LD + w.major * 16,
+                       in ? wc + w.major * a.R + w.minor * 8 : wi, in ? 16u : 0u);
           }
         } else {
-          const __nv_bfloat16 *wi = a.w + int64_t(tl.adapter) * a.R * a.N;
-          const int64_t col = c0 + 8 * (g >> 1);          // N % 8 == 0: 8 columns or none
-#pragma unroll
-          for (int j = 0; j < KJ; ++j) {
-            const int r = 16 * j + 4 * t;
-            if (col < a.N && r < a.R) {
-              uint4 v[4];
-#pragma unroll
-              for (int u = 0; u < 4; ++u)
-                v[u] = __ldg(reinterpret_cast<const uint4 *>(wi + int64_t(r + u) * a.N + col));
-              const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;   // this lane's column of each pair
-              b[j][0] = make_uint2(__byte_perm(v[0].x, v[1].x, sel), __byte_perm(v[2].x, v[3].x, sel));
-              b[j][1] = make_uint2(__byte_perm(v[0].y, v[1].y, sel), __byte_perm(v[2].y, v[3].y, sel));
-              b[j][2] = make_uint2(__byte_perm(v[0].z, v[1].z, sel), __byte_perm(v[2].z, v[3].z, sel));
-              b[j][3] = make_uint2(__byte_perm(v[0].w, v[1].w, sel), __byte_perm(v[2].w, v[3].w, sel));
-            }
+          const int g = tid & 15;                  // 8 columns; rows r = tid / 16 + 8 i
+          const bool cin = c0 + g * 8 < a.N;
+          const __nv_bfloat16 *wc = wi + c0 + g * 8;
+          const uint32_t dg = dw + uint32_t(g) * (a.Rp * 16 + 16);
+#pragma unroll 4
+          for (int r = tid >> 4; r < a.Rp; r += 8) {
+            const bool in = cin && r < a.R;
+            cp_async16(dg + r * 16, in ? wc + int64_t(r) * a.N : wi, in ? 16u : 0u);
           }
         }
+        stage_arrive<true>(&w_full[b]);
       }
-      const int64_t col = c0 + 8 * t;                      // this lane's 8 output columns
-      for (int m0 = 0; m0 < tl.rows; m0 += 16) {
-        const int row[2] = {rows_s[m0 + g], rows_s[m0 + g + 8]};
-        float d[4][4];
-        if (a.vec && col < a.N) {
+    }
+    cp_async_wait_all();
+  } else if (warp == 4) {
+    // -------------------------------------------------------------- MMA issuer
+    const uint32_t id = idesc_lora(LE_COLS, 0, WMN ? 1 : 0);
+    for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      if (a.plan.tiles[item / per_tile].x >= a.n) continue;
+      const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
+      for (int cb = cb0; cb < cb1; ++cb, ++blk) {
+        const int b = blk & 1;
+        const uint32_t ph = uint32_t(blk >> 1) & 1u;
+        if (!warp_wait(&acc_empty[b], ph ^ 1u) || !warp_wait(&w_full[b], ph)) {
+          ok = false;
+          break;
+        }
+        fence_proxy_async_smem();
+        tc_fence_after();
+        const uint64_t da = sdesc(sa, LE_LD, 128, 0);
+        const uint32_t bw = sw + b * a.w_bytes;
+        const uint64_t db = WMN ? sdesc(bw, 128, a.Rp * 16 + 16, 0) : sdesc(bw, LE_LD, 128, 0);
+        const uint32_t bstep = WMN ? 256 : 2 * LE_LD;            // 16 contraction indices
+        for (int i = NS - 1; i >= 0; --i)                        // the smallest parts first
+          for (int k = 0; k < a.Rp / 16; ++k)
+            tc_mma_bf16_el(tmem + b * LE_COLS,
+                           da + uint64_t(uint32_t(i * rg + 2 * k) * (LE_LD >> 4)),
+                           db + uint64_t(k * (bstep >> 4)), id, (i < NS - 1 || k) ? 1u : 0u);
+        tc_commit_el(&w_empty[b]);
+        tc_commit_el(&acc_full[b]);
+      }
+      if (ok) tc_commit_el(&a_empty);
+    }
+    __syncwarp();
+  } else {
+    // -------------------------------------------------------------- epilogue
+    const OT *base = static_cast<const OT *>(a.base);
+    OT *y = static_cast<OT *>(a.y);
+    const int w8 = warp - 5, q4 = warp & 3, half = w8 >> 2;     // TMEM lanes 32 q4 .., 64 columns
+    float *tp = epi + w8 * 32 * LE_EPI_LD;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+      const int4 tl = a.plan.tiles[item / per_tile];
+      const bool has = tl.x < a.n;
+      const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
+      // vec: rows 32 q4 + 8 j + lane / 4; else the tokens of all 32 rows, a lane each
+      int tok[4];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (base && row[u] >= 0) {
-              const OT *src = base + int64_t(row[u]) * a.N + col;
-              if constexpr (sizeof(OT) == 4) {
-                const float4 v0 = *reinterpret_cast<const float4 *>(src);
-                const float4 v1 = *reinterpret_cast<const float4 *>(src + 4);
+      for (int j = 0; j < 4; ++j) {
+        const int row = 32 * q4 + 8 * j + (lane >> 2);
+        tok[j] = row < tl.z ? a.plan.perm[tl.y + row] : -1;
+      }
+      const int row_l = 32 * q4 + lane;
+      const int tok_l = row_l < tl.z ? a.plan.perm[tl.y + row_l] : -1;
+      for (int cb = cb0; cb < cb1; ++cb) {
+        const int b = blk & 1;
+#pragma unroll 1
+        for (int ch = 0; ch < 2; ++ch) {
+          const int64_t c0 = int64_t(cb) * LE_COLS + half * 64 + ch * 32;
+          const int64_t c = c0 + (lane & 3) * 8;
+          uint4 in[4][sizeof(OT) / 2];
+          if (a.vec && base && c < a.N) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (tok[j] >= 0) {
+                const uint4 *src = reinterpret_cast<const uint4 *>(base + int64_t(tok[j]) * a.N + c);
+#pragma unroll
+                for (int u = 0; u < int(sizeof(OT) / 2); ++u) in[j][u] = src[u];
+              }
+          }
+          if (has && ch == 0) {
+            // a warp whose wait ran out goes on without waiting
+            if (ok) ok = warp_wait(&acc_full[b], uint32_t(blk >> 1) & 1u);
+            tc_fence_after();
+          }
+          if (has) {
+            uint32_t v[32];
+            tmem_ld32(tmem + (uint32_t(32 * q4) << 16) + b * LE_COLS + half * 64 + ch * 32, v);
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4 *>(tp + lane * LE_EPI_LD + e) =
+                  make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            __syncwarp();
+          }
+          if (a.vec) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+              if (has) {
+                const float4 *src = reinterpret_cast<const float4 *>(
+                    tp + (8 * j + (lane >> 2)) * LE_EPI_LD + (lane & 3) * 8);
+                const float4 v0 = src[0], v1 = src[1];
                 f[0] = v0.x; f[1] = v0.y; f[2] = v0.z; f[3] = v0.w;
                 f[4] = v1.x; f[5] = v1.y; f[6] = v1.z; f[7] = v1.w;
-              } else {
-                const uint4 v = *reinterpret_cast<const uint4 *>(src);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+              }
+              if (tok[j] < 0 || c >= a.N) continue;
+              uint4 *dst = reinterpret_cast<uint4 *>(y + int64_t(tok[j]) * a.N + c);
+              if constexpr (sizeof(OT) == 4) {
+                if (base) {
+                  const uint32_t *s = reinterpret_cast<const uint32_t *>(in[j]);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  f[2 * q] = bf_bits2f(uint16_t(w[q]));
-                  f[2 * q + 1] = bf_bits2f(uint16_t(w[q] >> 16));
+                  for (int e = 0; e < 8; ++e) f[e] += __uint_as_float(s[e]);
                 }
+                dst[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]),
+                                    __float_as_uint(f[2]), __float_as_uint(f[3]));
+                dst[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]),
+                                    __float_as_uint(f[6]), __float_as_uint(f[7]));
+              } else {
+                const uint32_t s[4] = {in[j][0].x, in[j][0].y, in[j][0].z, in[j][0].w};
+                uint32_t o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if (base) {
+                    f[2 * e] += bf_bits2f(uint16_t(s[e]));
+                    f[2 * e + 1] += bf_bits2f(uint16_t(s[e] >> 16));
+                  }
+                  o[e] = uint32_t(f2bf_bits(f[2 * e])) | (uint32_t(f2bf_bits(f[2 * e + 1])) << 16);
+                }
+                dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
               }
             }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              d[q][2 * u] = f[2 * q];
-              d[q][2 * u + 1] = f[2 * q + 1];
+          } else {
+            // rows that start anywhere: a row a step, a lane per column
+#pragma unroll 8
+            for (int r = 0; r < 32; ++r) {
+              const int tk = __shfl_sync(0xffffffffu, tok_l, r);
+              if (tk < 0 || c0 + lane >= a.N) continue;
+              const int64_t at = int64_t(tk) * a.N + c0 + lane;
+              float f = has ? tp[r * LE_EPI_LD + lane] : 0.0f;
+              if (base) f += float(base[at]);
+              y[at] = OT(f);
             }
           }
-        } else {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              d[e >> 1][2 * u + (e & 1)] =
-                  (base && row[u] >= 0 && col + e < a.N)
-                      ? float(base[int64_t(row[u]) * a.N + col + e]) : 0.0f;
+          __syncwarp();
         }
-        if (live) {
-          float acc[4][4] = {};
-#pragma unroll
-          for (int i = NS - 1; i >= 0; --i)                // the smallest parts first
-#pragma unroll
-            for (int j = 0; j < KJ; ++j) {
-              const uint2 *hp = le_h + ((i * KJ + j) * LR_TILE + m0) * 4;
-              const uint2 lo = hp[g * 4 + t], hi = hp[(g + 8) * 4 + t];
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                mma_bf16(acc[q], lo.x, hi.x, lo.y, hi.y, b[j][q].x, b[j][q].y);
-            }
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) d[q][e] += acc[q][e];
-        }
-        if (a.vec && col < a.N) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            if (row[u] < 0) continue;
-            OT *dst = y + int64_t(row[u]) * a.N + col;
-            if constexpr (sizeof(OT) == 4) {
-              *reinterpret_cast<float4 *>(dst) =
-                  make_float4(d[0][2 * u], d[0][2 * u + 1], d[1][2 * u], d[1][2 * u + 1]);
-              *reinterpret_cast<float4 *>(dst + 4) =
-                  make_float4(d[2][2 * u], d[2][2 * u + 1], d[3][2 * u], d[3][2 * u + 1]);
-            } else {
-              uint32_t w[4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                w[q] = uint32_t(f2bf_bits(d[q][2 * u])) | (uint32_t(f2bf_bits(d[q][2 * u + 1])) << 16);
-              *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (row[u] >= 0 && col + e < a.N)
-                y[int64_t(row[u]) * a.N + col + e] = OT(d[e >> 1][2 * u + (e & 1)]);
+        if (has) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[b]);
+          ++blk;
         }
       }
     }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 2 * LE_COLS);
   }
 }
 
 // ------------------------------------------------------------------ wgrad
 struct LoraGradSide {
   const __nv_bfloat16 *v;      // [T, C] long side: x (dA) or dy (dB)
-  const float *u;              // [T, R] rank side: g (dA) or h (dB)
+  const __nv_bfloat16 *u;      // [LR_PARTS][T][Rp] rank side, sorted: g (dA) or h (dB), scaled
   int64_t C;
-  int ncb;                     // 256-column blocks
-  const float *scaling;        // multiplies u (NULL: 1)
+  int ncb;                     // 128-column blocks
   void *out;                   // [n, R, C] (r_major) or [n, C, R]
   int r_major;
   int vec;                     // v's rows are 16-byte aligned
@@ -716,17 +852,19 @@ struct LoraGradSide {
 struct LoraWgrad {
   LoraGradSide side[2];
   int R, Rp, n;
+  int64_t plane;               // T * Rp
   LoraPlan plan;
-  float *part;                 // [2 * grid][Rp][256] partial sums
+  float *part;                 // [2 * grid][Rp][128] partial sums
   uint32_t u_bytes;            // one bf16 part of a stage of u: (Rp / 8) * LG_MN_LD
 };
 
 constexpr int LG_THREADS = 416;
-constexpr int LG_COLS = 256;
-constexpr int LG_X_BYTES = LR_KB * LG_COLS * 2;     // 32 KB: 4 pieces of [64 tokens x 128 B]
+constexpr int LG_COLS = 128;
+constexpr int LG_X_BYTES = LR_KB * LG_COLS * 2;     // 16 KB: 2 pieces of [64 tokens x 128 B]
+constexpr int LG_MIN_STAGES = 8;                    // a CTA's least share, see k_lora_wgrad
 constexpr int LG_MN_LD = LR_KB * 16 + 16;
 __host__ __device__ __forceinline__ constexpr uint32_t lg_tmem_cols(int Rp) {
-  return Rp <= 32 ? 128u : Rp <= 64 ? 256u : 512u;   // two buffers of two accumulators
+  return Rp <= 32 ? 64u : Rp <= 64 ? 128u : 256u;   // two accumulators
 }
 
 // One piece of work of a CTA: stages [s0, s1) of one (side, adapter, column block).
@@ -760,16 +898,17 @@ __device__ __forceinline__ LoraSeg lora_seg(const LoraWgrad &a, int64_t s, int64
   return g;
 }
 
-// D[256 columns x Rp] = sum over an adapter's tokens, two M = 128 accumulators in TMEM; both
-// operands have the token index as their rows in memory, which is the MMA's contraction
-// index: v as 128-byte-swizzled pieces of 64 columns, u (its bf16 parts) as unswizzled groups
-// of 8.  The work of both gradients (every adapter's 64-token stages times the column blocks)
-// is one line that the CTAs cut into equal pieces: an item that one CTA covers is written at
-// once, one that a cut divides is written as fp32 partial sums (at most two per CTA) and the
-// last CTA to arrive adds them in order.  Warps 0-3 copy v, 4-7 split u, 8 issues the MMAs,
-// 9-12 read TMEM; accumulators are double-buffered, so an item's stores overlap the next one.
+// D[128 columns x Rp] = sum over an adapter's tokens, in TMEM; both operands have the token
+// index as their rows in memory, which is the MMA's contraction index: v as 128-byte-swizzled
+// pieces of 64 columns, u (its bf16 parts) as unswizzled groups of 8.  The work of both
+// gradients (every adapter's 64-token stages times the column blocks) is one line that the CTAs
+// cut into equal pieces: an item that one CTA covers is written at once, one that a cut divides
+// is written as fp32 partial sums (at most two per CTA) and the last CTA to arrive adds them in
+// order.  A piece is at least min(8, the average item's) stages: cutting a few microseconds of
+// loads costs more in the join than it saves.  Warps 0-3 copy v, 4-7 u, 8 issues the MMAs, 9-12
+// read TMEM; accumulators are double-buffered, so an item's stores overlap the next one.
 template <typename OT, int S>
-__global__ void __launch_bounds__(LG_THREADS, S == 3 ? 2 : 1) k_lora_wgrad(const LoraWgrad a) {
+__global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_wgrad(const LoraWgrad a) {
   constexpr int NS = sizeof(OT) == 4 ? 3 : 2;
   extern __shared__ uint8_t lg_raw[];
   uint8_t *smem = lg_raw + ((1024u - (smem_u32(lg_raw) & 1023u)) & 1023u);
@@ -779,10 +918,10 @@ __global__ void __launch_bounds__(LG_THREADS, S == 3 ? 2 : 1) k_lora_wgrad(const
   __shared__ uint32_t tmem_slot;
   __shared__ int last_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t cols = lg_tmem_cols(a.Rp), acc_cols = cols / 2, half_cols = cols / 4;
+  const uint32_t cols = lg_tmem_cols(a.Rp), acc_cols = cols / 2;
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 8);
+      mbar_init(&full[s], 256);
       mbar_init(&empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -800,8 +939,10 @@ __global__ void __launch_bounds__(LG_THREADS, S == 3 ? 2 : 1) k_lora_wgrad(const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int64_t all = int64_t(a.plan.stages[a.n]) * (a.side[0].ncb + a.side[1].ncb);
-  const int64_t per = (all + gridDim.x - 1) / gridDim.x;
+  const int64_t stages = a.plan.stages[a.n], all = stages * (a.side[0].ncb + a.side[1].ncb);
+  const int used = max(1, a.plan.head[1]);
+  const int64_t per = max((all + gridDim.x - 1) / gridDim.x,
+                          min(int64_t(LG_MIN_STAGES), (stages + used - 1) / used));
   const int64_t w0 = min(int64_t(blockIdx.x) * per, all), w1 = min(w0 + per, all);
 
   if (warp < 8) {
@@ -811,79 +952,57 @@ __global__ void __launch_bounds__(LG_THREADS, S == 3 ? 2 : 1) k_lora_wgrad(const
     for (int64_t s = w0; s < w1 && ok;) {
       const LoraSeg sg = lora_seg(a, s, w1);
       const LoraGradSide &sd = a.side[sg.side];
-      const int p0 = a.plan.off[sg.adapter], pn = a.plan.off[sg.adapter + 1];
-      const float sc = sd.scaling ? sd.scaling[sg.adapter] : 1.0f;
-      for (int q = 0; q < sg.count; ++q, ++it) {
-        const int st = it % S;
-        if (!mbar_wait(&empty[st], (uint32_t(it / S) & 1u) ^ 1u)) {
-          ok = false;
-          break;
+      const int p0 = a.plan.off[sg.adapter] + sg.first * LR_KB, pn = a.plan.off[sg.adapter + 1];
+      if (warp < 4) {
+        // 64 rows x 16 chunks of 16 bytes: a warp's half takes a row, 8 steps for its 16 rows
+        // (fields of sd in registers: the copies' memory clobbers would have them read again)
+        const int64_t c = int64_t(sg.cb) * LG_COLS + (lane & 15) * 8, C = sd.C;
+        const bool cin = c < C, vec = sd.vec != 0;
+        const __nv_bfloat16 *v0 = sd.v, *vc = v0 + c;
+        const uint32_t d0 = sx + ((lane & 15) >> 3) * 8192 + (warp * 16 + (lane >> 4)) * 128;
+        const int r16 = warp * 16 + (lane & 15);
+        int tok_n = p0 + r16 < pn ? a.plan.perm[p0 + r16] : -1;    // one stage ahead
+        for (int q = 0; q < sg.count; ++q, ++it) {
+          const int st = it % S;
+          const int tok_l = tok_n, nx = p0 + (q + 1) * LR_KB + r16;
+          tok_n = q + 1 < sg.count && nx < pn ? a.plan.perm[nx] : -1;
+          if (!(ok = mbar_wait(&empty[st], (uint32_t(it / S) & 1u) ^ 1u))) break;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int row8 = (2 * j + (lane >> 4)) & 7;
+            const int tok = __shfl_sync(0xffffffffu, tok_l, 2 * j + (lane >> 4));
+            const uint32_t d = d0 + st * LG_X_BYTES + j * 256 + (((lane & 7) ^ row8) << 4);
+            const bool in = tok >= 0 && cin;
+            const __nv_bfloat16 *src = in ? vc + int64_t(tok) * C : v0;
+            if (vec) stage8<true>(d, src, in ? 8 : 0);
+            else stage8<false>(d, src, in ? C - c : 0);
+          }
+          if (vec) stage_arrive<true>(&full[st]);
+          else stage_arrive<false>(&full[st]);
         }
-        const int pos = p0 + (sg.first + q) * LR_KB;       // sorted position of the stage's row 0
-        if (warp < 4) {
-          // 64 rows x 32 chunks of 16 bytes: a warp's 32 lanes take one row
-          const int64_t c = int64_t(sg.cb) * LG_COLS + lane * 8;
-          const uint32_t d0 = sx + st * LG_X_BYTES + (lane >> 3) * 8192;
-          // the token indices of this warp's 16 rows, one load a lane
-          const int mine = pos + warp * 16 + (lane & 15);
-          const int tok_l = mine < pn ? a.plan.perm[mine] : -1;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int row = warp * 16 + j;
-            const int tok = __shfl_sync(0xffffffffu, tok_l, j);
-            const uint32_t d = d0 + row * 128 + (((lane & 7) ^ (row & 7)) << 4);
-            const bool in = tok >= 0 && c < sd.C;
-            const __nv_bfloat16 *src = in ? sd.v + int64_t(tok) * sd.C + c : sd.v;
-            if (sd.vec) stage8<true>(d, src, in ? 8 : 0);
-            else stage8<false>(d, src, in ? sd.C - c : 0);
-          }
-          cp_async_commit();
-          if (it >= S - 2) {
-            cp_async_wait<S - 2>();
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[(it - (S - 2)) % S]);
-          }
-        } else {
-          const int e = tid - 128, row = e & 63;
-          const int tok = pos + row < pn ? a.plan.perm[pos + row] : -1;
-          const uint32_t d = su + st * u_stage + row * 16;
-          for (int g = e >> 6; g < (a.Rp >> 3); g += 2) {
-            float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (tok >= 0 && g * 8 < a.R) {
-              const float4 *src = reinterpret_cast<const float4 *>(sd.u + int64_t(tok) * a.R + g * 8);
-              const float4 v0 = __ldg(src), v1 = __ldg(src + 1);
-              f[0] = v0.x * sc; f[1] = v0.y * sc; f[2] = v0.z * sc; f[3] = v0.w * sc;
-              f[4] = v1.x * sc; f[5] = v1.y * sc; f[6] = v1.z * sc; f[7] = v1.w * sc;
-            }
-            uint32_t w[NS][4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              uint16_t plo[NS], phi[NS];
-              split_bf16<NS>(f[2 * x], plo);
-              split_bf16<NS>(f[2 * x + 1], phi);
-#pragma unroll
-              for (int i = 0; i < NS; ++i) w[i][x] = uint32_t(plo[i]) | (uint32_t(phi[i]) << 16);
-            }
+      } else {
+        const GridWalk u0(tid - 128, a.Rp >> 3);
+        const __nv_bfloat16 *ub = sd.u;
+        for (int q = 0; q < sg.count; ++q, ++it) {
+          const int st = it % S;
+          if (!(ok = mbar_wait(&empty[st], (uint32_t(it / S) & 1u) ^ 1u))) break;
+          const int pos = p0 + q * LR_KB;
+          const __nv_bfloat16 *up = ub + int64_t(pos) * a.Rp;
+#pragma unroll 4
+          for (GridWalk w = u0; w.major < LR_KB; w.next()) {
+            const bool in = pos + w.major < pn;
+            const __nv_bfloat16 *src = in ? up + w.major * a.Rp + w.minor * 8 : ub;
+            const uint32_t d = su + st * u_stage + w.minor * LG_MN_LD + w.major * 16;
 #pragma unroll
             for (int i = 0; i < NS; ++i)
-              st_shared16(d + i * a.u_bytes + g * LG_MN_LD,
-                          make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]));
+              cp_async16(d + i * a.u_bytes, src + (in ? i * a.plane : 0), in ? 16u : 0u);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[st]);
+          stage_arrive<true>(&full[st]);
         }
       }
       s += sg.count;
     }
-    if (warp < 4) {
-      cp_async_wait<0>();
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0 && ok)
-        for (int e = max(0, it - (S - 2)); e < it; ++e) mbar_arrive(&full[e % S]);
-    }
+    cp_async_wait_all();
   } else if (warp == 8) {
     // -------------------------------------------------------------- MMA issuer
     const uint32_t id = idesc_lora(a.Rp, 1, 1);
@@ -900,6 +1019,7 @@ __global__ void __launch_bounds__(LG_THREADS, S == 3 ? 2 : 1) k_lora_wgrad(const
           ok = false;
           break;
         }
+        fence_proxy_async_smem();
         tc_fence_after();
         const uint64_t dv = sdesc(sx + st * LG_X_BYTES, 8192, 1024, 2);
         const uint64_t du = sdesc(su + st * u_stage, 128, LG_MN_LD, 0);
@@ -907,11 +1027,9 @@ __global__ void __launch_bounds__(LG_THREADS, S == 3 ? 2 : 1) k_lora_wgrad(const
         for (int k = 0; k < 4; ++k)                 // 16 tokens an MMA
 #pragma unroll
           for (int i = 0; i < NS; ++i)
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
-              tc_mma_bf16_el(acc + hf * half_cols, dv + uint64_t(128 * k + 1024 * hf),
-                             du + uint64_t(16 * k) + uint64_t(i * (a.u_bytes >> 4)), id,
-                             (q || k || i) ? 1u : 0u);
+            tc_mma_bf16_el(acc, dv + uint64_t(128 * k),
+                           du + uint64_t(16 * k) + uint64_t(i * (a.u_bytes >> 4)), id,
+                           (q || k || i) ? 1u : 0u);
         tc_commit_el(&empty[st]);
       }
       if (!ok) break;
@@ -924,7 +1042,7 @@ __global__ void __launch_bounds__(LG_THREADS, S == 3 ? 2 : 1) k_lora_wgrad(const
   } else {
     // -------------------------------------------------------------- epilogue
     const int e4 = tid - 288;                       // 0 .. 127
-    const int q4 = warp & 3;                        // TMEM lanes 32 q4 .. + 31
+    const int col = 32 * (warp & 3) + lane;         // this thread's TMEM lane and column
     int seg = 0;
     bool ok = true;
     for (int64_t s = w0; s < w1; ++seg) {
@@ -933,22 +1051,19 @@ __global__ void __launch_bounds__(LG_THREADS, S == 3 ? 2 : 1) k_lora_wgrad(const
       // a warp whose wait ran out goes on without waiting: the others meet it at the barriers
       if (ok) ok = warp_wait(&acc_full[seg & 1], uint32_t(seg >> 1) & 1u);
       tc_fence_after();
-      const uint32_t acc = tmem + uint32_t(seg & 1) * acc_cols + (uint32_t(32 * q4) << 16);
+      const uint32_t acc = tmem + uint32_t(seg & 1) * acc_cols + (uint32_t(32 * (warp & 3)) << 16);
       const int64_t f = sg.item0 / per, l = (sg.item0 + sg.total - 1) / per;   // CTAs of the item
-      const int col = 32 * q4 + lane;               // this thread's column in each half
       OT *out = static_cast<OT *>(sd.out) + int64_t(sg.adapter) * a.R * sd.C;
-      const int slot = 2 * int(blockIdx.x) + (s == w0 ? 0 : 1);
-      float *mine = a.part + int64_t(slot) * a.Rp * LG_COLS;
       bool join = f == l;
       if (f != l) {
-        for (int hf = 0; hf < 2; ++hf)
-          for (int c0 = 0; c0 < a.Rp; c0 += 32) {
-            uint32_t v[32];
-            tmem_ld32(acc + hf * half_cols + c0, v);
+        float *mine = a.part + int64_t(2 * int(blockIdx.x) + (s == w0 ? 0 : 1)) * a.Rp * LG_COLS;
+        for (int c0 = 0; c0 < a.Rp; c0 += 32) {
+          uint32_t v[32];
+          tmem_ld32(acc + c0, v);
 #pragma unroll
-            for (int x = 0; x < 32; ++x)
-              if (c0 + x < a.R) mine[(c0 + x) * LG_COLS + hf * 128 + col] = __uint_as_float(v[x]);
-          }
+          for (int x = 0; x < 32; ++x)
+            if (c0 + x < a.R) __stcg(mine + (c0 + x) * LG_COLS + col, __uint_as_float(v[x]));
+        }
         __threadfence();
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (e4 == 0) last_s = atomicAdd(a.plan.tickets + f, 1) == int(l - f);
@@ -957,48 +1072,47 @@ __global__ void __launch_bounds__(LG_THREADS, S == 3 ? 2 : 1) k_lora_wgrad(const
         if (join) __threadfence();
       }
       if (join) {
-        for (int hf = 0; hf < 2; ++hf) {
-          const int64_t c = int64_t(sg.cb) * LG_COLS + hf * 128 + col;
-          for (int c0 = 0; c0 < a.Rp; c0 += 32) {
-            uint32_t v[32];
-            if (f == l) {
-              tmem_ld32(acc + hf * half_cols + c0, v);
+        const int64_t c = int64_t(sg.cb) * LG_COLS + col;
+        for (int c0 = 0; c0 < a.Rp; c0 += 32) {
+          uint32_t v[32];
+          if (f == l) {
+            tmem_ld32(acc + c0, v);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) v[x] = 0u;
+#pragma unroll 2
+            for (int64_t k = f; k <= l; ++k) {
+              const int sl = 2 * int(k) + (k == f && sg.item0 > f * per ? 1 : 0);
+              const float *src = a.part + int64_t(sl) * a.Rp * LG_COLS + col;
+#pragma unroll
+              for (int x = 0; x < 32; ++x)
+                if (c0 + x < a.R)
+                  v[x] = __float_as_uint(__uint_as_float(v[x]) + __ldcg(src + (c0 + x) * LG_COLS));
+            }
+          }
+          if (c < sd.C) {
+            if (sd.r_major) {
+#pragma unroll
+              for (int x = 0; x < 32; ++x)
+                if (c0 + x < a.R) out[int64_t(c0 + x) * sd.C + c] = OT(__uint_as_float(v[x]));
             } else {
 #pragma unroll
-              for (int x = 0; x < 32; ++x) v[x] = 0u;
-              for (int64_t k = f; k <= l; ++k) {
-                const int sl = 2 * int(k) + (k == f && sg.item0 > f * per ? 1 : 0);
-                const float *src = a.part + int64_t(sl) * a.Rp * LG_COLS + hf * 128 + col;
+              for (int x = 0; x < 32; x += 8)
+                if (c0 + x < a.R) {
+                  OT *dst = out + c * a.R + c0 + x;
+                  if constexpr (sizeof(OT) == 4) {
+                    *reinterpret_cast<uint4 *>(dst) = make_uint4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+                    *reinterpret_cast<uint4 *>(dst + 4) =
+                        make_uint4(v[x + 4], v[x + 5], v[x + 6], v[x + 7]);
+                  } else {
+                    uint32_t w[4];
 #pragma unroll
-                for (int x = 0; x < 32; ++x)
-                  if (c0 + x < a.R)
-                    v[x] = __float_as_uint(__uint_as_float(v[x]) + __ldcg(src + (c0 + x) * LG_COLS));
-              }
-            }
-            if (c < sd.C) {
-              if (sd.r_major) {
-#pragma unroll
-                for (int x = 0; x < 32; ++x)
-                  if (c0 + x < a.R) out[int64_t(c0 + x) * sd.C + c] = OT(__uint_as_float(v[x]));
-              } else {
-#pragma unroll
-                for (int x = 0; x < 32; x += 8)
-                  if (c0 + x < a.R) {
-                    OT *dst = out + c * a.R + c0 + x;
-                    if constexpr (sizeof(OT) == 4) {
-                      *reinterpret_cast<uint4 *>(dst) = make_uint4(v[x], v[x + 1], v[x + 2], v[x + 3]);
-                      *reinterpret_cast<uint4 *>(dst + 4) =
-                          make_uint4(v[x + 4], v[x + 5], v[x + 6], v[x + 7]);
-                    } else {
-                      uint32_t w[4];
-#pragma unroll
-                      for (int y = 0; y < 4; ++y)
-                        w[y] = uint32_t(f2bf_bits(__uint_as_float(v[x + 2 * y]))) |
-                               (uint32_t(f2bf_bits(__uint_as_float(v[x + 2 * y + 1]))) << 16);
-                      *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                    for (int y = 0; y < 4; ++y)
+                      w[y] = uint32_t(f2bf_bits(__uint_as_float(v[x + 2 * y]))) |
+                             (uint32_t(f2bf_bits(__uint_as_float(v[x + 2 * y + 1]))) << 16);
+                    *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
                   }
-              }
+                }
             }
           }
         }
