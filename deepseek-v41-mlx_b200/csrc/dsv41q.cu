@@ -893,25 +893,26 @@ int lora_rp(int64_t R) { return int((R + 15) / 16 * 16); }
 // the most tiles that T tokens on n adapters (and none) can make
 int64_t lora_max_tiles(int64_t T, int64_t n) { return T / LR_TILE + std::min(n + 1, T); }
 
+// 64-row blocks of the parts: an adapter's last one is padded
+int64_t lora_max_blocks(int64_t T, int64_t n) { return T / LR_KB + std::min(n, T); }
+
 // wgrad: stages of the ring, CTAs an SM and the grid.  Four or five stages that fit twice into
 // an SM run as two CTAs (one's joins and stores behind the other's loads); larger ones as one
 // CTA of up to six.
 struct LoraWgradShape {
   int stages, grid;
   size_t smem;
-  uint32_t u_bytes;
 };
 LoraWgradShape lora_wgrad_shape(int64_t T, int64_t K, int64_t N, int64_t n, int64_t R,
                                 int grad_dtype) {
   LoraWgradShape s;
   const int Rp = lora_rp(R), ns = grad_dtype == DSV41_F32 ? 3 : 2;
-  s.u_bytes = uint32_t(Rp / 8) * LG_MN_LD;
-  const size_t stage = LG_X_BYTES + size_t(ns) * s.u_bytes;
+  const size_t stage = LG_X_BYTES + size_t(ns) * Rp * 128;
   const int twice = int((112 * 1024 - 1024) / stage), once = int((224 * 1024 - 1024) / stage);
   const bool two = twice >= 4;
   s.stages = two ? std::min(twice, 5) : std::min(once, 6);
   s.smem = s.stages * stage + 1024;
-  const int64_t work = (T / LR_KB + std::min(n, T)) * (ceil_div(K, LG_COLS) + ceil_div(N, LG_COLS));
+  const int64_t work = lora_max_blocks(T, n) * (ceil_div(K, LG_COLS) + ceil_div(N, LG_COLS));
   s.grid = int(std::max<int64_t>(1, std::min<int64_t>(work, int64_t(num_sms()) * (two ? 2 : 1))));
   return s;
 }
@@ -919,7 +920,6 @@ LoraWgradShape lora_wgrad_shape(int64_t T, int64_t K, int64_t N, int64_t n, int6
 struct LoraWs {
   LoraPlan plan;
   __nv_bfloat16 *parts, *h_parts;
-  int64_t plane;
   float *sums;
   bool ok;
   size_t used;
@@ -933,10 +933,10 @@ LoraWs lora_carve(void *ws, size_t cap, int64_t T, int64_t K, int64_t N, int64_t
   w.plan.head = c.take<int>(2);
   w.plan.off = c.take<int>(n + 2);
   w.plan.stages = c.take<int>(n + 1);
-  w.plane = T * lora_rp(R);
-  w.parts = c.take<__nv_bfloat16>(LR_PARTS * w.plane);
+  const size_t parts = size_t(LR_PARTS) * lora_max_blocks(T, n) * 64 * lora_rp(R);
+  w.parts = c.take<__nv_bfloat16>(parts);
   if (backward) {
-    w.h_parts = c.take<__nv_bfloat16>(LR_PARTS * w.plane);
+    w.h_parts = c.take<__nv_bfloat16>(parts);
     // the larger of the two grids (bf16 and fp32 gradients)
     const int grid = std::max(lora_wgrad_shape(T, K, N, n, R, DSV41_BF16).grid,
                               lora_wgrad_shape(T, K, N, n, R, DSV41_F32).grid);
@@ -949,9 +949,42 @@ LoraWs lora_carve(void *ws, size_t cap, int64_t T, int64_t K, int64_t N, int64_t
   return w;
 }
 
+// [rows, cols] of 2- or 4-byte values as 128-byte pieces of single rows and of groups of rows
+int lora_rows_maps(LoraRows *m, const void *p, int64_t rows, int64_t cols, size_t esize) {
+  const CUtensorMapDataType dt =
+      esize == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint32_t box = uint32_t(128 / esize);
+  int rc = make_tmap_2d(&m->gather, p, dt, cols, rows, cols * esize, box, 1);
+  if (!rc) rc = make_tmap_2d(&m->run, p, dt, cols, rows, cols * esize, box, LR_GROUP);
+  return rc;
+}
+
+// A bank [n][rows][cols] of bf16, box bx x by of one adapter, swizzled by the box's row
+int lora_bank_map(CUtensorMap *m, const void *p, int64_t n, int64_t rows, int64_t cols, uint32_t bx,
+                  uint32_t by) {
+  int rc = get_encoder();
+  if (rc) return rc;
+  cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(n)};
+  cuuint64_t strides[2] = {cuuint64_t(cols) * 2, cuuint64_t(rows) * cols * 2};
+  cuuint32_t box[3] = {bx, by, 1}, estr[3] = {1, 1, 1};
+  const CUtensorMapSwizzle swz = bx == 64   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                 : bx == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                 : bx == 16 ? CU_TENSOR_MAP_SWIZZLE_32B
+                                            : CU_TENSOR_MAP_SWIZZLE_NONE;
+  const CUresult r = g_encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(p), dims,
+                                    strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(DSV41_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return DSV41_OK;
+}
+
+// values of r a piece (LoraPieces)
+int lora_pw(int64_t R) { return R % 64 == 0 ? 64 : R % 32 == 0 ? 32 : R % 16 == 0 ? 16 : 8; }
+
 int lora_plan_launch(const int32_t *ids, int64_t T, int64_t n, const LoraPlan &plan,
                      cudaStream_t st) {
-  const size_t smem = size_t(4) * (n + 1) * 4;
+  const size_t smem = size_t(5) * (n + 1) * 4;
   DSV41_LAUNCH(max_dynamic_smem(k_lora_plan, smem), "lora_plan");
   const unsigned C = unsigned(std::min<int64_t>(LP_MAX_CTAS, ceil_div(T, 1024)));
   ProfScope prof("lora_plan", st);
@@ -975,11 +1008,12 @@ cudaError_t lora_decode_launch(const LoraDecode &p, int64_t T, cudaStream_t st) 
 }
 
 template <bool WMN, bool VEC, int S>
-cudaError_t lora_shrink_go(const LoraShrink &a, unsigned clusters, unsigned C, cudaStream_t st) {
-  const size_t smem = size_t(S) * (LS_X_BYTES + a.w_bytes) + 1024;
+cudaError_t lora_shrink_go(const LoraShrinkMaps &maps, const LoraShrink &a, unsigned clusters,
+                           unsigned C, cudaStream_t st) {
+  const size_t smem = size_t(S) * (LS_X_BYTES + a.Rp * 128) + 1024;
   cudaError_t e = max_dynamic_smem(k_lora_shrink<WMN, VEC, S>, smem);
   if (e != cudaSuccess) return e;
-  return launch_cluster(k_lora_shrink<WMN, VEC, S>, clusters * C, C, LS_THREADS, smem, st, a);
+  return launch_cluster(k_lora_shrink<WMN, VEC, S>, clusters * C, C, LS_THREADS, smem, st, maps, a);
 }
 
 // The contraction is split over the CTAs of a cluster as far as the tiles leave SMs free (two
@@ -990,51 +1024,69 @@ int lora_shrink_launch(LoraShrink a, int64_t T, cudaStream_t st) {
   unsigned C = 8;
   while (C > 1 && (ceil_div(T, LR_TILE) * C > slots || C > nkb)) C >>= 1;
   const unsigned clusters = unsigned(std::min<int64_t>(lora_max_tiles(T, a.n), slots / C));
-  a.w_bytes = WMN ? uint32_t(a.Rp / 8) * LS_MN_LD : uint32_t(a.Rp) * 128;
+  a.T = T;
+  a.pw = lora_pw(a.R);
+  LoraShrinkMaps maps{};
+  int rc = WMN ? lora_bank_map(&maps.w, a.w, a.n, a.K, a.R, uint32_t(a.pw), LR_KB)
+               : lora_bank_map(&maps.w, a.w, a.n, a.R, a.K, LR_KB, uint32_t(a.R));
+  if (!rc && VEC) rc = lora_rows_maps(&maps.x, a.x, T, a.K, 2);
+  if (rc) return rc;
   ProfScope prof("lora_shrink", st);
-  if (a.Rp <= 32) DSV41_LAUNCH((lora_shrink_go<WMN, VEC, 5>(a, clusters, C, st)), "lora_shrink");
-  else if (a.Rp <= 64) DSV41_LAUNCH((lora_shrink_go<WMN, VEC, 4>(a, clusters, C, st)), "lora_shrink");
-  else DSV41_LAUNCH((lora_shrink_go<WMN, VEC, 3>(a, clusters, C, st)), "lora_shrink");
+  if (a.Rp <= 32) DSV41_LAUNCH((lora_shrink_go<WMN, VEC, 5>(maps, a, clusters, C, st)), "lora_shrink");
+  else if (a.Rp <= 64) DSV41_LAUNCH((lora_shrink_go<WMN, VEC, 4>(maps, a, clusters, C, st)), "lora_shrink");
+  else DSV41_LAUNCH((lora_shrink_go<WMN, VEC, 3>(maps, a, clusters, C, st)), "lora_shrink");
   return DSV41_OK;
 }
 
-// Work items of up to 16 column blocks, about three for each CTA that runs at once.
+// Work items of up to 32 column blocks (128 bytes of a row each), about three for each CTA; the
+// rest of the shared memory is the ring of base and output tiles.
 template <bool WMN, typename OT>
 int lora_expand_launch(LoraExpand a, int64_t T, cudaStream_t st) {
+  constexpr int CB = 128 / int(sizeof(OT));
   a.Rp = lora_rp(a.R);
-  a.a_bytes = uint32_t((sizeof(OT) == 4 ? 3 : 2) * (a.Rp / 8)) * LE_LD;
-  a.w_bytes = WMN ? uint32_t(LE_COLS / 8) * (a.Rp * 16 + 16) : uint32_t(a.Rp / 8) * LE_LD;
-  const size_t smem = a.a_bytes + 2 * a.w_bytes + LE_EPI_BYTES;
-  const int64_t slots = int64_t(num_sms()) * (smem <= 112 * 1024 ? 2 : 1);
-  a.ncb = int(ceil_div(a.N, LE_COLS));
-  a.cpu = int(std::max<int64_t>(1, std::min<int64_t>(16, ceil_div(T, LR_TILE) * a.ncb / (3 * slots))));
+  a.pw = lora_pw(a.R);
+  const size_t rest = size_t((sizeof(OT) == 4 ? 3 : 2) * (a.Rp / 8)) * 2048 +
+                      size_t(LE_BUF) * CB * a.Rp * 2 + 1024;
+  a.ring = int(std::min<size_t>(LE_RING_MAX, (225 * 1024 - rest) / LE_TILE_BYTES)) & ~1;
+  const size_t smem = rest + size_t(a.ring) * LE_TILE_BYTES;
+  const int64_t slots = num_sms();
+  a.ncb = int(ceil_div(a.N, CB));
+  a.cpu = int(std::max<int64_t>(1, std::min<int64_t>(32, ceil_div(T, LR_TILE) * a.ncb / (3 * slots))));
   a.vec = a.N * sizeof(OT) % 16 == 0 && aligned(a.base, 16) && aligned(a.y, 16);
+  LoraExpandMaps maps{};
+  int rc = WMN ? lora_bank_map(&maps.w, a.w, a.n, a.R, a.N, CB, uint32_t(a.R))
+               : lora_bank_map(&maps.w, a.w, a.n, a.N, a.R, uint32_t(a.pw), CB);
+  if (!rc && a.vec && a.base) rc = lora_rows_maps(&maps.base, a.base, T, a.N, sizeof(OT));
+  if (!rc && a.vec) rc = lora_rows_maps(&maps.y, a.y, T, a.N, sizeof(OT));
+  if (rc) return rc;
   const unsigned grid = unsigned(std::min<int64_t>(
       lora_max_tiles(T, a.n) * ceil_div(a.ncb, a.cpu), slots));
   ProfScope prof("lora_expand", st);
   cudaError_t e = max_dynamic_smem(k_lora_expand<WMN, OT>, smem);
   if (e == cudaSuccess) {
-    k_lora_expand<WMN, OT><<<grid, LE_THREADS, smem, st>>>(a);
+    k_lora_expand<WMN, OT><<<grid, LE_THREADS, smem, st>>>(maps, a);
     e = cudaGetLastError();
   }
   return cuda_status(e, "lora_expand");
 }
 
 template <typename OT, int S>
-cudaError_t lora_wgrad_go(const LoraWgrad &a, const LoraWgradShape &sh, cudaStream_t st) {
+cudaError_t lora_wgrad_go(const LoraWgradMaps &m, const LoraWgrad &a, const LoraWgradShape &sh,
+                          cudaStream_t st) {
   cudaError_t e = max_dynamic_smem(k_lora_wgrad<OT, S>, sh.smem);
   if (e != cudaSuccess) return e;
-  k_lora_wgrad<OT, S><<<unsigned(sh.grid), LG_THREADS, sh.smem, st>>>(a);
+  k_lora_wgrad<OT, S><<<unsigned(sh.grid), LG_THREADS, sh.smem, st>>>(m, a);
   return cudaGetLastError();
 }
 
 template <typename OT>
-cudaError_t lora_wgrad_launch(const LoraWgrad &a, const LoraWgradShape &sh, cudaStream_t st) {
+cudaError_t lora_wgrad_launch(const LoraWgradMaps &m, const LoraWgrad &a, const LoraWgradShape &sh,
+                              cudaStream_t st) {
   switch (sh.stages) {
-    case 6: return lora_wgrad_go<OT, 6>(a, sh, st);
-    case 5: return lora_wgrad_go<OT, 5>(a, sh, st);
-    case 4: return lora_wgrad_go<OT, 4>(a, sh, st);
-    default: return lora_wgrad_go<OT, 3>(a, sh, st);
+    case 6: return lora_wgrad_go<OT, 6>(m, a, sh, st);
+    case 5: return lora_wgrad_go<OT, 5>(m, a, sh, st);
+    case 4: return lora_wgrad_go<OT, 4>(m, a, sh, st);
+    default: return lora_wgrad_go<OT, 3>(m, a, sh, st);
   }
 }
 
@@ -1085,13 +1137,13 @@ extern "C" int dsv41_lora_forward(const void *x, int64_t T, int64_t K, const voi
   s.scaling = scaling;
   s.out = h_out;
   s.parts = w.parts;
-  s.plane = w.plane;
+  s.np = out_dtype == DSV41_F32 ? 3 : 2;
   s.plan = w.plan;
   rc = lora_shrink_launch<false, true>(s, T, st);
   if (rc) return rc;
   LoraExpand e{};
   e.parts = w.parts;
-  e.plane = w.plane;
+  e.np = s.np;
   e.w = static_cast<const __nv_bfloat16 *>(b);
   e.N = N;
   e.R = int(R);
@@ -1145,13 +1197,13 @@ extern "C" int dsv41_lora_backward(const void *dy, const void *x, const float *h
   s.parts = w.parts;
   s.h = h;
   s.h_parts = w.h_parts;
-  s.plane = w.plane;
+  s.np = dx_dtype == DSV41_F32 || grad_dtype == DSV41_F32 ? 3 : 2;
   s.plan = w.plan;
   rc = N % 8 == 0 ? lora_shrink_launch<true, true>(s, T, st) : lora_shrink_launch<true, false>(s, T, st);
   if (rc) return rc;
   LoraExpand e{};
   e.parts = w.parts;
-  e.plane = w.plane;
+  e.np = s.np;
   e.w = static_cast<const __nv_bfloat16 *>(a);
   e.N = K;
   e.R = int(R);
@@ -1169,13 +1221,17 @@ extern "C" int dsv41_lora_backward(const void *dy, const void *x, const float *h
   g.R = int(R);
   g.Rp = lora_rp(R);
   g.n = int(n);
-  g.plane = w.plane;
+  g.np = s.np;
+  g.T = T;
   g.plan = w.plan;
   g.part = w.sums;
-  g.u_bytes = sh.u_bytes;
+  LoraWgradMaps maps{};
+  rc = lora_rows_maps(&maps.v[0], x, T, K, 2);
+  if (!rc && N % 8 == 0) rc = lora_rows_maps(&maps.v[1], dy, T, N, 2);
+  if (rc) return rc;
   ProfScope prof("lora_wgrad", st);
-  const cudaError_t ge = grad_dtype == DSV41_F32 ? lora_wgrad_launch<float>(g, sh, st)
-                                                 : lora_wgrad_launch<__nv_bfloat16>(g, sh, st);
+  const cudaError_t ge = grad_dtype == DSV41_F32 ? lora_wgrad_launch<float>(maps, g, sh, st)
+                                                 : lora_wgrad_launch<__nv_bfloat16>(maps, g, sh, st);
   return cuda_status(ge, "lora_wgrad");
 }
 

@@ -33,10 +33,11 @@ constexpr int LR_KB = 64;           // contraction length of a stage
 // ------------------------------------------------------------------ plan
 struct LoraPlan {
   int *perm;       // [T] token of sorted position p
-  int4 *tiles;     // {adapter (n: none), first position, rows, 0}
+  int4 *tiles;     // {adapter (n: none), first position, rows, first 64-row block of the parts}
   int *head;       // [2] tiles, adapters with tokens
   int *off;        // [n + 2] first position of each adapter (n: none), then T
-  int *stages;     // [n + 1] 64-token stages of the adapters before this one (wgrad's work)
+  int *stages;     // [n + 1] 64-row blocks of the adapters before this one: where an adapter's
+                   // parts begin, and wgrad's work
   int *tickets;    // zeroed here: wgrad's joins
   int n_tickets;
 };
@@ -83,7 +84,8 @@ constexpr int LP_MAX_CTAS = 8;
 __global__ void __launch_bounds__(1024, 1)
     k_lora_plan(const int32_t *__restrict__ ids, int T, int n, LoraPlan p) {
   extern __shared__ int lp_smem[];                                    // [n + 1] each
-  int *cnt = lp_smem, *pos = cnt + (n + 1), *tile0 = pos + (n + 1), *first = tile0 + (n + 1);
+  int *cnt = lp_smem, *pos = cnt + (n + 1), *tile0 = pos + (n + 1), *first = tile0 + (n + 1),
+      *block0 = first + (n + 1);
   __shared__ int wsum[32][3];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = gridDim.x, rank = blockIdx.x;
@@ -119,9 +121,10 @@ __global__ void __launch_bounds__(1024, 1)
       first[b] = run[0] + v[0] - total;
       pos[b] = first[b] + before;
       tile0[b] = run[1] + v[1] - nt;
+      block0[b] = run[2] + v[2] - ns;
       if (rank == 0) {
         p.off[b] = first[b];
-        p.stages[b] = run[2] + v[2] - ns;
+        p.stages[b] = block0[b];
         if (b == n) p.off[n + 1] = T;
       }
     }
@@ -142,7 +145,8 @@ __global__ void __launch_bounds__(1024, 1)
       else hi = mid - 1;
     }
     const int p0 = first[lo] + (i - tile0[lo]) * LR_TILE;
-    p.tiles[i] = make_int4(lo, p0, min(LR_TILE, (lo == n ? T : first[lo + 1]) - p0), 0);
+    p.tiles[i] = make_int4(lo, p0, min(LR_TILE, (lo == n ? T : first[lo + 1]) - p0),
+                           block0[lo] + (i - tile0[lo]) * (LR_TILE / LR_KB));
   }
   // scatter: batches of 1024 tokens, their warps one after another
   for (int b0 = t0; b0 < t1; b0 += 1024) {
@@ -185,68 +189,163 @@ __device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lbo, uint32_t
   return uint64_t((saddr >> 4) & 0x3FFF) | (uint64_t(lbo >> 4) << 16) |
          (uint64_t(sbo >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(swz) << 61);
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t src_bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(src_bytes)
-               : "memory");
+// Four rows of a [rows][columns] tensor map whose box is 128 bytes of one row, by row index: 512
+// bytes, 128-byte swizzle.  A converged warp runs it, one elected lane issues.
+__device__ __forceinline__ void tma_gather4_el(uint32_t dst, const CUtensorMap *map, uint64_t *bar,
+                                               int32_t x, int4 rows) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z),
+      "r"(rows.w), "r"(smem_u32(bar))
+      : "memory");
 }
-// the same, asking L2 for the 256 bytes around it: rows are walked 128 bytes a stage
-__device__ __forceinline__ void cp_async16_256(uint32_t dst, const void *src, uint32_t src_bytes) {
-  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(src_bytes)
-               : "memory");
+__device__ __forceinline__ void tma_load_3d_el(uint32_t dst, const CUtensorMap *map, uint64_t *bar,
+                                               int32_t x, int32_t y, int32_t z) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
 }
-__device__ __forceinline__ void cp_async_wait_all() {
-  asm volatile("cp.async.wait_all;" ::: "memory");
+__device__ __forceinline__ void tma_rows_el(uint32_t dst, const CUtensorMap *map, uint64_t *bar,
+                                            int32_t x, int32_t y) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
 }
-// This thread's part of a stage is on its way: its arrival on `full` follows its copies.  The
-// MMA warp fences the proxies once it has seen the barrier.  Element stores are fenced and released
-// by the thread itself.
-template <bool VEC> __device__ __forceinline__ void stage_arrive(uint64_t *full) {
-  if constexpr (VEC) {
-    cp_async_arrive_noinc(full);
-  } else {
-    cp_async_wait_all();
-    fence_proxy_async_smem();
-    mbar_arrive(full);
+// The other direction; completion by bulk groups of the elected lane (elect.sync picks the same
+// lane of a full warp every time).
+__device__ __forceinline__ void tma_scatter4_el(const CUtensorMap *map, uint32_t src, int32_t x,
+                                                int4 rows) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.global.shared::cta.tile::scatter4.bulk_group"
+      " [%0, {%1, %2, %3, %4, %5}], [%6];\n\t}" ::"l"(reinterpret_cast<uint64_t>(map)),
+      "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(src)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_rows_el(const CUtensorMap *map, uint32_t src, int32_t x,
+                                                  int32_t y) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n\t}" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(x), "r"(y), "r"(src)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_commit_el() {
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+               "@e cp.async.bulk.commit_group;\n\t}" ::: "memory");
+}
+// every bulk store of the elected lane has read its shared memory / is complete
+__device__ __forceinline__ void bulk_wait_read_el() {
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+               "@e cp.async.bulk.wait_group.read 0;\n\t}" ::: "memory");
+  __syncwarp();
+}
+__device__ __forceinline__ void bulk_wait_el() {
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+               "@e cp.async.bulk.wait_group 0;\n\t}" ::: "memory");
+  __syncwarp();
+}
+
+// The 16 token rows of a group, as a warp holds them: lane l's tok is the token of row l & 15
+// (missing rows repeat the last one).  Sorting is stable, so tokens ascend: the group is one run
+// of rows if its last and first are as far apart as their places.
+constexpr int LR_GROUP = 16;
+struct LoraRows {
+  CUtensorMap gather, run;     // boxes of 128 bytes of one row / of LR_GROUP rows
+};
+// 128 bytes of each of the group's first `rows` rows to shared memory (the rest of the group may
+// be filled too): one TMA instruction for a run of rows, else one for every four.
+__device__ __forceinline__ uint32_t lora_rows_bytes(bool run, int rows) {
+  return run ? LR_GROUP * 128 : uint32_t((rows + 3) >> 2) * 512;
+}
+__device__ __forceinline__ void lora_rows_load(uint32_t dst, const LoraRows &m, uint64_t *bar, int x,
+                                               int tok, bool run, int rows) {
+  if (run) {
+    tma_rows_el(dst, &m.run, bar, x, __shfl_sync(0xffffffffu, tok, 0));
+    return;
   }
+  for (int j = 0; 4 * j < rows; ++j)
+    tma_gather4_el(dst + j * 512, &m.gather, bar, x,
+                   make_int4(__shfl_sync(0xffffffffu, tok, 4 * j), __shfl_sync(0xffffffffu, tok, 4 * j + 1),
+                             __shfl_sync(0xffffffffu, tok, 4 * j + 2),
+                             __shfl_sync(0xffffffffu, tok, 4 * j + 3)));
 }
 __device__ __forceinline__ void st_shared16(uint32_t dst, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y),
                "r"(v.z), "r"(v.w)
                : "memory");
 }
-// Items e = tid + 128 i of a [major][minor] grid, without a division an item.
-struct GridWalk {
-  int major, minor, dmajor, dminor, n;
-  __device__ __forceinline__ GridWalk(int e, int n_minor)
-      : major(e / n_minor), minor(e % n_minor), dmajor(128 / n_minor), dminor(128 % n_minor),
-        n(n_minor) {}
-  __device__ __forceinline__ void next() {
-    major += dmajor;
-    minor += dminor;
-    if (minor >= n) {
-      minor -= n;
-      ++major;
+// Eight bf16 values of a row that starts anywhere (rows of a length that is no multiple of 8) to
+// shared memory, zeros past `valid` of them (<= 0: nothing is read): the one or two aligned
+// 16-byte words that hold them, shifted.  `end`: the tensor's end, past which no word is read.
+__device__ __forceinline__ void stage8_any(uint32_t dst, const __nv_bfloat16 *src, int64_t valid,
+                                           const __nv_bfloat16 *end) {
+  uint4 o = make_uint4(0, 0, 0, 0);
+  if (valid > 0) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(src), lo = at & ~uintptr_t(15);
+    const int sh = int(at & 15) >> 1;                       // elements before src in its word
+    const int n = valid < 8 ? int(valid) : 8;
+    if (lo + 32 <= reinterpret_cast<uintptr_t>(end)) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4 *>(lo));
+      const uint4 v = sh + n > 8 ? __ldg(reinterpret_cast<const uint4 *>(lo) + 1) : o;
+      const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+      uint32_t r[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t a = 0, b = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (q == (sh >> 1)) {
+            a = w[i + q];
+            b = w[i + q + 1 < 8 ? i + q + 1 : 7];
+          }
+        r[i] = (sh & 1) ? __funnelshift_r(a, b, 16) : a;
+        const int left = n - 2 * i;
+        r[i] &= left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u;
+      }
+      o = make_uint4(r[0], r[1], r[2], r[3]);
+    } else {
+      uint32_t w[4] = {0, 0, 0, 0};
+      const uint16_t *s = reinterpret_cast<const uint16_t *>(src);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < n) w[e >> 1] |= uint32_t(__ldg(s + e)) << (16 * (e & 1));
+      o = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
-};
-// Eight bf16 values of a row to shared memory, zeros past `valid` of them (valid <= 0: none is
-// read).  VEC: the row is 16-byte aligned and valid is 0 or >= 8 (one asynchronous copy);
-// otherwise (rows of a length that is no multiple of 8) element loads.
-template <bool VEC>
-__device__ __forceinline__ void stage8(uint32_t dst, const __nv_bfloat16 *src, int64_t valid) {
-  if constexpr (VEC) {
-    cp_async16_256(dst, src, valid > 0 ? 16u : 0u);
-  } else {
-    uint32_t w[4] = {0, 0, 0, 0};
-    const uint16_t *s = reinterpret_cast<const uint16_t *>(src);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < valid) w[e >> 1] |= uint32_t(__ldg(s + e)) << (16 * (e & 1));
-    st_shared16(dst, make_uint4(w[0], w[1], w[2], w[3]));
-  }
+  st_shared16(dst, o);
 }
+
+// A bank's matrix [rows][R] (contiguous in r) comes to shared memory in pieces of pw values of
+// r, pw the largest of 64, 32, 16, 8 that divides R: rows of 2 pw bytes under the swizzle of that
+// width (none for 8), which is the tensor core's canonical layout with either index contracted.
+struct LoraPieces {
+  uint32_t swz, rb;            // descriptor's layout type; bytes of a row of a piece
+  __device__ __forceinline__ explicit LoraPieces(int pw)
+      : swz(pw == 64 ? 2u : pw == 32 ? 4u : pw == 16 ? 6u : 0u), rb(uint32_t(pw) * 2) {}
+  // r is not contracted (rows are), `rows` of them staged
+  __device__ __forceinline__ uint64_t desc_mn(uint32_t at, uint32_t rows) const {
+    return swz ? sdesc(at, rows * rb, 8 * rb, swz) : sdesc(at, 128, rows * 16, 0);
+  }
+  __device__ __forceinline__ uint32_t step_mn() const { return 16 * rb; }      // 16 rows
+  // r is contracted
+  __device__ __forceinline__ uint64_t desc_k(uint32_t at, uint32_t rows) const {
+    return swz ? sdesc(at, 16, 8 * rb, swz) : sdesc(at, rows * 16, 128, 0);
+  }
+  __device__ __forceinline__ uint32_t off_k(uint32_t k, uint32_t rows) const {  // k16 step k
+    const uint32_t b = 32 * k;
+    return swz ? b / rb * (rows * rb) + b % rb : 2 * k * rows * 16;
+  }
+};
 
 // v as bf16 parts; the rest after each part is exact in fp32 (and zero after an infinity or NaN).
 template <int NS>
@@ -258,51 +357,65 @@ __device__ __forceinline__ void split_bf16(float v, uint16_t (&p)[NS]) {
   }
 }
 
-// Four values times sc to their parts: LR_PARTS planes of [T][Rp], `plane` apart.
+// The parts in memory: blocks of 64 sorted rows of one adapter (its last block padded with zero
+// rows), [block][part][Rp / 8][64 rows][8]: the order in which a tensor core takes a 64-row (or,
+// two blocks, 128-row) operand without swizzle, so that a block is one or a few bulk copies.
 constexpr int LR_PARTS = 3;
-__device__ __forceinline__ void store_parts(__nv_bfloat16 *dst, int64_t plane, float4 v, float sc) {
+__device__ __forceinline__ void store_parts(__nv_bfloat16 *parts, int np, int Rp, int block, int row,
+                                            int c4, float4 v, float sc) {
   uint16_t p[4][LR_PARTS];
   split_bf16<LR_PARTS>(v.x * sc, p[0]);
   split_bf16<LR_PARTS>(v.y * sc, p[1]);
   split_bf16<LR_PARTS>(v.z * sc, p[2]);
   split_bf16<LR_PARTS>(v.w * sc, p[3]);
+  __nv_bfloat16 *dst = parts + int64_t(block + (row >> 6)) * np * Rp * 64 + (c4 >> 3) * 512 +
+                       (row & 63) * 8 + (c4 & 7);
 #pragma unroll
   for (int i = 0; i < LR_PARTS; ++i)
-    *reinterpret_cast<uint2 *>(dst + i * plane) = make_uint2(
-        uint32_t(p[0][i]) | (uint32_t(p[1][i]) << 16), uint32_t(p[2][i]) | (uint32_t(p[3][i]) << 16));
+    if (i < np)
+      *reinterpret_cast<uint2 *>(dst + i * Rp * 64) = make_uint2(
+          uint32_t(p[0][i]) | (uint32_t(p[1][i]) << 16),
+          uint32_t(p[2][i]) | (uint32_t(p[3][i]) << 16));
 }
 
 // ------------------------------------------------------------------ shrink
 struct LoraTile {
-  int adapter, p0, rows;       // n: none; first sorted position; rows <= LR_TILE
+  int adapter, p0, rows, block;     // n: none; first sorted position; rows <= LR_TILE
 };
 struct LoraShrink {
   const __nv_bfloat16 *x;      // [T, K]
+  int64_t T;
   int64_t K;                   // contraction length
   const __nv_bfloat16 *w;      // [n][R][K], or [n][K][R] (WMN)
   int R, Rp, n;                // Rp: R rounded up to 16
   const float *scaling;        // NULL: 1
   float *out;                  // [T, R] the product as it is, or NULL
-  __nv_bfloat16 *parts;        // [LR_PARTS][T][Rp] the product times scaling, sorted order
+  __nv_bfloat16 *parts;        // the product times scaling, np parts
   const float *h;              // [T, R] or NULL: a second value to scale and split the same way
   __nv_bfloat16 *h_parts;
-  int64_t plane;               // T * Rp
+  int np;
   LoraPlan plan;
-  uint32_t w_bytes;            // staged bytes of w in a stage
+  int pw;                      // WMN: see LoraPieces
+};
+struct LoraShrinkMaps {
+  LoraRows x;
+  CUtensorMap w;               // [n][R][K], box 64 k x R; WMN: [n][K][R], box pw x 64 k
 };
 
 constexpr int LS_THREADS = 160;
 constexpr int LS_X_BYTES = LR_TILE * LR_KB * 2;     // 16 KB
-constexpr int LS_MN_LD = LR_KB * 16 + 16;           // bytes between 8-wide r groups (WMN)
 
 // D[128 tokens x Rp] in TMEM: tcgen05.mma kind::f16, M = 128, N = Rp.  A cluster of C CTAs
 // takes one tile, each CTA a C-th of the contraction; the partial sums meet in distributed
-// shared memory and are added in rank order.  Warps 0-3 gather the token rows (64 values of
-// 128 rows a stage) and the adapter's values with 16-byte asynchronous copies, several stages
-// ahead; warp 4 issues the MMAs.  Rows past the tile's are zeros, so nothing that other tokens
-// hold can reach it.
+// shared memory and are added in rank order.  Warps 0-3 fetch 32 token rows each, 64 values a
+// stage, warp 0 also the adapter's values, all by TMA; warp 4 issues the MMAs.  (Both went
+// through cp.async first: 512 bytes cost about 20 shared-memory cycles that way, which all but
+// caps an SM at its share of HBM.)  What stands in the rows past the tile's only reaches
+// accumulator rows that nobody reads.  Rows that TMA cannot address, of odd lengths, are staged
+// by the threads.
 template <bool WMN, bool VEC, int S>
-__global__ void __launch_bounds__(LS_THREADS, 2) k_lora_shrink(const LoraShrink a) {
+__global__ void __launch_bounds__(LS_THREADS, 2)
+    k_lora_shrink(const __grid_constant__ LoraShrinkMaps maps, const LoraShrink a) {
   extern __shared__ uint8_t ls_raw[];
   uint8_t *smem = ls_raw + ((1024u - (smem_u32(ls_raw) & 1023u)) & 1023u);
   const uint32_t sx = smem_u32(smem), sw = sx + S * LS_X_BYTES;
@@ -314,7 +427,7 @@ __global__ void __launch_bounds__(LS_THREADS, 2) k_lora_shrink(const LoraShrink 
   const uint32_t cols = a.Rp <= 32 ? 32u : a.Rp <= 64 ? 64u : 128u;
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 128);
+      mbar_init(&full[s], 4);
       mbar_init(&empty[s], 1);
     }
     mbar_init(&acc_full, 1);
@@ -335,71 +448,79 @@ __global__ void __launch_bounds__(LS_THREADS, 2) k_lora_shrink(const LoraShrink 
   bool ok = true;                         // no wait of this thread has run out
   for (int i = int(cluster_id_x()); i < ntiles; i += int(ncluster_x())) {
     const int4 tv = a.plan.tiles[i];
-    const LoraTile tl{tv.x, tv.y, tv.z};
+    const LoraTile tl{tv.x, tv.y, tv.z, tv.w};
     if (tl.adapter == a.n) {              // no adapter: h = 0
       if (rank == 0 && a.out)
         for (int e = tid; e < tl.rows * a.R; e += LS_THREADS)
           a.out[int64_t(a.plan.perm[tl.p0 + e / a.R]) * a.R + e % a.R] = 0.0f;
       continue;
     }
-    if (tid < LR_TILE) rows_s[tid] = tid < tl.rows ? a.plan.perm[tl.p0 + tid] : -1;
+    if (tid < LR_TILE) rows_s[tid] = a.plan.perm[tl.p0 + min(tid, tl.rows - 1)];
     __syncthreads();
     if (warp < 4) {
       // ------------------------------------------------------------ producers
-      const int c = tid & 7, r0 = tid >> 3;          // 16-byte chunk, rows r0 + 16 j
-      int tok[8];
+      int tok[2], rows[2];                           // this warp's two groups of 16 rows
+      bool run[2];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) tok[j] = rows_s[r0 + 16 * j];
-      const __nv_bfloat16 *wi = a.w + int64_t(tl.adapter) * a.R * a.K;
-      const GridWalk w0(tid, a.Rp >> 3);             // WMN: 8-wide groups of r, contraction rows
-      const uint32_t swz = uint32_t(c ^ (r0 & 7)) << 4;
+      for (int h = 0; h < 2; ++h) {
+        const int r = warp * 32 + h * LR_GROUP;
+        tok[h] = rows_s[r + (lane & 15)];
+        rows[h] = max(0, min(LR_GROUP, tl.rows - r));
+        run[h] = rows[h] > 0 && rows_s[r + rows[h] - 1] - rows_s[r] == rows[h] - 1;
+      }
+      uint32_t tx = warp == 0 ? uint32_t(a.R) * 128 : 0u;
+      if (VEC) tx += lora_rows_bytes(run[0], rows[0]) + lora_rows_bytes(run[1], rows[1]);
       int jt = it;
       for (int kb = kb0; kb < kb1 && ok; ++kb, ++jt) {
         const int s = jt % S;
-        if (!mbar_wait(&empty[s], (uint32_t(jt / S) & 1u) ^ 1u)) {
-          ok = false;
-          break;
-        }
-        const int64_t k = int64_t(kb) * LR_KB + c * 8;
-        const uint32_t dx = sx + s * LS_X_BYTES + r0 * 128 + swz;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          stage8<VEC>(dx + j * 2048, tok[j] < 0 ? a.x : a.x + int64_t(tok[j]) * a.K + k,
-                      tok[j] < 0 ? 0 : a.K - k);
-        const uint32_t dw = sw + s * a.w_bytes;
-        if constexpr (!WMN) {
-          for (int r = r0; r < a.Rp; r += 16)
-            cp_async16(dw + r * 128 + swz, r < a.R && k < a.K ? wi + r * a.K + k : wi,
-                       r < a.R && k < a.K ? 16u : 0u);
-        } else {
-          const __nv_bfloat16 *wk = wi + int64_t(kb) * LR_KB * a.R;
-          const int rows = int(min(int64_t(LR_KB), a.K - int64_t(kb) * LR_KB));
+        if (!(ok = warp_wait(&empty[s], (uint32_t(jt / S) & 1u) ^ 1u))) break;
+        const uint32_t dx = sx + s * LS_X_BYTES + warp * 4096, dw = sw + s * (a.Rp * 128);
+        if constexpr (!VEC) {
+          const int64_t k = int64_t(kb) * LR_KB + (lane & 7) * 8;
 #pragma unroll 4
-          for (GridWalk w = w0; w.major < LR_KB; w.next()) {
-            const bool in = w.minor * 8 < a.R && w.major < rows;
-            cp_async16(dw + w.minor * LS_MN_LD + w.major * 16,
-                       in ? wk + w.major * a.R + w.minor * 8 : wi, in ? 16u : 0u);
+          for (int j = 0; j < 8; ++j) {              // 8 lanes a row
+            const int row = j * 4 + (lane >> 3);
+            stage8_any(dx + row * 128 + (((lane & 7) ^ (row & 7)) << 4),
+                       a.x + int64_t(rows_s[warp * 32 + row]) * a.K + k, a.K - k, a.x + a.T * a.K);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], tx);
+        __syncwarp();
+        if constexpr (VEC) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (rows[h] > 0)
+              lora_rows_load(dx + h * 2048, maps.x, &full[s], kb * LR_KB, tok[h], run[h], rows[h]);
+        }
+        if (warp == 0) {
+          if constexpr (!WMN) {
+            tma_load_3d_el(dw, &maps.w, &full[s], kb * LR_KB, 0, tl.adapter);
+          } else {
+            for (int r = 0; r < a.R; r += a.pw)
+              tma_load_3d_el(dw + r * 128, &maps.w, &full[s], r, kb * LR_KB, tl.adapter);
           }
         }
-        stage_arrive<VEC>(&full[s]);
       }
     } else {
       // ------------------------------------------------------------ MMA issuer
       const uint32_t id = idesc_lora(a.Rp, 0, WMN ? 1 : 0);
+      const LoraPieces pc(WMN ? a.pw : 64);
       for (int kb = kb0; kb < kb1 && ok; ++kb) {
         const int jt = it + kb - kb0, s = jt % S;
         if (!warp_wait(&full[s], uint32_t(jt / S) & 1u)) {
           ok = false;
           break;
         }
-        fence_proxy_async_smem();
         tc_fence_after();
         const uint64_t da = sdesc_sw128(sx + s * LS_X_BYTES);
-        const uint32_t bw = sw + s * a.w_bytes;
-        const uint64_t db = WMN ? sdesc(bw, 128, LS_MN_LD, 0) : sdesc_sw128(bw);
+        const uint32_t bw = sw + s * (a.Rp * 128);
+        const uint64_t db = WMN ? pc.desc_mn(bw, LR_KB) : sdesc_sw128(bw);
+        const uint32_t step = WMN ? pc.step_mn() >> 4 : 2;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          tc_mma_bf16_el(tmem, da + uint64_t(2 * k), db + uint64_t((WMN ? 16 : 2) * k), id,
+          tc_mma_bf16_el(tmem, da + uint64_t(2 * k), db + uint64_t(step * k), id,
                          (kb > kb0 || k) ? 1u : 0u);
         tc_commit_el(&empty[s]);
       }
@@ -407,59 +528,60 @@ __global__ void __launch_bounds__(LS_THREADS, 2) k_lora_shrink(const LoraShrink 
       __syncwarp();
     }
     it += kb1 - kb0;
-    // ------------------------------------------------------------ the C partial sums
+    // ------------------------------------------------------------ the C partial sums: every
+    // thread sends its row to the CTA that adds that row, red[rank][row of the owner][Rp]
     float *red = reinterpret_cast<float *>(smem);
-    const int ld = a.Rp + 4;
+    const int ld = a.Rp + 4, own = LR_TILE / C;      // rows a CTA adds
     if (warp < 4) {
       if (ok) ok = warp_wait(&acc_full, uint32_t(done) & 1u);
       tc_fence_after();
+    }
+    ++done;
+    cluster_sync();                       // nobody's stages are in use any more
+    if (warp < 4) {
+      const uint32_t to = mapa_rank(red + (rank * own + tid % own) * ld, tid / own);
       for (int c0 = 0; c0 < a.Rp; c0 += 32) {
         uint32_t v[32];
         tmem_ld32(tmem + (uint32_t(32 * warp) << 16) + c0, v);
-        float *dst = red + tid * ld + c0;
 #pragma unroll
         for (int e = 0; e < 32; e += 4)
           if (c0 + e < a.Rp)
-            *reinterpret_cast<uint4 *>(dst + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (c0 + e) * 4),
+                         "r"(v[e]), "r"(v[e + 1]), "r"(v[e + 2]), "r"(v[e + 3])
+                         : "memory");
       }
       tc_fence_before();
     }
-    ++done;
     cluster_sync();
     tc_fence_after();
     const float sc = a.scaling ? a.scaling[tl.adapter] : 1.0f;
-    const int q4 = a.Rp >> 2, row_a = LR_TILE * rank / C, row_b = LR_TILE * (rank + 1) / C;
+    const int q4 = a.Rp >> 2;
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int e = tid; e < (row_b - row_a) * q4; e += LS_THREADS) {
-      const int row = row_a + e / q4, c4 = (e % q4) * 4;
-      if (row >= tl.rows) break;
-      const bool in = c4 < a.R;                    // the padding of Rp: zeros
-      const int64_t tok = rows_s[row], at = int64_t(tl.p0 + row) * a.Rp + c4;
-      float4 v[8], s = zero;                       // all requests in flight, added in rank order
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        v[q] = zero;
-        if (in && q < C)
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(v[q].x), "=f"(v[q].y), "=f"(v[q].z), "=f"(v[q].w)
-                       : "r"(mapa_rank(red + row * ld + c4, q))
-                       : "memory");
-      }
+    for (int e = tid; e < own * q4; e += LS_THREADS) {
+      const int lrow = e / q4, row = rank * own + lrow, c4 = (e % q4) * 4;
+      if (row >= ((tl.rows + 63) & ~63)) break;
+      const bool in = c4 < a.R && row < tl.rows;   // the padding of Rp and of the block: zeros
+      const int64_t tok = rows_s[row];
       const float4 h = in && a.h ? __ldg(reinterpret_cast<const float4 *>(a.h + tok * a.R + c4)) : zero;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        s.x += v[q].x;
-        s.y += v[q].y;
-        s.z += v[q].z;
-        s.w += v[q].w;
-      }
+      float4 s = zero;
+      if (in)
+        for (int q = 0; q < C; ++q) {
+          const float4 v = *reinterpret_cast<const float4 *>(red + (q * own + lrow) * ld + c4);
+          s.x += v.x;
+          s.y += v.y;
+          s.z += v.z;
+          s.w += v.w;
+        }
       if (a.out && in) *reinterpret_cast<float4 *>(a.out + tok * a.R + c4) = s;
-      store_parts(a.parts + at, a.plane, s, sc);
-      if (a.h) store_parts(a.h_parts + at, a.plane, h, sc);
+      // (zeros are not scaled: an infinite scaling would make them NaN)
+      store_parts(a.parts, a.np, a.Rp, tl.block, row, c4, s, in ? sc : 1.0f);
+      if (a.h) store_parts(a.h_parts, a.np, a.Rp, tl.block, row, c4, h, in ? sc : 1.0f);
     }
-    cluster_sync();                       // before the stages are written again
+    __syncthreads();                      // before the stages are written again
+    // the copies' writes come after these reads and the peers' stores
+    fence_proxy_async_smem();
   }
-  cp_async_wait_all();
+  cluster_sync();                         // no peer's stores are on their way
   tc_fence_before();
   __syncthreads();
   if (warp == 4) {
@@ -586,54 +708,77 @@ __global__ void __launch_bounds__(LD_THREADS) k_lora_decode(const LoraDecode p) 
 
 // ------------------------------------------------------------------ expand
 struct LoraExpand {
-  const __nv_bfloat16 *parts;  // [LR_PARTS][T][Rp] h times scaling, sorted order
-  int64_t plane;
+  const __nv_bfloat16 *parts;  // the parts of h times scaling (np of them)
   const __nv_bfloat16 *w;      // [n][N][R], or [n][R][N] (WMN)
   int64_t N;
-  int R, Rp, n;
+  int R, Rp, n, np;
   const void *base;            // [T, N] or NULL
   void *y;                     // [T, N]
   LoraPlan plan;
-  int ncb, cpu;                // 128-column blocks, and how many of them a work item takes
-  int vec;                     // rows of base and y are 16-byte aligned
-  uint32_t a_bytes, w_bytes;   // staged bytes of the parts and of a column block of W
+  int ncb, cpu;                // column blocks, and how many of them a work item takes
+  int vec;                     // rows of base and y are 16-byte aligned: TMA moves them
+  int ring;                    // tiles of 128 rows x 128 bytes in shared memory (even)
+  int pw;                      // !WMN: see LoraPieces
+};
+struct LoraExpandMaps {
+  LoraRows base, y;
+  CUtensorMap w;               // [n][N][R], box pw x CB columns; WMN: [n][R][N], box CB columns x R
 };
 
-constexpr int LE_COLS = 128;
-constexpr int LE_THREADS = 13 * 32;
-constexpr int LE_LD = 128 * 16 + 16;              // bytes between 8-wide k groups of 128 rows
-constexpr int LE_EPI_LD = 36;                     // floats of a transposition row
-constexpr int LE_EPI_BYTES = 8 * 32 * LE_EPI_LD * 4;
+constexpr int LE_THREADS = 14 * 32;
+constexpr int LE_BUF = 4;                         // column blocks of W and accumulators in flight
+constexpr int LE_TILE_BYTES = LR_TILE * 128;      // 16 KB
+constexpr int LE_RING_MAX = 8;
+constexpr int LE_EPI_LD = 36;                     // floats of a transposition row (odd rows only)
 
-// D[128 tokens x 128 columns] in TMEM (tcgen05.mma kind::f16, double-buffered): the tile's
-// parts are the A operand, contraction NS * Rp, staged once for a work item's column blocks; a
-// block of W is the B operand, double-buffered, in its own order in memory (rows of r for B,
-// columns contiguous for A: the MMA takes either).  Warps 0-3 stage, 4 issues the MMAs, 5-12
-// read TMEM, turn 32 x 32 pieces through shared memory and move base and y in 64- or 128-byte
-// pieces of a row.  mma.sync with its accumulators stored straight from registers took 185 us
-// at T 8192, N 14336, R 32 (two CTAs an SM at 122 registers, too few loads in flight).
+// D[128 tokens x CB columns] in TMEM (tcgen05.mma kind::f16; CB columns are 128 bytes of a row of
+// y): the tile's parts are the A operand, contraction NS * Rp, staged once for a work item's
+// column blocks; a block of W is the B operand, in its own order in memory (rows of r for B,
+// columns contiguous for A: the MMA takes either).  base comes in through a ring of 16 KB tiles,
+// the epilogue adds the accumulators to it in place, a thread a row, and the tile goes out the
+// same way (128-byte swizzle: no bank conflicts); rows that follow one another move 16 an
+// instruction, others four.  Warps 0-3 fetch base, 4 issues the MMAs, 5 fetches W and the parts,
+// 6-9 and 10-13 are two epilogues that take turns.  Row-wise plain loads and stores, through a
+// transposition in shared memory, kept the load/store pipe busy for twice the time that HBM
+// needs (135 us at T 8192, N 14336, R 32).  Rows that TMA cannot address (odd lengths) are still
+// moved that way.
 template <bool WMN, typename OT>
-__global__ void __launch_bounds__(LE_THREADS, 2) k_lora_expand(const LoraExpand a) {
+__global__ void __launch_bounds__(LE_THREADS, 1)
+    k_lora_expand(const __grid_constant__ LoraExpandMaps maps, const LoraExpand a) {
   constexpr int NS = sizeof(OT) == 4 ? 3 : 2;
-  extern __shared__ __align__(128) uint8_t le_smem[];
-  const uint32_t sa = smem_u32(le_smem), sw = sa + a.a_bytes;
-  float *epi = reinterpret_cast<float *>(le_smem + a.a_bytes + 2 * a.w_bytes);
-  __shared__ uint64_t a_empty, w_full[2], w_empty[2], acc_full[2], acc_empty[2];
+  constexpr int CB = 128 / int(sizeof(OT));       // columns of a block
+  extern __shared__ uint8_t le_raw[];
+  uint8_t *smem = le_raw + ((1024u - (smem_u32(le_raw) & 1023u)) & 1023u);
+  const uint32_t w_bytes = uint32_t(CB) * a.Rp * 2;
+  const uint32_t s_ring = smem_u32(smem), sw = s_ring + a.ring * LE_TILE_BYTES,
+                 sa = sw + LE_BUF * w_bytes;
+  __shared__ uint64_t a_full, a_empty, w_full[LE_BUF], w_empty[LE_BUF], acc_full[LE_BUF],
+      acc_empty[LE_BUF], b_full[LE_RING_MAX], b_empty[LE_RING_MAX];
   __shared__ uint32_t tmem_slot;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
+    mbar_init(&a_full, 1);
     mbar_init(&a_empty, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&w_full[i], 128);
+    for (int i = 0; i < LE_BUF; ++i) {
+      mbar_init(&w_full[i], 1);
       mbar_init(&w_empty[i], 1);
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 8);
+      mbar_init(&acc_empty[i], 4);
+    }
+    for (int i = 0; i < a.ring; ++i) {
+      mbar_init(&b_full[i], 4);
+      mbar_init(&b_empty[i], 4);
     }
     fence_barrier_init();
   }
   if (warp == 4) {
-    tmem_alloc(&tmem_slot, 2 * LE_COLS);
+    tmem_alloc(&tmem_slot, LE_BUF * CB);
     tmem_relinquish();
+  }
+  if (a.Rp > a.R) {               // the contraction's padding: zero for good, no copy writes it
+    for (int e = tid; e < LE_BUF * CB; e += LE_THREADS)
+      st_shared16(sw + e / CB * w_bytes + uint32_t(a.R) * CB * 2 + e % CB * 16, make_uint4(0, 0, 0, 0));
+    fence_proxy_async_smem();
   }
   tc_fence_before();
   __syncthreads();
@@ -642,227 +787,285 @@ __global__ void __launch_bounds__(LE_THREADS, 2) k_lora_expand(const LoraExpand 
   const int per_tile = (a.ncb + a.cpu - 1) / a.cpu, rg = a.Rp >> 3;
   const int64_t items = int64_t(a.plan.head[0]) * per_tile;
   bool ok = true;
-  int blk = 0, live = 0;                          // column blocks and live items so far
+  int blk = 0, live = 0;          // column blocks (warps 4 and 5: of live tiles), live items so far
   if (warp < 4) {
-    // -------------------------------------------------------------- staging
-    const GridWalk w0(tid, rg);
-    for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const int4 tl = a.plan.tiles[item / per_tile];
-      if (tl.x >= a.n) continue;
-      const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
-      const __nv_bfloat16 *wi = a.w + int64_t(tl.x) * a.R * a.N;
-      if (!(ok = mbar_wait(&a_empty, (uint32_t(live) & 1u) ^ 1u))) break;
-      ++live;
-      const __nv_bfloat16 *pt = a.parts + int64_t(tl.y) * a.Rp;
-#pragma unroll 2
-      for (GridWalk w = w0; w.major < LR_TILE; w.next()) {
-        const bool in = w.major < tl.z;
-        const __nv_bfloat16 *src = in ? pt + w.major * a.Rp + w.minor * 8 : a.parts;
+    // -------------------------------------------------------------- base, 32 rows a warp
+    if (a.vec && a.base) {
+      for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        const int4 tl = a.plan.tiles[item / per_tile];
+        const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
+        int tok[2], rows[2];
+        bool run[2];
+        uint32_t tx = 0;
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
-          cp_async16(sa + uint32_t(i * rg + w.minor) * LE_LD + w.major * 16,
-                     src + (in ? i * a.plane : 0), in ? 16u : 0u);
-      }
-      for (int cb = cb0; cb < cb1 && ok; ++cb, ++blk) {
-        const int b = blk & 1;
-        if (!(ok = mbar_wait(&w_empty[b], (uint32_t(blk >> 1) & 1u) ^ 1u))) break;
-        const int64_t c0 = int64_t(cb) * LE_COLS;
-        const uint32_t dw = sw + b * a.w_bytes;
-        if constexpr (!WMN) {
-          const __nv_bfloat16 *wc = wi + c0 * a.R;
-          const int n_cols = int(min(int64_t(LE_COLS), a.N - c0));
-#pragma unroll 4
-          for (GridWalk w = w0; w.major < LE_COLS; w.next()) {
-            const bool in = w.major < n_cols && w.minor * 8 < a.R;
-            cp_async16(dw + uint32_t(w.minor) * LE_LD + w.major * 16,
-                       in ? wc + w.major * a.R + w.minor * 8 : wi, in ? 16u : 0u);
-          }
-        } else {
-          const int g = tid & 15;                  // 8 columns; rows r = tid / 16 + 8 i
-          const bool cin = c0 + g * 8 < a.N;
-          const __nv_bfloat16 *wc = wi + c0 + g * 8;
-          const uint32_t dg = dw + uint32_t(g) * (a.Rp * 16 + 16);
-#pragma unroll 4
-          for (int r = tid >> 4; r < a.Rp; r += 8) {
-            const bool in = cin && r < a.R;
-            cp_async16(dg + r * 16, in ? wc + int64_t(r) * a.N : wi, in ? 16u : 0u);
-          }
+        for (int h = 0; h < 2; ++h) {
+          const int r = warp * 32 + h * LR_GROUP;
+          tok[h] = a.plan.perm[tl.y + min(r + (lane & 15), tl.z - 1)];
+          rows[h] = max(0, min(LR_GROUP, tl.z - r));
+          const int last = __shfl_sync(0xffffffffu, tok[h], max(0, rows[h] - 1));
+          run[h] = rows[h] > 0 && last - __shfl_sync(0xffffffffu, tok[h], 0) == rows[h] - 1;
+          tx += lora_rows_bytes(run[h], rows[h]);
         }
-        stage_arrive<true>(&w_full[b]);
+        for (int cb = cb0; cb < cb1; ++cb, ++blk) {
+          const int s = blk % a.ring;
+          if (!(ok = warp_wait(&b_empty[s], (uint32_t(blk / a.ring) & 1u) ^ 1u))) break;
+          if (lane == 0) mbar_arrive_expect_tx(&b_full[s], tx);
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (rows[h] > 0)
+              lora_rows_load(s_ring + s * LE_TILE_BYTES + warp * 4096 + h * 2048, maps.base,
+                             &b_full[s], cb * CB, tok[h], run[h], rows[h]);
+        }
       }
+      for (int e = max(0, blk - a.ring); e < blk; ++e)
+        warp_wait(&b_full[e % a.ring], uint32_t(e / a.ring) & 1u);
     }
-    cp_async_wait_all();
   } else if (warp == 4) {
     // -------------------------------------------------------------- MMA issuer
-    const uint32_t id = idesc_lora(LE_COLS, 0, WMN ? 1 : 0);
+    const uint32_t id = idesc_lora(CB, 0, WMN ? 1 : 0);
+    const LoraPieces pc(WMN ? CB : a.pw);
     for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
       if (a.plan.tiles[item / per_tile].x >= a.n) continue;
       const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
+      if (!(ok = warp_wait(&a_full, uint32_t(live) & 1u))) break;
+      ++live;
       for (int cb = cb0; cb < cb1; ++cb, ++blk) {
-        const int b = blk & 1;
-        const uint32_t ph = uint32_t(blk >> 1) & 1u;
+        const int b = blk % LE_BUF;
+        const uint32_t ph = uint32_t(blk / LE_BUF) & 1u;
         if (!warp_wait(&acc_empty[b], ph ^ 1u) || !warp_wait(&w_full[b], ph)) {
           ok = false;
           break;
         }
-        fence_proxy_async_smem();
         tc_fence_after();
-        const uint64_t da = sdesc(sa, LE_LD, 128, 0);
-        const uint32_t bw = sw + b * a.w_bytes;
-        const uint64_t db = WMN ? sdesc(bw, 128, a.Rp * 16 + 16, 0) : sdesc(bw, LE_LD, 128, 0);
-        const uint32_t bstep = WMN ? 256 : 2 * LE_LD;            // 16 contraction indices
+        const uint64_t da = sdesc(sa, 2048, 128, 0);
+        const uint32_t bw = sw + b * w_bytes;
+        const uint64_t db = WMN ? pc.desc_mn(bw, a.Rp) : pc.desc_k(bw, CB);
         for (int i = NS - 1; i >= 0; --i)                        // the smallest parts first
-          for (int k = 0; k < a.Rp / 16; ++k)
-            tc_mma_bf16_el(tmem + b * LE_COLS,
-                           da + uint64_t(uint32_t(i * rg + 2 * k) * (LE_LD >> 4)),
-                           db + uint64_t(k * (bstep >> 4)), id, (i < NS - 1 || k) ? 1u : 0u);
+          for (int k = 0; k < a.Rp / 16; ++k) {
+            const uint32_t off = WMN ? k * pc.step_mn() : pc.off_k(k, CB);
+            tc_mma_bf16_el(tmem + b * CB, da + uint64_t(uint32_t(i * rg + 2 * k) * 128),
+                           db + uint64_t(off >> 4), id, (i < NS - 1 || k) ? 1u : 0u);
+          }
         tc_commit_el(&w_empty[b]);
         tc_commit_el(&acc_full[b]);
       }
       if (ok) tc_commit_el(&a_empty);
     }
     __syncwarp();
+  } else if (warp == 5) {
+    // -------------------------------------------------------------- W and the parts
+    for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      const int4 tl = a.plan.tiles[item / per_tile];
+      if (tl.x >= a.n) continue;
+      const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
+      // the tile's one or two blocks of parts, a [64][8] group a copy
+      if (!(ok = warp_wait(&a_empty, (uint32_t(live) & 1u) ^ 1u))) break;
+      ++live;
+      const int nb = tl.z > 64 ? 2 : 1;
+      if (lane == 0) mbar_arrive_expect_tx(&a_full, uint32_t(nb * NS * rg) * 1024);
+      __syncwarp();
+      for (int b = 0; b < nb; ++b) {
+        const __nv_bfloat16 *src = a.parts + int64_t(tl.w + b) * a.np * a.Rp * 64;
+        for (int g = 0; g < NS * rg; ++g)
+          bulk_load_el(sa + g * 2048 + b * 1024, src + g * 512, 1024, &a_full);
+      }
+      for (int cb = cb0; cb < cb1; ++cb, ++blk) {
+        const int b = blk % LE_BUF;
+        if (!(ok = warp_wait(&w_empty[b], (uint32_t(blk / LE_BUF) & 1u) ^ 1u))) break;
+        const uint32_t dw = sw + b * w_bytes;
+        if (lane == 0) mbar_arrive_expect_tx(&w_full[b], uint32_t(CB) * a.R * 2);
+        __syncwarp();
+        if constexpr (WMN) {
+          tma_load_3d_el(dw, &maps.w, &w_full[b], cb * CB, 0, tl.x);
+        } else {
+          for (int r = 0; r < a.R; r += a.pw)
+            tma_load_3d_el(dw + uint32_t(r) * CB * 2, &maps.w, &w_full[b], r, cb * CB, tl.x);
+        }
+      }
+    }
+    // the last copies have landed before the CTA can end (bounded)
+    if (live > 0) warp_wait(&a_full, uint32_t(live - 1) & 1u);
+    for (int e = max(0, blk - LE_BUF); e < blk; ++e)
+      warp_wait(&w_full[e % LE_BUF], uint32_t(e / LE_BUF) & 1u);
   } else {
     // -------------------------------------------------------------- epilogue
     const OT *base = static_cast<const OT *>(a.base);
     OT *y = static_cast<OT *>(a.y);
-    const int w8 = warp - 5, q4 = warp & 3, half = w8 >> 2;     // TMEM lanes 32 q4 .., 64 columns
-    float *tp = epi + w8 * 32 * LE_EPI_LD;
+    const int grp = (warp - 6) >> 2, q4 = warp & 3;      // TMEM lanes 32 q4 .. + 31
+    const int row = 32 * q4 + lane;                      // this thread's row of the tile
+    float *tp = reinterpret_cast<float *>(smem) + (warp - 6) * 32 * LE_EPI_LD;
+    int all = 0, prev = -1;                              // blocks so far; the tile last stored
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
       const int4 tl = a.plan.tiles[item / per_tile];
       const bool has = tl.x < a.n;
       const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
-      // vec: rows 32 q4 + 8 j + lane / 4; else the tokens of all 32 rows, a lane each
-      int tok[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = 32 * q4 + 8 * j + (lane >> 2);
-        tok[j] = row < tl.z ? a.plan.perm[tl.y + row] : -1;
-      }
-      const int row_l = 32 * q4 + lane;
-      const int tok_l = row_l < tl.z ? a.plan.perm[tl.y + row_l] : -1;
-      for (int cb = cb0; cb < cb1; ++cb) {
-        const int b = blk & 1;
-#pragma unroll 1
-        for (int ch = 0; ch < 2; ++ch) {
-          const int64_t c0 = int64_t(cb) * LE_COLS + half * 64 + ch * 32;
-          const int64_t c = c0 + (lane & 3) * 8;
-          uint4 in[4][sizeof(OT) / 2];
-          if (a.vec && base && c < a.N) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (tok[j] >= 0) {
-                const uint4 *src = reinterpret_cast<const uint4 *>(base + int64_t(tok[j]) * a.N + c);
-#pragma unroll
-                for (int u = 0; u < int(sizeof(OT) / 2); ++u) in[j][u] = src[u];
-              }
-          }
-          if (has && ch == 0) {
-            // a warp whose wait ran out goes on without waiting
-            if (ok) ok = warp_wait(&acc_full[b], uint32_t(blk >> 1) & 1u);
-            tc_fence_after();
-          }
-          if (has) {
-            uint32_t v[32];
-            tmem_ld32(tmem + (uint32_t(32 * q4) << 16) + b * LE_COLS + half * 64 + ch * 32, v);
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4 *>(tp + lane * LE_EPI_LD + e) =
-                  make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+      const int tok = row < tl.z ? a.plan.perm[tl.y + row] : -1;
+      for (int cb = cb0; cb < cb1; ++cb, ++all, blk += has ? 1 : 0) {
+        if ((all & 1) != grp) continue;
+        const int b = blk % LE_BUF, s = all % a.ring;
+        const uint32_t tacc = tmem + (uint32_t(32 * q4) << 16) + b * CB;
+        if (a.vec) {
+          // the tile of this warp's last turn has been read: the fetch may refill it
+          if (prev >= 0) {
+            bulk_wait_read_el();
+            if (base && lane == 0) mbar_arrive(&b_empty[prev]);
             __syncwarp();
           }
-          if (a.vec) {
+          // a warp whose wait ran out goes on without waiting
+          if (base && ok) ok = warp_wait(&b_full[s], uint32_t(all / a.ring) & 1u);
+        }
+        if (has) {
+          if (ok) ok = warp_wait(&acc_full[b], uint32_t(blk / LE_BUF) & 1u);
+          tc_fence_after();
+        }
+        if (a.vec) {
+          uint8_t *trow = smem + s * LE_TILE_BYTES + row * 128;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-              if (has) {
-                const float4 *src = reinterpret_cast<const float4 *>(
-                    tp + (8 * j + (lane >> 2)) * LE_EPI_LD + (lane & 3) * 8);
-                const float4 v0 = src[0], v1 = src[1];
-                f[0] = v0.x; f[1] = v0.y; f[2] = v0.z; f[3] = v0.w;
-                f[4] = v1.x; f[5] = v1.y; f[6] = v1.z; f[7] = v1.w;
+          for (int h = 0; h < CB; h += 32) {
+            uint32_t v[32];
+            if (has) {
+              tmem_ld32(tacc + h, v);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = 0u;
+            }
+            if constexpr (sizeof(OT) == 4) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                float4 *at = reinterpret_cast<float4 *>(trow + ((k ^ (row & 7)) << 4));
+                float4 o = base ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+                o.x += __uint_as_float(v[4 * k]);
+                o.y += __uint_as_float(v[4 * k + 1]);
+                o.z += __uint_as_float(v[4 * k + 2]);
+                o.w += __uint_as_float(v[4 * k + 3]);
+                *at = o;
               }
-              if (tok[j] < 0 || c >= a.N) continue;
-              uint4 *dst = reinterpret_cast<uint4 *>(y + int64_t(tok[j]) * a.N + c);
-              if constexpr (sizeof(OT) == 4) {
-                if (base) {
-                  const uint32_t *s = reinterpret_cast<const uint32_t *>(in[j]);
+            } else {
 #pragma unroll
-                  for (int e = 0; e < 8; ++e) f[e] += __uint_as_float(s[e]);
-                }
-                dst[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]),
-                                    __float_as_uint(f[2]), __float_as_uint(f[3]));
-                dst[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]),
-                                    __float_as_uint(f[6]), __float_as_uint(f[7]));
-              } else {
-                const uint32_t s[4] = {in[j][0].x, in[j][0].y, in[j][0].z, in[j][0].w};
+              for (int k = 0; k < 4; ++k) {
+                uint4 *at = reinterpret_cast<uint4 *>(trow + (((h / 8 + k) ^ (row & 7)) << 4));
+                const uint4 in = base ? *at : make_uint4(0, 0, 0, 0);
+                const uint32_t w[4] = {in.x, in.y, in.z, in.w};
                 uint32_t o[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                  if (base) {
-                    f[2 * e] += bf_bits2f(uint16_t(s[e]));
-                    f[2 * e + 1] += bf_bits2f(uint16_t(s[e] >> 16));
-                  }
-                  o[e] = uint32_t(f2bf_bits(f[2 * e])) | (uint32_t(f2bf_bits(f[2 * e + 1])) << 16);
+                  const float lo = __uint_as_float(w[e] << 16) + __uint_as_float(v[8 * k + 2 * e]);
+                  const float hi = __uint_as_float(w[e] & 0xFFFF0000u) +
+                                   __uint_as_float(v[8 * k + 2 * e + 1]);
+                  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+                  o[e] = *reinterpret_cast<const uint32_t *>(&p);
                 }
-                dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+                *at = make_uint4(o[0], o[1], o[2], o[3]);
               }
             }
-          } else {
-            // rows that start anywhere: a row a step, a lane per column
+          }
+          if (has) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[b]);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {                    // this warp's two groups of 16 rows
+            const int r0 = 32 * q4 + h * LR_GROUP, rows = min(LR_GROUP, tl.z - r0);
+            const uint32_t tile = s_ring + s * LE_TILE_BYTES + r0 * 128;
+            const int t0 = __shfl_sync(0xffffffffu, tok, h * LR_GROUP);
+            if (rows == LR_GROUP &&
+                __shfl_sync(0xffffffffu, tok, h * LR_GROUP + LR_GROUP - 1) - t0 == LR_GROUP - 1) {
+              tma_store_rows_el(&maps.y.run, tile, cb * CB, t0);
+              continue;
+            }
+            for (int j = 0; 4 * j < rows; ++j) {
+              const int4 r = make_int4(__shfl_sync(0xffffffffu, tok, h * LR_GROUP + 4 * j),
+                                       __shfl_sync(0xffffffffu, tok, h * LR_GROUP + 4 * j + 1),
+                                       __shfl_sync(0xffffffffu, tok, h * LR_GROUP + 4 * j + 2),
+                                       __shfl_sync(0xffffffffu, tok, h * LR_GROUP + 4 * j + 3));
+              if (4 * j + 4 <= rows) {
+                tma_scatter4_el(&maps.y.gather, tile + j * 512, cb * CB, r);
+              } else {
+                // the tile's last one to three rows: 8 lanes a row
+                const int rr = 4 * j + (lane >> 3), k = lane & 7;
+                const int64_t c = int64_t(cb) * CB + k * (16 / int(sizeof(OT)));
+                const int t4 = lane >> 3 == 0 ? r.x : lane >> 3 == 1 ? r.y : r.z;
+                if (rr < rows && c < a.N)
+                  *reinterpret_cast<uint4 *>(y + int64_t(t4) * a.N + c) =
+                      *reinterpret_cast<const uint4 *>(smem + s * LE_TILE_BYTES + (r0 + rr) * 128 +
+                                                       ((k ^ (rr & 7)) << 4));
+              }
+            }
+          }
+          bulk_commit_el();
+          prev = s;
+        } else {
+          // rows that start anywhere: 32 x 32 pieces turned in shared memory, a lane a column
+#pragma unroll
+          for (int h = 0; h < CB; h += 32) {
+            if (has) {
+              uint32_t v[32];
+              tmem_ld32(tacc + h, v);
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<uint4 *>(tp + lane * LE_EPI_LD + e) =
+                    make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            }
+            __syncwarp();
+            const int64_t c = int64_t(cb) * CB + h + lane;
 #pragma unroll 8
             for (int r = 0; r < 32; ++r) {
-              const int tk = __shfl_sync(0xffffffffu, tok_l, r);
-              if (tk < 0 || c0 + lane >= a.N) continue;
-              const int64_t at = int64_t(tk) * a.N + c0 + lane;
+              const int tk = __shfl_sync(0xffffffffu, tok, r);
+              if (tk < 0 || c >= a.N) continue;
+              const int64_t at = int64_t(tk) * a.N + c;
               float f = has ? tp[r * LE_EPI_LD + lane] : 0.0f;
               if (base) f += float(base[at]);
               y[at] = OT(f);
             }
+            __syncwarp();
           }
-          __syncwarp();
-        }
-        if (has) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[b]);
-          ++blk;
+          if (has) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[b]);
+          }
         }
       }
     }
+    bulk_wait_el();
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 4) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * LE_COLS);
+    tmem_dealloc(tmem, LE_BUF * CB);
   }
 }
 
 // ------------------------------------------------------------------ wgrad
 struct LoraGradSide {
   const __nv_bfloat16 *v;      // [T, C] long side: x (dA) or dy (dB)
-  const __nv_bfloat16 *u;      // [LR_PARTS][T][Rp] rank side, sorted: g (dA) or h (dB), scaled
+  const __nv_bfloat16 *u;      // rank side, the parts of g (dA) or h (dB)
   int64_t C;
   int ncb;                     // 128-column blocks
   void *out;                   // [n, R, C] (r_major) or [n, C, R]
   int r_major;
-  int vec;                     // v's rows are 16-byte aligned
+  int vec;                     // v's rows are 16-byte aligned: TMA reads them
 };
 struct LoraWgrad {
   LoraGradSide side[2];
-  int R, Rp, n;
-  int64_t plane;               // T * Rp
+  int R, Rp, n, np;
+  int64_t T;
   LoraPlan plan;
   float *part;                 // [2 * grid][Rp][128] partial sums
-  uint32_t u_bytes;            // one bf16 part of a stage of u: (Rp / 8) * LG_MN_LD
+};
+struct LoraWgradMaps {
+  LoraRows v[2];               // the long sides
 };
 
-constexpr int LG_THREADS = 416;
+constexpr int LG_THREADS = 288;
 constexpr int LG_COLS = 128;
 constexpr int LG_X_BYTES = LR_KB * LG_COLS * 2;     // 16 KB: 2 pieces of [64 tokens x 128 B]
 constexpr int LG_MIN_STAGES = 8;                    // a CTA's least share, see k_lora_wgrad
-constexpr int LG_MN_LD = LR_KB * 16 + 16;
 __host__ __device__ __forceinline__ constexpr uint32_t lg_tmem_cols(int Rp) {
   return Rp <= 32 ? 64u : Rp <= 64 ? 128u : 256u;   // two accumulators
 }
@@ -905,15 +1108,17 @@ __device__ __forceinline__ LoraSeg lora_seg(const LoraWgrad &a, int64_t s, int64
 // cut into equal pieces: an item that one CTA covers is written at once, one that a cut divides
 // is written as fp32 partial sums (at most two per CTA) and the last CTA to arrive adds them in
 // order.  A piece is at least min(8, the average item's) stages: cutting a few microseconds of
-// loads costs more in the join than it saves.  Warps 0-3 copy v, 4-7 u, 8 issues the MMAs, 9-12
-// read TMEM; accumulators are double-buffered, so an item's stores overlap the next one.
+// loads costs more in the join than it saves.  Warps 0-3 fetch v's rows (missing ones repeat one of
+// the adapter's own, against zero rows of u), warp 0 also copies u's block; 4 issues the MMAs, 5-8 read TMEM; accumulators are double-buffered, so an item's stores
+// overlap the next one.
 template <typename OT, int S>
-__global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_wgrad(const LoraWgrad a) {
+__global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_wgrad(
+    const __grid_constant__ LoraWgradMaps maps, const LoraWgrad a) {
   constexpr int NS = sizeof(OT) == 4 ? 3 : 2;
   extern __shared__ uint8_t lg_raw[];
   uint8_t *smem = lg_raw + ((1024u - (smem_u32(lg_raw) & 1023u)) & 1023u);
   const uint32_t sx = smem_u32(smem), su = sx + S * LG_X_BYTES;
-  const uint32_t u_stage = NS * a.u_bytes;
+  const uint32_t u_bytes = uint32_t(a.Rp) * 128, u_stage = NS * u_bytes;   // a part, all parts
   __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2], mma_done;
   __shared__ uint32_t tmem_slot;
   __shared__ int last_s;
@@ -921,7 +1126,7 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
   const uint32_t cols = lg_tmem_cols(a.Rp), acc_cols = cols / 2;
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 256);
+      mbar_init(&full[s], 4);
       mbar_init(&empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -931,7 +1136,7 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
     mbar_init(&mma_done, 1);
     fence_barrier_init();
   }
-  if (warp == 8) {
+  if (warp == 4) {
     tmem_alloc(&tmem_slot, cols);
     tmem_relinquish();
   }
@@ -945,65 +1150,59 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
                           min(int64_t(LG_MIN_STAGES), (stages + used - 1) / used));
   const int64_t w0 = min(int64_t(blockIdx.x) * per, all), w1 = min(w0 + per, all);
 
-  if (warp < 8) {
+  if (warp < 4) {
     // -------------------------------------------------------------- producers
     int it = 0;
     bool ok = true;
     for (int64_t s = w0; s < w1 && ok;) {
       const LoraSeg sg = lora_seg(a, s, w1);
       const LoraGradSide &sd = a.side[sg.side];
+      const LoraRows &map = maps.v[sg.side];
       const int p0 = a.plan.off[sg.adapter] + sg.first * LR_KB, pn = a.plan.off[sg.adapter + 1];
-      if (warp < 4) {
-        // 64 rows x 16 chunks of 16 bytes: a warp's half takes a row, 8 steps for its 16 rows
-        // (fields of sd in registers: the copies' memory clobbers would have them read again)
-        const int64_t c = int64_t(sg.cb) * LG_COLS + (lane & 15) * 8, C = sd.C;
-        const bool cin = c < C, vec = sd.vec != 0;
-        const __nv_bfloat16 *v0 = sd.v, *vc = v0 + c;
-        const uint32_t d0 = sx + ((lane & 15) >> 3) * 8192 + (warp * 16 + (lane >> 4)) * 128;
-        const int r16 = warp * 16 + (lane & 15);
-        int tok_n = p0 + r16 < pn ? a.plan.perm[p0 + r16] : -1;    // one stage ahead
-        for (int q = 0; q < sg.count; ++q, ++it) {
-          const int st = it % S;
-          const int tok_l = tok_n, nx = p0 + (q + 1) * LR_KB + r16;
-          tok_n = q + 1 < sg.count && nx < pn ? a.plan.perm[nx] : -1;
-          if (!(ok = mbar_wait(&empty[st], (uint32_t(it / S) & 1u) ^ 1u))) break;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int row8 = (2 * j + (lane >> 4)) & 7;
-            const int tok = __shfl_sync(0xffffffffu, tok_l, 2 * j + (lane >> 4));
-            const uint32_t d = d0 + st * LG_X_BYTES + j * 256 + (((lane & 7) ^ row8) << 4);
-            const bool in = tok >= 0 && cin;
-            const __nv_bfloat16 *src = in ? vc + int64_t(tok) * C : v0;
-            if (vec) stage8<true>(d, src, in ? 8 : 0);
-            else stage8<false>(d, src, in ? C - c : 0);
+      // (fields of sd in registers: the copies' memory clobbers would have them read again)
+      const bool vec = sd.vec != 0;
+      const __nv_bfloat16 *v = sd.v, *v_end = v + a.T * sd.C;
+      const int64_t C = sd.C;
+      const __nv_bfloat16 *u = sd.u + int64_t(a.plan.stages[sg.adapter] + sg.first) * a.np * a.Rp * 64;
+      const int c0 = sg.cb * LG_COLS;
+      int tok_n = a.plan.perm[min(p0 + warp * 16 + (lane & 15), pn - 1)];    // one stage ahead
+      for (int q = 0; q < sg.count; ++q, ++it) {
+        const int st = it % S;
+        const int tok = tok_n;
+        if (q + 1 < sg.count)
+          tok_n = a.plan.perm[min(p0 + (q + 1) * LR_KB + warp * 16 + (lane & 15), pn - 1)];
+        if (!(ok = warp_wait(&empty[st], (uint32_t(it / S) & 1u) ^ 1u))) break;
+        const uint32_t dv = sx + st * LG_X_BYTES + warp * 2048;
+        if (vec) {
+          // (only rows of the stage itself: what u's zero rows meet must be the adapter's own)
+          const int last = __shfl_sync(0xffffffffu, tok, LR_GROUP - 1);
+          const bool run = p0 + q * LR_KB + warp * LR_GROUP + LR_GROUP <= pn &&
+                           last - __shfl_sync(0xffffffffu, tok, 0) == LR_GROUP - 1;
+          if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * LR_GROUP * 128 + (warp == 0 ? u_stage : 0));
+          __syncwarp();
+          lora_rows_load(dv, map, &full[st], c0, tok, run, LR_GROUP);
+          lora_rows_load(dv + 8192, map, &full[st], c0 + 64, tok, run, LR_GROUP);
+        } else {
+#pragma unroll 2
+          for (int j = 0; j < 8; ++j) {            // half a warp takes a row, 16 chunks
+            const int row = 2 * j + (lane >> 4), k8 = lane & 15;
+            const int tk = __shfl_sync(0xffffffffu, tok, row);
+            stage8_any(dv + (k8 >> 3) * 8192 + row * 128 + (((k8 & 7) ^ (row & 7)) << 4),
+                       v + int64_t(tk) * C + c0 + k8 * 8, C - c0 - k8 * 8, v_end);
           }
-          if (vec) stage_arrive<true>(&full[st]);
-          else stage_arrive<false>(&full[st]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(&full[st], warp == 0 ? u_stage : 0);
+          __syncwarp();
         }
-      } else {
-        const GridWalk u0(tid - 128, a.Rp >> 3);
-        const __nv_bfloat16 *ub = sd.u;
-        for (int q = 0; q < sg.count; ++q, ++it) {
-          const int st = it % S;
-          if (!(ok = mbar_wait(&empty[st], (uint32_t(it / S) & 1u) ^ 1u))) break;
-          const int pos = p0 + q * LR_KB;
-          const __nv_bfloat16 *up = ub + int64_t(pos) * a.Rp;
-#pragma unroll 4
-          for (GridWalk w = u0; w.major < LR_KB; w.next()) {
-            const bool in = pos + w.major < pn;
-            const __nv_bfloat16 *src = in ? up + w.major * a.Rp + w.minor * 8 : ub;
-            const uint32_t d = su + st * u_stage + w.minor * LG_MN_LD + w.major * 16;
-#pragma unroll
-            for (int i = 0; i < NS; ++i)
-              cp_async16(d + i * a.u_bytes, src + (in ? i * a.plane : 0), in ? 16u : 0u);
-          }
-          stage_arrive<true>(&full[st]);
-        }
+        if (warp == 0)
+          bulk_load_el(su + st * u_stage, u + int64_t(q) * a.np * a.Rp * 64, u_stage, &full[st]);
       }
       s += sg.count;
     }
-    cp_async_wait_all();
-  } else if (warp == 8) {
+    // the last stages' copies have landed before the CTA can end (bounded)
+    for (int e = max(0, it - S); e < it; ++e) warp_wait(&full[e % S], uint32_t(e / S) & 1u);
+  } else if (warp == 4) {
     // -------------------------------------------------------------- MMA issuer
     const uint32_t id = idesc_lora(a.Rp, 1, 1);
     int it = 0, seg = 0;
@@ -1019,16 +1218,15 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
           ok = false;
           break;
         }
-        fence_proxy_async_smem();
         tc_fence_after();
         const uint64_t dv = sdesc(sx + st * LG_X_BYTES, 8192, 1024, 2);
-        const uint64_t du = sdesc(su + st * u_stage, 128, LG_MN_LD, 0);
+        const uint64_t du = sdesc(su + st * u_stage, 128, 1024, 0);
 #pragma unroll
         for (int k = 0; k < 4; ++k)                 // 16 tokens an MMA
 #pragma unroll
           for (int i = 0; i < NS; ++i)
             tc_mma_bf16_el(acc, dv + uint64_t(128 * k),
-                           du + uint64_t(16 * k) + uint64_t(i * (a.u_bytes >> 4)), id,
+                           du + uint64_t(16 * k) + uint64_t(i * (u_bytes >> 4)), id,
                            (q || k || i) ? 1u : 0u);
         tc_commit_el(&empty[st]);
       }
@@ -1041,7 +1239,7 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
     __syncwarp();
   } else {
     // -------------------------------------------------------------- epilogue
-    const int e4 = tid - 288;                       // 0 .. 127
+    const int e4 = tid - 160;                       // 0 .. 127
     const int col = 32 * (warp & 3) + lane;         // this thread's TMEM lane and column
     int seg = 0;
     bool ok = true;
@@ -1136,7 +1334,7 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 4) {
     tc_fence_after();
     tmem_dealloc(tmem, cols);
   }

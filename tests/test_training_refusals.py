@@ -49,11 +49,13 @@ def test_workspaces_stay_proportionate():
     lib = L.load()
     for T in (1, 64, 777, 8192):
         for n in (1, 64, 1024):
-            # a few floats a token and rank; for the gradients at most two partial sums a CTA
+            # three bf16 values a token and rank (an adapter's tokens padded to 64); for the
+            # gradients twice that and at most two partial sums a CTA
             f = lib.dsv41_lora_workspace_size(T, 7168, 4096, n, 64, 0)
             g = lib.dsv41_lora_workspace_size(T, 7168, 4096, n, 64, 1)
-            assert f <= T * (64 * 6 + 64) + n * 64 + (1 << 20)
-            assert g <= 2 * f + T * 64 * 6 + 2 * 2 * 148 * 64 * 128 * 4 + (1 << 20)
+            pad = min(n, T) * 64 * 64 * 6
+            assert f <= T * (64 * 6 + 64) + pad + n * 64 + (1 << 20)
+            assert g <= 2 * (f + T * 64 * 6 + pad + (1 << 20)) + 2 * 2 * 148 * 64 * 128 * 4 + n * 64
     assert lib.dsv41_moe_balance_workspace_size(65536, 384, 16) <= 65536 * 8 + 4096
 
 
