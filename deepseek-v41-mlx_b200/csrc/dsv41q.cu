@@ -360,19 +360,23 @@ cudaError_t max_dynamic_smem(void (*kernel)(KArgs...), size_t bytes) {
   return e;
 }
 
+// A launch in clusters; with `after`, as the programmatic dependent of the launch before it (the
+// kernel waits for that one's results itself).
 template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsigned cluster, unsigned block,
-                           size_t smem, cudaStream_t st, Args... args) {
+cudaError_t launch_cluster(bool after, void (*kernel)(KArgs...), unsigned grid, unsigned cluster,
+                           unsigned block, size_t smem, cudaStream_t st, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim = {cluster, 1, 1};
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = after ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -749,7 +753,7 @@ cudaError_t balance_go(const BalArgs &p, const BalShape &sh, cudaStream_t st) {
   if (sh.cluster) {
     cudaError_t e = max_dynamic_smem(k_balance_small<IT, NV, VEC, GRAD>, sh.smem);
     if (e != cudaSuccess) return e;
-    return launch_cluster(k_balance_small<IT, NV, VEC, GRAD>, sh.grid, sh.cluster, 32 * BL_WARPS,
+    return launch_cluster(false, k_balance_small<IT, NV, VEC, GRAD>, sh.grid, sh.cluster, 32 * BL_WARPS,
                           sh.smem, st, p);
   }
   k_balance<IT, NV, VEC, GRAD><<<sh.grid, 32 * BL_WARPS, sh.smem, st>>>(p);
@@ -831,7 +835,7 @@ extern "C" int dsv41_moe_balance(const void *logits, int dtype, int64_t T, int64
     ProfScope prof("balance_count", st);
     if (n <= BL_COUNT_INTS) {
       DSV41_LAUNCH(max_dynamic_smem(k_balance_count, n * 4), "balance_count");
-      DSV41_LAUNCH(launch_cluster(k_balance_count, 8, 8, 1024, size_t(n) * 4, st, p),
+      DSV41_LAUNCH(launch_cluster(false, k_balance_count, 8, 8, 1024, size_t(n) * 4, st, p),
                    "balance_count");
     } else {
       DSV41_LAUNCH(cudaMemsetAsync(p.live, 0, (S + 1) * 4, st), "balance memset");
@@ -988,7 +992,7 @@ int lora_plan_launch(const int32_t *ids, int64_t T, int64_t n, const LoraPlan &p
   DSV41_LAUNCH(max_dynamic_smem(k_lora_plan, smem), "lora_plan");
   const unsigned C = unsigned(std::min<int64_t>(LP_MAX_CTAS, ceil_div(T, 1024)));
   ProfScope prof("lora_plan", st);
-  DSV41_LAUNCH(launch_cluster(k_lora_plan, C, C, 1024, smem, st, ids, int(T), int(n), plan),
+  DSV41_LAUNCH(launch_cluster(false, k_lora_plan, C, C, 1024, smem, st, ids, int(T), int(n), plan),
                "lora_plan");
   return DSV41_OK;
 }
@@ -1000,11 +1004,11 @@ template <typename OT>
 cudaError_t lora_decode_launch(const LoraDecode &p, int64_t T, cudaStream_t st) {
   const unsigned C = 8;
   const unsigned grid = unsigned(T) * C;
-  if (p.R <= 8) return launch_cluster(k_lora_decode<OT, 1, 1>, grid, C, LD_THREADS, 0, st, p);
-  if (p.R <= 16) return launch_cluster(k_lora_decode<OT, 2, 2>, grid, C, LD_THREADS, 0, st, p);
-  if (p.R <= 32) return launch_cluster(k_lora_decode<OT, 4, 4>, grid, C, LD_THREADS, 0, st, p);
-  if (p.R <= 64) return launch_cluster(k_lora_decode<OT, 8, 8>, grid, C, LD_THREADS, 0, st, p);
-  return launch_cluster(k_lora_decode<OT, 16, 16>, grid, C, LD_THREADS, 0, st, p);
+  if (p.R <= 8) return launch_cluster(false, k_lora_decode<OT, 1, 1>, grid, C, LD_THREADS, 0, st, p);
+  if (p.R <= 16) return launch_cluster(false, k_lora_decode<OT, 2, 2>, grid, C, LD_THREADS, 0, st, p);
+  if (p.R <= 32) return launch_cluster(false, k_lora_decode<OT, 4, 4>, grid, C, LD_THREADS, 0, st, p);
+  if (p.R <= 64) return launch_cluster(false, k_lora_decode<OT, 8, 8>, grid, C, LD_THREADS, 0, st, p);
+  return launch_cluster(false, k_lora_decode<OT, 16, 16>, grid, C, LD_THREADS, 0, st, p);
 }
 
 template <bool WMN, bool VEC, int S>
@@ -1013,7 +1017,7 @@ cudaError_t lora_shrink_go(const LoraShrinkMaps &maps, const LoraShrink &a, unsi
   const size_t smem = size_t(S) * (LS_X_BYTES + a.Rp * 128) + 1024;
   cudaError_t e = max_dynamic_smem(k_lora_shrink<WMN, VEC, S>, smem);
   if (e != cudaSuccess) return e;
-  return launch_cluster(k_lora_shrink<WMN, VEC, S>, clusters * C, C, LS_THREADS, smem, st, maps, a);
+  return launch_cluster(true, k_lora_shrink<WMN, VEC, S>, clusters * C, C, LS_THREADS, smem, st, maps, a);
 }
 
 // The contraction is split over the CTAs of a cluster as far as the tiles leave SMs free (two
@@ -1064,8 +1068,7 @@ int lora_expand_launch(LoraExpand a, int64_t T, cudaStream_t st) {
   ProfScope prof("lora_expand", st);
   cudaError_t e = max_dynamic_smem(k_lora_expand<WMN, OT>, smem);
   if (e == cudaSuccess) {
-    k_lora_expand<WMN, OT><<<grid, LE_THREADS, smem, st>>>(maps, a);
-    e = cudaGetLastError();
+    e = launch_pdl_if(true, k_lora_expand<WMN, OT>, dim3(grid), dim3(LE_THREADS), smem, st, maps, a);
   }
   return cuda_status(e, "lora_expand");
 }
@@ -1075,8 +1078,8 @@ cudaError_t lora_wgrad_go(const LoraWgradMaps &m, const LoraWgrad &a, const Lora
                           cudaStream_t st) {
   cudaError_t e = max_dynamic_smem(k_lora_wgrad<OT, S>, sh.smem);
   if (e != cudaSuccess) return e;
-  k_lora_wgrad<OT, S><<<unsigned(sh.grid), LG_THREADS, sh.smem, st>>>(m, a);
-  return cudaGetLastError();
+  return launch_pdl_if(true, k_lora_wgrad<OT, S>, dim3(unsigned(sh.grid)), dim3(LG_THREADS), sh.smem,
+                       st, m, a);
 }
 
 template <typename OT>

@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(1024, 1)
   __shared__ int wsum[32][3];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = gridDim.x, rank = blockIdx.x;
+  pdl_trigger();
   const int per = (((T + C - 1) / C) + 1023) & ~1023;
   const int t0 = int(min(int64_t(rank) * per, int64_t(T)));
   const int t1 = int(min(int64_t(t0) + per, int64_t(T)));
@@ -336,15 +337,21 @@ struct LoraPieces {
   __device__ __forceinline__ uint64_t desc_mn(uint32_t at, uint32_t rows) const {
     return swz ? sdesc(at, rows * rb, 8 * rb, swz) : sdesc(at, 128, rows * 16, 0);
   }
-  __device__ __forceinline__ uint32_t step_mn() const { return 16 * rb; }      // 16 rows
   // r is contracted
   __device__ __forceinline__ uint64_t desc_k(uint32_t at, uint32_t rows) const {
     return swz ? sdesc(at, 16, 8 * rb, swz) : sdesc(at, rows * 16, 128, 0);
   }
-  __device__ __forceinline__ uint32_t off_k(uint32_t k, uint32_t rows) const {  // k16 step k
-    const uint32_t b = 32 * k;
-    return swz ? b / rb * (rows * rb) + b % rb : 2 * k * rows * 16;
+};
+// Byte offset of the k-th MMA's 16 contraction indices in a staged operand (shifts only: the
+// issuing warp's address arithmetic is what an MMA of this size costs).
+struct LoraSteps {
+  uint32_t shift, mask, big;
+  __device__ __forceinline__ LoraSteps(uint32_t sh, uint32_t b) : shift(sh), mask((1u << sh) - 1), big(b) {}
+  static __device__ __forceinline__ LoraSteps mn(const LoraPieces &p) { return LoraSteps(0, 16 * p.rb); }
+  static __device__ __forceinline__ LoraSteps k(const LoraPieces &p, uint32_t rows) {
+    return p.swz ? LoraSteps(p.rb == 128 ? 2 : p.rb == 64 ? 1 : 0, rows * p.rb) : LoraSteps(0, rows * 32);
   }
+  __device__ __forceinline__ uint32_t at(uint32_t i) const { return (i >> shift) * big + (i & mask) * 32; }
 };
 
 // v as bf16 parts; the rest after each part is exact in fp32 (and zero after an infinity or NaN).
@@ -403,6 +410,7 @@ struct LoraShrinkMaps {
 };
 
 constexpr int LS_THREADS = 160;
+constexpr int LS_BATCH = 4;
 constexpr int LS_X_BYTES = LR_TILE * LR_KB * 2;     // 16 KB
 
 // D[128 tokens x Rp] in TMEM: tcgen05.mma kind::f16, M = 128, N = Rp.  A cluster of C CTAs
@@ -441,6 +449,8 @@ __global__ void __launch_bounds__(LS_THREADS, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  pdl_wait();                             // the plan
+  pdl_trigger();
   const int nkb = int((a.K + LR_KB - 1) / LR_KB);
   const int kb0 = int(int64_t(nkb) * rank / C), kb1 = int(int64_t(nkb) * (rank + 1) / C);
   const int ntiles = a.plan.head[0];
@@ -517,7 +527,7 @@ __global__ void __launch_bounds__(LS_THREADS, 2)
         const uint64_t da = sdesc_sw128(sx + s * LS_X_BYTES);
         const uint32_t bw = sw + s * (a.Rp * 128);
         const uint64_t db = WMN ? pc.desc_mn(bw, LR_KB) : sdesc_sw128(bw);
-        const uint32_t step = WMN ? pc.step_mn() >> 4 : 2;
+        const uint32_t step = WMN ? pc.rb : 2;        // 16 rows, or 32 bytes
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           tc_mma_bf16_el(tmem, da + uint64_t(2 * k), db + uint64_t(step * k), id,
@@ -532,6 +542,21 @@ __global__ void __launch_bounds__(LS_THREADS, 2)
     // thread sends its row to the CTA that adds that row, red[rank][row of the owner][Rp]
     float *red = reinterpret_cast<float *>(smem);
     const int ld = a.Rp + 4, own = LR_TILE / C;      // rows a CTA adds
+    const int q4 = a.Rp >> 2;
+    const float sc = a.scaling ? a.scaling[tl.adapter] : 1.0f;
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    // this thread's next pieces of h, requested ahead of the waits
+    float4 hv[LS_BATCH];
+    auto load_h = [&](int e0) {
+#pragma unroll
+      for (int u = 0; u < LS_BATCH; ++u) {
+        const int e = e0 + u * LS_THREADS, row = rank * own + e / q4, c4 = (e % q4) * 4;
+        hv[u] = zero;
+        if (a.h && e < own * q4 && c4 < a.R && row < tl.rows)
+          hv[u] = __ldg(reinterpret_cast<const float4 *>(a.h + int64_t(rows_s[row]) * a.R + c4));
+      }
+    };
+    load_h(tid);
     if (warp < 4) {
       if (ok) ok = warp_wait(&acc_full, uint32_t(done) & 1u);
       tc_fence_after();
@@ -554,28 +579,29 @@ __global__ void __launch_bounds__(LS_THREADS, 2)
     }
     cluster_sync();
     tc_fence_after();
-    const float sc = a.scaling ? a.scaling[tl.adapter] : 1.0f;
-    const int q4 = a.Rp >> 2;
-    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int e = tid; e < own * q4; e += LS_THREADS) {
-      const int lrow = e / q4, row = rank * own + lrow, c4 = (e % q4) * 4;
-      if (row >= ((tl.rows + 63) & ~63)) break;
-      const bool in = c4 < a.R && row < tl.rows;   // the padding of Rp and of the block: zeros
-      const int64_t tok = rows_s[row];
-      const float4 h = in && a.h ? __ldg(reinterpret_cast<const float4 *>(a.h + tok * a.R + c4)) : zero;
-      float4 s = zero;
-      if (in)
-        for (int q = 0; q < C; ++q) {
-          const float4 v = *reinterpret_cast<const float4 *>(red + (q * own + lrow) * ld + c4);
-          s.x += v.x;
-          s.y += v.y;
-          s.z += v.z;
-          s.w += v.w;
-        }
-      if (a.out && in) *reinterpret_cast<float4 *>(a.out + tok * a.R + c4) = s;
-      // (zeros are not scaled: an infinite scaling would make them NaN)
-      store_parts(a.parts, a.np, a.Rp, tl.block, row, c4, s, in ? sc : 1.0f);
-      if (a.h) store_parts(a.h_parts, a.np, a.Rp, tl.block, row, c4, h, in ? sc : 1.0f);
+#pragma unroll 1
+    for (int e0 = tid; e0 < own * q4; e0 += LS_BATCH * LS_THREADS) {
+      if (e0 != tid) load_h(e0);
+#pragma unroll
+      for (int u = 0; u < LS_BATCH; ++u) {
+        const int e = e0 + u * LS_THREADS;
+        const int lrow = e / q4, row = rank * own + lrow, c4 = (e % q4) * 4;
+        if (lrow >= own || row >= ((tl.rows + 63) & ~63)) break;
+        const bool in = c4 < a.R && row < tl.rows;   // the padding of Rp and of the block: zeros
+        float4 s = zero;
+        if (in)
+          for (int q = 0; q < C; ++q) {
+            const float4 v = *reinterpret_cast<const float4 *>(red + (q * own + lrow) * ld + c4);
+            s.x += v.x;
+            s.y += v.y;
+            s.z += v.z;
+            s.w += v.w;
+          }
+        if (a.out && in) *reinterpret_cast<float4 *>(a.out + int64_t(rows_s[row]) * a.R + c4) = s;
+        // (zeros are not scaled: an infinite scaling would make them NaN)
+        store_parts(a.parts, a.np, a.Rp, tl.block, row, c4, s, in ? sc : 1.0f);
+        if (a.h) store_parts(a.h_parts, a.np, a.Rp, tl.block, row, c4, hv[u], in ? sc : 1.0f);
+      }
     }
     __syncthreads();                      // before the stages are written again
     // the copies' writes come after these reads and the peers' stores
@@ -784,6 +810,8 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  pdl_wait();                             // the parts
+  pdl_trigger();
   const int per_tile = (a.ncb + a.cpu - 1) / a.cpu, rg = a.Rp >> 3;
   const int64_t items = int64_t(a.plan.head[0]) * per_tile;
   bool ok = true;
@@ -825,6 +853,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
     // -------------------------------------------------------------- MMA issuer
     const uint32_t id = idesc_lora(CB, 0, WMN ? 1 : 0);
     const LoraPieces pc(WMN ? CB : a.pw);
+    const LoraSteps steps = WMN ? LoraSteps::mn(pc) : LoraSteps::k(pc, CB);
     for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
       if (a.plan.tiles[item / per_tile].x >= a.n) continue;
       const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
@@ -842,11 +871,10 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
         const uint32_t bw = sw + b * w_bytes;
         const uint64_t db = WMN ? pc.desc_mn(bw, a.Rp) : pc.desc_k(bw, CB);
         for (int i = NS - 1; i >= 0; --i)                        // the smallest parts first
-          for (int k = 0; k < a.Rp / 16; ++k) {
-            const uint32_t off = WMN ? k * pc.step_mn() : pc.off_k(k, CB);
+#pragma unroll 4
+          for (int k = 0; k < a.Rp / 16; ++k)
             tc_mma_bf16_el(tmem + b * CB, da + uint64_t(uint32_t(i * rg + 2 * k) * 128),
-                           db + uint64_t(off >> 4), id, (i < NS - 1 || k) ? 1u : 0u);
-          }
+                           db + uint64_t(steps.at(k) >> 4), id, (i < NS - 1 || k) ? 1u : 0u);
         tc_commit_el(&w_empty[b]);
         tc_commit_el(&acc_full[b]);
       }
@@ -1144,6 +1172,7 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  pdl_wait();                             // the parts
   const int64_t stages = a.plan.stages[a.n], all = stages * (a.side[0].ncb + a.side[1].ncb);
   const int used = max(1, a.plan.head[1]);
   const int64_t per = max((all + gridDim.x - 1) / gridDim.x,
