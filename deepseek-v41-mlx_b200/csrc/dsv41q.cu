@@ -983,6 +983,22 @@ int lora_bank_map(CUtensorMap *m, const void *p, int64_t n, int64_t rows, int64_
   return DSV41_OK;
 }
 
+// The parts [blocks][np Rp / 8][1 KB] for expand's A operand: two blocks' groups of one part,
+// [group][block][1 KB] in shared memory
+int lora_parts_map(CUtensorMap *m, const void *p, int64_t blocks, int np, int Rp) {
+  int rc = get_encoder();
+  if (rc) return rc;
+  const cuuint64_t kb = 1024, row = cuuint64_t(np) * (Rp / 8) * kb;
+  cuuint64_t dims[3] = {256, cuuint64_t(blocks), cuuint64_t(np) * (Rp / 8)}, strides[2] = {row, kb};
+  cuuint32_t box[3] = {256, 2, cuuint32_t(Rp / 8)}, estr[3] = {1, 1, 1};
+  const CUresult r = g_encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void *>(p), dims,
+                                    strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                    CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(DSV41_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return DSV41_OK;
+}
+
 // values of r a piece (LoraPieces)
 int lora_pw(int64_t R) { return R % 64 == 0 ? 64 : R % 32 == 0 ? 32 : R % 16 == 0 ? 16 : 8; }
 
@@ -1042,24 +1058,41 @@ int lora_shrink_launch(LoraShrink a, int64_t T, cudaStream_t st) {
   return DSV41_OK;
 }
 
-// Work items of up to 32 column blocks (128 bytes of a row each), about three for each CTA; the
-// rest of the shared memory is the ring of base and output tiles.
+// Column blocks (128 bytes of a row each) of a work item.  With w blocks a CTA, items of c blocks
+// end up to c blocks apart and each costs about a block to start: c = sqrt(w) has the least of
+// both.  (How many tiles the adapters' ends add is not known here, so the items are not fitted to
+// the number of CTAs: that ran a second round for a few items, 53 against 37 us at T 4096.)
+int lora_expand_cpu(int64_t tiles, int64_t ncb, int64_t slots) {
+  int64_t c = 1;
+  while (c < ncb && c * c * slots < tiles * ncb) ++c;
+  return int(c);
+}
+
+// What the parts (two buffers if they fit) and W's blocks (four or two) leave of the shared memory
+// is the ring of base and output tiles.
 template <bool WMN, typename OT>
 int lora_expand_launch(LoraExpand a, int64_t T, cudaStream_t st) {
-  constexpr int CB = 128 / int(sizeof(OT));
+  constexpr int CB = 128 / int(sizeof(OT)), NS = sizeof(OT) == 4 ? 3 : 2;
   a.Rp = lora_rp(a.R);
   a.pw = lora_pw(a.R);
-  const size_t rest = size_t((sizeof(OT) == 4 ? 3 : 2) * (a.Rp / 8)) * 2048 +
-                      size_t(LE_BUF) * CB * a.Rp * 2 + 1024;
-  a.ring = int(std::min<size_t>(LE_RING_MAX, (225 * 1024 - rest) / LE_TILE_BYTES)) & ~1;
+  size_t rest = 0;
+  for (int choice = 0; choice < 3; ++choice) {
+    a.abuf = choice < 2 ? 2 : 1;
+    a.wbuf = choice == 1 ? 2 : LE_BUF;
+    rest = size_t(a.abuf) * NS * a.Rp * 256 + size_t(a.wbuf) * CB * a.Rp * 2 + 1024;
+    a.ring = rest > 193 * 1024 ? 0 : int(std::min<size_t>(LE_RING_MAX, (225 * 1024 - rest) / LE_TILE_BYTES));
+    a.ring -= a.ring % LE_GROUPS;
+    if (a.ring >= 2 * LE_GROUPS) break;
+  }
   const size_t smem = rest + size_t(a.ring) * LE_TILE_BYTES;
   const int64_t slots = num_sms();
   a.ncb = int(ceil_div(a.N, CB));
-  a.cpu = int(std::max<int64_t>(1, std::min<int64_t>(32, ceil_div(T, LR_TILE) * a.ncb / (3 * slots))));
+  a.cpu = lora_expand_cpu(ceil_div(T, LR_TILE), a.ncb, slots);
   a.vec = a.N * sizeof(OT) % 16 == 0 && aligned(a.base, 16) && aligned(a.y, 16);
   LoraExpandMaps maps{};
   int rc = WMN ? lora_bank_map(&maps.w, a.w, a.n, a.R, a.N, CB, uint32_t(a.R))
                : lora_bank_map(&maps.w, a.w, a.n, a.N, a.R, uint32_t(a.pw), CB);
+  if (!rc) rc = lora_parts_map(&maps.parts, a.parts, lora_max_blocks(T, a.n), a.np, a.Rp);
   if (!rc && a.vec && a.base) rc = lora_rows_maps(&maps.base, a.base, T, a.N, sizeof(OT));
   if (!rc && a.vec) rc = lora_rows_maps(&maps.y, a.y, T, a.N, sizeof(OT));
   if (rc) return rc;

@@ -733,6 +733,19 @@ __global__ void __launch_bounds__(LD_THREADS) k_lora_decode(const LoraDecode p) 
 }
 
 // ------------------------------------------------------------------ expand
+// The MMAs of one block, NS parts (the smallest first) times KS steps: unrolled, about 42 cycles
+// an MMA to issue against 75 in a loop.
+template <int NS, int KS>
+__device__ __forceinline__ void lora_issue(uint32_t acc, uint64_t da, uint64_t db, uint32_t id,
+                                           const LoraSteps &steps, int rg) {
+#pragma unroll
+  for (int i = NS - 1; i >= 0; --i)
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+      tc_mma_bf16_el(acc, da + uint64_t(uint32_t(i * rg + 2 * k) * 128),
+                     db + uint64_t(steps.at(k) >> 4), id, (i < NS - 1 || k) ? 1u : 0u);
+}
+
 struct LoraExpand {
   const __nv_bfloat16 *parts;  // the parts of h times scaling (np of them)
   const __nv_bfloat16 *w;      // [n][N][R], or [n][R][N] (WMN)
@@ -743,18 +756,21 @@ struct LoraExpand {
   LoraPlan plan;
   int ncb, cpu;                // column blocks, and how many of them a work item takes
   int vec;                     // rows of base and y are 16-byte aligned: TMA moves them
-  int ring;                    // tiles of 128 rows x 128 bytes in shared memory (even)
+  int ring;                    // tiles of 128 rows x 128 bytes in shared memory (of LE_GROUPS)
+  int abuf, wbuf;              // buffers of the parts and of W's column blocks
   int pw;                      // !WMN: see LoraPieces
 };
 struct LoraExpandMaps {
   LoraRows base, y;
   CUtensorMap w;               // [n][N][R], box pw x CB columns; WMN: [n][R][N], box CB columns x R
+  CUtensorMap parts;           // [np Rp / 8][blocks][1 KB], box of a part's groups of two blocks
 };
 
-constexpr int LE_THREADS = 14 * 32;
-constexpr int LE_BUF = 4;                         // column blocks of W and accumulators in flight
+constexpr int LE_GROUPS = 3;                      // epilogues of four warps that take turns
+constexpr int LE_THREADS = (6 + 4 * LE_GROUPS) * 32;
+constexpr int LE_BUF = 4;                         // accumulators (and at most as many blocks of W)
 constexpr int LE_TILE_BYTES = LR_TILE * 128;      // 16 KB
-constexpr int LE_RING_MAX = 8;
+constexpr int LE_RING_MAX = 9;
 constexpr int LE_EPI_LD = 36;                     // floats of a transposition row (odd rows only)
 
 // D[128 tokens x CB columns] in TMEM (tcgen05.mma kind::f16; CB columns are 128 bytes of a row of
@@ -764,7 +780,8 @@ constexpr int LE_EPI_LD = 36;                     // floats of a transposition r
 // the epilogue adds the accumulators to it in place, a thread a row, and the tile goes out the
 // same way (128-byte swizzle: no bank conflicts); rows that follow one another move 16 an
 // instruction, others four.  Warps 0-3 fetch base, 4 issues the MMAs, 5 fetches W and the parts,
-// 6-9 and 10-13 are two epilogues that take turns.  Row-wise plain loads and stores, through a
+// the others are three epilogues that take turns (one's turn is about 2500 cycles a tile: two fell
+// behind HBM).  Row-wise plain loads and stores, through a
 // transposition in shared memory, kept the load/store pipe busy for twice the time that HBM
 // needs (135 us at T 8192, N 14336, R 32).  Rows that TMA cannot address (odd lengths) are still
 // moved that way.
@@ -777,14 +794,16 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
   uint8_t *smem = le_raw + ((1024u - (smem_u32(le_raw) & 1023u)) & 1023u);
   const uint32_t w_bytes = uint32_t(CB) * a.Rp * 2;
   const uint32_t s_ring = smem_u32(smem), sw = s_ring + a.ring * LE_TILE_BYTES,
-                 sa = sw + LE_BUF * w_bytes;
-  __shared__ uint64_t a_full, a_empty, w_full[LE_BUF], w_empty[LE_BUF], acc_full[LE_BUF],
+                 sa = sw + a.wbuf * w_bytes, a_bytes = uint32_t(NS) * a.Rp * 256;
+  __shared__ uint64_t a_full[2], a_empty[2], w_full[LE_BUF], w_empty[LE_BUF], acc_full[LE_BUF],
       acc_empty[LE_BUF], b_full[LE_RING_MAX], b_empty[LE_RING_MAX];
   __shared__ uint32_t tmem_slot;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    mbar_init(&a_full, 1);
-    mbar_init(&a_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&a_full[i], 1);
+      mbar_init(&a_empty[i], 1);
+    }
     for (int i = 0; i < LE_BUF; ++i) {
       mbar_init(&w_full[i], 1);
       mbar_init(&w_empty[i], 1);
@@ -802,7 +821,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
     tmem_relinquish();
   }
   if (a.Rp > a.R) {               // the contraction's padding: zero for good, no copy writes it
-    for (int e = tid; e < LE_BUF * CB; e += LE_THREADS)
+    for (int e = tid; e < a.wbuf * CB; e += LE_THREADS)
       st_shared16(sw + e / CB * w_bytes + uint32_t(a.R) * CB * 2 + e % CB * 16, make_uint4(0, 0, 0, 0));
     fence_proxy_async_smem();
   }
@@ -857,28 +876,35 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
     for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
       if (a.plan.tiles[item / per_tile].x >= a.n) continue;
       const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
-      if (!(ok = warp_wait(&a_full, uint32_t(live) & 1u))) break;
+      const int ab = live % a.abuf;
+      if (!(ok = warp_wait(&a_full[ab], uint32_t(live / a.abuf) & 1u))) break;
       ++live;
+      const uint64_t da = sdesc(sa + ab * a_bytes, 2048, 128, 0);
       for (int cb = cb0; cb < cb1; ++cb, ++blk) {
-        const int b = blk % LE_BUF;
-        const uint32_t ph = uint32_t(blk / LE_BUF) & 1u;
-        if (!warp_wait(&acc_empty[b], ph ^ 1u) || !warp_wait(&w_full[b], ph)) {
+        const int b = blk % LE_BUF, wb = blk % a.wbuf;
+        if (!warp_wait(&acc_empty[b], (uint32_t(blk / LE_BUF) & 1u) ^ 1u) ||
+            !warp_wait(&w_full[wb], uint32_t(blk / a.wbuf) & 1u)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint64_t da = sdesc(sa, 2048, 128, 0);
-        const uint32_t bw = sw + b * w_bytes;
+        const uint32_t bw = sw + wb * w_bytes;
         const uint64_t db = WMN ? pc.desc_mn(bw, a.Rp) : pc.desc_k(bw, CB);
-        for (int i = NS - 1; i >= 0; --i)                        // the smallest parts first
-#pragma unroll 4
-          for (int k = 0; k < a.Rp / 16; ++k)
-            tc_mma_bf16_el(tmem + b * CB, da + uint64_t(uint32_t(i * rg + 2 * k) * 128),
-                           db + uint64_t(steps.at(k) >> 4), id, (i < NS - 1 || k) ? 1u : 0u);
-        tc_commit_el(&w_empty[b]);
+        switch (a.Rp) {
+          case 16: lora_issue<NS, 1>(tmem + b * CB, da, db, id, steps, rg); break;
+          case 32: lora_issue<NS, 2>(tmem + b * CB, da, db, id, steps, rg); break;
+          case 64: lora_issue<NS, 4>(tmem + b * CB, da, db, id, steps, rg); break;
+          case 128: lora_issue<NS, 8>(tmem + b * CB, da, db, id, steps, rg); break;
+          default:
+            for (int i = NS - 1; i >= 0; --i)
+              for (int k = 0; k < a.Rp / 16; ++k)
+                tc_mma_bf16_el(tmem + b * CB, da + uint64_t(uint32_t(i * rg + 2 * k) * 128),
+                               db + uint64_t(steps.at(k) >> 4), id, (i < NS - 1 || k) ? 1u : 0u);
+        }
+        tc_commit_el(&w_empty[wb]);
         tc_commit_el(&acc_full[b]);
       }
-      if (ok) tc_commit_el(&a_empty);
+      if (ok) tc_commit_el(&a_empty[ab]);
     }
     __syncwarp();
   } else if (warp == 5) {
@@ -887,20 +913,19 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
       const int4 tl = a.plan.tiles[item / per_tile];
       if (tl.x >= a.n) continue;
       const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
-      // the tile's one or two blocks of parts, a [64][8] group a copy
-      if (!(ok = warp_wait(&a_empty, (uint32_t(live) & 1u) ^ 1u))) break;
+      // two 64-row blocks of parts (the second may be another adapter's: its rows reach only
+      // accumulator rows that nobody reads)
+      const int ab = live % a.abuf;
+      if (!(ok = warp_wait(&a_empty[ab], (uint32_t(live / a.abuf) & 1u) ^ 1u))) break;
       ++live;
-      const int nb = tl.z > 64 ? 2 : 1;
-      if (lane == 0) mbar_arrive_expect_tx(&a_full, uint32_t(nb * NS * rg) * 1024);
+      if (lane == 0) mbar_arrive_expect_tx(&a_full[ab], a_bytes);
       __syncwarp();
-      for (int b = 0; b < nb; ++b) {
-        const __nv_bfloat16 *src = a.parts + int64_t(tl.w + b) * a.np * a.Rp * 64;
-        for (int g = 0; g < NS * rg; ++g)
-          bulk_load_el(sa + g * 2048 + b * 1024, src + g * 512, 1024, &a_full);
-      }
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        tma_load_3d_el(sa + ab * a_bytes + i * a.Rp * 256, &maps.parts, &a_full[ab], 0, tl.w, i * rg);
       for (int cb = cb0; cb < cb1; ++cb, ++blk) {
-        const int b = blk % LE_BUF;
-        if (!(ok = warp_wait(&w_empty[b], (uint32_t(blk / LE_BUF) & 1u) ^ 1u))) break;
+        const int b = blk % a.wbuf;
+        if (!(ok = warp_wait(&w_empty[b], (uint32_t(blk / a.wbuf) & 1u) ^ 1u))) break;
         const uint32_t dw = sw + b * w_bytes;
         if (lane == 0) mbar_arrive_expect_tx(&w_full[b], uint32_t(CB) * a.R * 2);
         __syncwarp();
@@ -913,9 +938,10 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
       }
     }
     // the last copies have landed before the CTA can end (bounded)
-    if (live > 0) warp_wait(&a_full, uint32_t(live - 1) & 1u);
-    for (int e = max(0, blk - LE_BUF); e < blk; ++e)
-      warp_wait(&w_full[e % LE_BUF], uint32_t(e / LE_BUF) & 1u);
+    for (int e = max(0, live - a.abuf); e < live; ++e)
+      warp_wait(&a_full[e % a.abuf], uint32_t(e / a.abuf) & 1u);
+    for (int e = max(0, blk - a.wbuf); e < blk; ++e)
+      warp_wait(&w_full[e % a.wbuf], uint32_t(e / a.wbuf) & 1u);
   } else {
     // -------------------------------------------------------------- epilogue
     const OT *base = static_cast<const OT *>(a.base);
@@ -930,7 +956,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
       const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
       const int tok = row < tl.z ? a.plan.perm[tl.y + row] : -1;
       for (int cb = cb0; cb < cb1; ++cb, ++all, blk += has ? 1 : 0) {
-        if ((all & 1) != grp) continue;
+        if (all % LE_GROUPS != grp) continue;
         const int b = blk % LE_BUF, s = all % a.ring;
         const uint32_t tacc = tmem + (uint32_t(32 * q4) << 16) + b * CB;
         if (a.vec) {
@@ -942,6 +968,17 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
           }
           // a warp whose wait ran out goes on without waiting
           if (base && ok) ok = warp_wait(&b_full[s], uint32_t(all / a.ring) & 1u);
+        }
+        OT odd[CB / 32][32];                               // !vec: base, a row a register
+        if (!a.vec && base) {
+#pragma unroll
+          for (int h = 0; h < CB / 32; ++h)
+#pragma unroll
+            for (int r = 0; r < 32; ++r) {
+              const int tk = __shfl_sync(0xffffffffu, tok, r);
+              const int64_t c = int64_t(cb) * CB + h * 32 + lane;
+              odd[h][r] = tk >= 0 && c < a.N ? base[int64_t(tk) * a.N + c] : OT(0.0f);
+            }
         }
         if (has) {
           if (ok) ok = warp_wait(&acc_full[b], uint32_t(blk / LE_BUF) & 1u);
@@ -1040,14 +1077,12 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
             }
             __syncwarp();
             const int64_t c = int64_t(cb) * CB + h + lane;
-#pragma unroll 8
+#pragma unroll
             for (int r = 0; r < 32; ++r) {
               const int tk = __shfl_sync(0xffffffffu, tok, r);
-              if (tk < 0 || c >= a.N) continue;
-              const int64_t at = int64_t(tk) * a.N + c;
               float f = has ? tp[r * LE_EPI_LD + lane] : 0.0f;
-              if (base) f += float(base[at]);
-              y[at] = OT(f);
+              if (base) f += float(odd[h / 32][r]);
+              if (tk >= 0 && c < a.N) y[int64_t(tk) * a.N + c] = OT(f);
             }
             __syncwarp();
           }
@@ -1137,7 +1172,7 @@ __device__ __forceinline__ LoraSeg lora_seg(const LoraWgrad &a, int64_t s, int64
 // is written as fp32 partial sums (at most two per CTA) and the last CTA to arrive adds them in
 // order.  A piece is at least min(8, the average item's) stages: cutting a few microseconds of
 // loads costs more in the join than it saves.  Warps 0-3 fetch v's rows (missing ones repeat one of
-// the adapter's own, against zero rows of u), warp 0 also copies u's block; 4 issues the MMAs, 5-8 read TMEM; accumulators are double-buffered, so an item's stores
+// the adapter's own, against zero rows of u) and u's block, each every fourth stage; 4 issues the MMAs, 5-8 read TMEM; accumulators are double-buffered, so an item's stores
 // overlap the next one.
 template <typename OT, int S>
 __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_wgrad(
@@ -1154,7 +1189,7 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
   const uint32_t cols = lg_tmem_cols(a.Rp), acc_cols = cols / 2;
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 4);
+      mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -1194,39 +1229,47 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
       const int64_t C = sd.C;
       const __nv_bfloat16 *u = sd.u + int64_t(a.plan.stages[sg.adapter] + sg.first) * a.np * a.Rp * 64;
       const int c0 = sg.cb * LG_COLS;
-      int tok_n = a.plan.perm[min(p0 + warp * 16 + (lane & 15), pn - 1)];    // one stage ahead
-      for (int q = 0; q < sg.count; ++q, ++it) {
-        const int st = it % S;
-        const int tok = tok_n;
-        if (q + 1 < sg.count)
-          tok_n = a.plan.perm[min(p0 + (q + 1) * LR_KB + warp * 16 + (lane & 15), pn - 1)];
-        if (!(ok = warp_wait(&empty[st], (uint32_t(it / S) & 1u) ^ 1u))) break;
-        const uint32_t dv = sx + st * LG_X_BYTES + warp * 2048;
+      // every fourth stage is this warp's; its 64 rows as two tokens a lane, one turn ahead
+      int q = (warp - it) & 3;
+      int tn0 = a.plan.perm[min(p0 + q * LR_KB + lane, pn - 1)];
+      int tn1 = a.plan.perm[min(p0 + q * LR_KB + 32 + lane, pn - 1)];
+      for (; q < sg.count; q += 4) {
+        const int i = it + q, st = i % S;
+        const int tok[2] = {tn0, tn1};
+        tn0 = a.plan.perm[min(p0 + (q + 4) * LR_KB + lane, pn - 1)];
+        tn1 = a.plan.perm[min(p0 + (q + 4) * LR_KB + 32 + lane, pn - 1)];
+        if (!(ok = warp_wait(&empty[st], (uint32_t(i / S) & 1u) ^ 1u))) break;
+        const uint32_t dv = sx + st * LG_X_BYTES;
+        const int left = pn - p0 - q * LR_KB;              // rows of the adapter from here on
         if (vec) {
-          // (only rows of the stage itself: what u's zero rows meet must be the adapter's own)
-          const int last = __shfl_sync(0xffffffffu, tok, LR_GROUP - 1);
-          const bool run = p0 + q * LR_KB + warp * LR_GROUP + LR_GROUP <= pn &&
-                           last - __shfl_sync(0xffffffffu, tok, 0) == LR_GROUP - 1;
-          if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * LR_GROUP * 128 + (warp == 0 ? u_stage : 0));
+          if (lane == 0) mbar_arrive_expect_tx(&full[st], LG_X_BYTES + u_stage);
           __syncwarp();
-          lora_rows_load(dv, map, &full[st], c0, tok, run, LR_GROUP);
-          lora_rows_load(dv + 8192, map, &full[st], c0 + 64, tok, run, LR_GROUP);
+          bulk_load_el(su + st * u_stage, u + int64_t(q) * a.np * a.Rp * 64, u_stage, &full[st]);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            // (only rows of the stage itself: what u's zero rows meet must be the adapter's own)
+            const int tg = __shfl_sync(0xffffffffu, tok[g >> 1], (g & 1) * 16 + (lane & 15));
+            const bool run = left >= (g + 1) * LR_GROUP &&
+                             __shfl_sync(0xffffffffu, tg, 15) - __shfl_sync(0xffffffffu, tg, 0) == 15;
+            lora_rows_load(dv + g * 2048, map, &full[st], c0, tg, run, LR_GROUP);
+            lora_rows_load(dv + g * 2048 + 8192, map, &full[st], c0 + 64, tg, run, LR_GROUP);
+          }
         } else {
-#pragma unroll 2
-          for (int j = 0; j < 8; ++j) {            // half a warp takes a row, 16 chunks
+#pragma unroll 4
+          for (int j = 0; j < 32; ++j) {           // half a warp takes a row, 16 chunks
             const int row = 2 * j + (lane >> 4), k8 = lane & 15;
-            const int tk = __shfl_sync(0xffffffffu, tok, row);
+            const int tk = __shfl_sync(0xffffffffu, j < 16 ? tok[0] : tok[1], row & 31);
             stage8_any(dv + (k8 >> 3) * 8192 + row * 128 + (((k8 & 7) ^ (row & 7)) << 4),
                        v + int64_t(tk) * C + c0 + k8 * 8, C - c0 - k8 * 8, v_end);
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(&full[st], warp == 0 ? u_stage : 0);
+          if (lane == 0) mbar_arrive_expect_tx(&full[st], u_stage);
           __syncwarp();
-        }
-        if (warp == 0)
           bulk_load_el(su + st * u_stage, u + int64_t(q) * a.np * a.Rp * 64, u_stage, &full[st]);
+        }
       }
+      it += sg.count;
       s += sg.count;
     }
     // the last stages' copies have landed before the CTA can end (bounded)
