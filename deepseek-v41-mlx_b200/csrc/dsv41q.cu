@@ -944,9 +944,7 @@ LoraWs lora_carve(void *ws, size_t cap, int64_t T, int64_t K, int64_t N, int64_t
     // the larger of the two grids (bf16 and fp32 gradients)
     const int grid = std::max(lora_wgrad_shape(T, K, N, n, R, DSV41_BF16).grid,
                               lora_wgrad_shape(T, K, N, n, R, DSV41_F32).grid);
-    w.plan.tickets = c.take<int>(grid);
-    w.plan.n_tickets = grid;
-    w.sums = c.take<float>(size_t(2) * grid * lora_rp(R) * LG_COLS);
+    w.sums = c.take<float>(size_t(2) * grid * R * LG_COLS);
   }
   w.ok = c.ok;
   w.used = align_up(c.off, 256);
@@ -1111,8 +1109,11 @@ cudaError_t lora_wgrad_go(const LoraWgradMaps &m, const LoraWgrad &a, const Lora
                           cudaStream_t st) {
   cudaError_t e = max_dynamic_smem(k_lora_wgrad<OT, S>, sh.smem);
   if (e != cudaSuccess) return e;
-  return launch_pdl_if(true, k_lora_wgrad<OT, S>, dim3(unsigned(sh.grid)), dim3(LG_THREADS), sh.smem,
-                       st, m, a);
+  e = launch_pdl_if(true, k_lora_wgrad<OT, S>, dim3(unsigned(sh.grid)), dim3(LG_THREADS), sh.smem, st,
+                    m, a);
+  if (e != cudaSuccess) return e;
+  return launch_pdl_if(true, k_lora_join<OT>, dim3(unsigned(sh.grid), unsigned(a.R / 8)),
+                       dim3(LG_COLS), 0, st, a);
 }
 
 template <typename OT>
@@ -1261,6 +1262,7 @@ extern "C" int dsv41_lora_backward(const void *dy, const void *x, const float *h
   g.T = T;
   g.plan = w.plan;
   g.part = w.sums;
+  g.grid = sh.grid;
   LoraWgradMaps maps{};
   rc = lora_rows_maps(&maps.v[0], x, T, K, 2);
   if (!rc && N % 8 == 0) rc = lora_rows_maps(&maps.v[1], dy, T, N, 2);

@@ -38,8 +38,6 @@ struct LoraPlan {
   int *off;        // [n + 2] first position of each adapter (n: none), then T
   int *stages;     // [n + 1] 64-row blocks of the adapters before this one: where an adapter's
                    // parts begin, and wgrad's work
-  int *tickets;    // zeroed here: wgrad's joins
-  int n_tickets;
 };
 
 // The bin of token t: its adapter in [0, n), or n.  Ids at or past n raise the bad-index status.
@@ -132,7 +130,6 @@ __global__ void __launch_bounds__(1024, 1)
     used += __syncthreads_count(b < n && total > 0);
     for (int i = 0; i < 3; ++i) run[i] += tot[i];
   }
-  for (int i = rank * 1024 + tid; i < p.n_tickets; i += C * 1024) p.tickets[i] = 0;
   if (rank == 0 && tid == 0) {
     p.head[0] = run[1];
     p.head[1] = used;
@@ -1119,7 +1116,8 @@ struct LoraWgrad {
   int R, Rp, n, np;
   int64_t T;
   LoraPlan plan;
-  float *part;                 // [2 * grid][Rp][128] partial sums
+  float *part;                 // [2 * grid][R][128] partial sums
+  int grid;
 };
 struct LoraWgradMaps {
   LoraRows v[2];               // the long sides
@@ -1129,8 +1127,9 @@ constexpr int LG_THREADS = 288;
 constexpr int LG_COLS = 128;
 constexpr int LG_X_BYTES = LR_KB * LG_COLS * 2;     // 16 KB: 2 pieces of [64 tokens x 128 B]
 constexpr int LG_MIN_STAGES = 8;                    // a CTA's least share, see k_lora_wgrad
-__host__ __device__ __forceinline__ constexpr uint32_t lg_tmem_cols(int Rp) {
-  return Rp <= 32 ? 64u : Rp <= 64 ? 128u : 256u;   // two accumulators
+// Two accumulators of the MMA's N columns (at least 32: the epilogue reads 32 at a time).
+__host__ __device__ __forceinline__ constexpr uint32_t lg_acc_cols(int n) {
+  return n <= 32 ? 32u : n <= 64 ? 64u : n <= 128 ? 128u : 256u;
 }
 
 // One piece of work of a CTA: stages [s0, s1) of one (side, adapter, column block).
@@ -1164,16 +1163,59 @@ __device__ __forceinline__ LoraSeg lora_seg(const LoraWgrad &a, int64_t s, int64
   return g;
 }
 
+// How the CTAs cut the line of work: `per` stages each.  A piece is at least min(8, the average
+// item's) stages: cutting a few microseconds of loads costs more in the join than it saves.
+struct LoraCut {
+  int64_t all, per;
+  __device__ __forceinline__ explicit LoraCut(const LoraWgrad &a) {
+    const int64_t stages = a.plan.stages[a.n];
+    const int used = max(1, a.plan.head[1]);
+    all = stages * (a.side[0].ncb + a.side[1].ncb);
+    per = max((all + a.grid - 1) / a.grid, min(int64_t(LG_MIN_STAGES), (stages + used - 1) / used));
+    per = max(per, int64_t(1));
+  }
+};
+
+// One value per r of 32 from c0 on, for column c of the item: rounded and written
+template <typename OT>
+__device__ __forceinline__ void lora_wgrad_store(const LoraGradSide &sd, OT *out, int R, int64_t c,
+                                                 int c0, int count, const float *v) {
+  if (c >= sd.C) return;
+  if (sd.r_major) {
+#pragma unroll
+    for (int x = 0; x < 32; ++x)
+      if (x < count && c0 + x < R) out[int64_t(c0 + x) * sd.C + c] = OT(v[x]);
+    return;
+  }
+#pragma unroll
+  for (int x = 0; x < 32; x += 8)
+    if (x < count && c0 + x < R) {
+      OT *dst = out + c * R + c0 + x;
+      if constexpr (sizeof(OT) == 4) {
+        *reinterpret_cast<float4 *>(dst) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+        *reinterpret_cast<float4 *>(dst + 4) = make_float4(v[x + 4], v[x + 5], v[x + 6], v[x + 7]);
+      } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          w[y] = uint32_t(f2bf_bits(v[x + 2 * y])) | (uint32_t(f2bf_bits(v[x + 2 * y + 1])) << 16);
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+}
+
 // D[128 columns x Rp] = sum over an adapter's tokens, in TMEM; both operands have the token
 // index as their rows in memory, which is the MMA's contraction index: v as 128-byte-swizzled
-// pieces of 64 columns, u (its bf16 parts) as unswizzled groups of 8.  The work of both
-// gradients (every adapter's 64-token stages times the column blocks) is one line that the CTAs
-// cut into equal pieces: an item that one CTA covers is written at once, one that a cut divides
-// is written as fp32 partial sums (at most two per CTA) and the last CTA to arrive adds them in
-// order.  A piece is at least min(8, the average item's) stages: cutting a few microseconds of
-// loads costs more in the join than it saves.  Warps 0-3 fetch v's rows (missing ones repeat one of
-// the adapter's own, against zero rows of u) and u's block, each every fourth stage; 4 issues the MMAs, 5-8 read TMEM; accumulators are double-buffered, so an item's stores
-// overlap the next one.
+// pieces of 64 columns, u as unswizzled groups of 8.  u's bf16 parts stand side by side as NS Rp
+// columns of one MMA where 256 columns hold them (v is then read once for all of them) and the
+// epilogue adds them; else they are accumulated one after another.  The work of both gradients
+// (every adapter's 64-token stages times the column blocks) is one line that the CTAs cut into
+// equal pieces: an item that one CTA covers is written at once, one that a cut divides is written
+// as fp32 partial sums, at most two per CTA, which k_lora_join adds in order (the last CTA to
+// arrive did that first: 17 us of one CTA's time behind 41 us of work at T 8192, R 64).  Warps
+// 0-3 fetch v's rows (missing ones repeat one of the adapter's own, against zero rows of u) and
+// u's block, each every fourth stage; 4 issues the MMAs, 5-8 read TMEM; accumulators are
+// double-buffered, so an item's stores overlap the next one.
 template <typename OT, int S>
 __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_wgrad(
     const __grid_constant__ LoraWgradMaps maps, const LoraWgrad a) {
@@ -1184,9 +1226,10 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
   const uint32_t u_bytes = uint32_t(a.Rp) * 128, u_stage = NS * u_bytes;   // a part, all parts
   __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2], mma_done;
   __shared__ uint32_t tmem_slot;
-  __shared__ int last_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t cols = lg_tmem_cols(a.Rp), acc_cols = cols / 2;
+  const bool wide = NS * a.Rp <= 256;
+  const uint32_t mma_n = wide ? NS * a.Rp : a.Rp;
+  const uint32_t acc_cols = lg_acc_cols(int(mma_n)), cols = 2 * acc_cols;
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
@@ -1208,11 +1251,9 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   pdl_wait();                             // the parts
-  const int64_t stages = a.plan.stages[a.n], all = stages * (a.side[0].ncb + a.side[1].ncb);
-  const int used = max(1, a.plan.head[1]);
-  const int64_t per = max((all + gridDim.x - 1) / gridDim.x,
-                          min(int64_t(LG_MIN_STAGES), (stages + used - 1) / used));
-  const int64_t w0 = min(int64_t(blockIdx.x) * per, all), w1 = min(w0 + per, all);
+  pdl_trigger();
+  const LoraCut cut(a);
+  const int64_t w0 = min(int64_t(blockIdx.x) * cut.per, cut.all), w1 = min(w0 + cut.per, cut.all);
 
   if (warp < 4) {
     // -------------------------------------------------------------- producers
@@ -1276,7 +1317,7 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
     for (int e = max(0, it - S); e < it; ++e) warp_wait(&full[e % S], uint32_t(e / S) & 1u);
   } else if (warp == 4) {
     // -------------------------------------------------------------- MMA issuer
-    const uint32_t id = idesc_lora(a.Rp, 1, 1);
+    const uint32_t id = idesc_lora(mma_n, 1, 1);
     int it = 0, seg = 0;
     bool ok = true;
     for (int64_t s = w0; s < w1 && ok; ++seg) {
@@ -1293,13 +1334,19 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
         tc_fence_after();
         const uint64_t dv = sdesc(sx + st * LG_X_BYTES, 8192, 1024, 2);
         const uint64_t du = sdesc(su + st * u_stage, 128, 1024, 0);
+        if (wide) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)                 // 16 tokens an MMA
+          for (int k = 0; k < 4; ++k)               // 16 tokens an MMA
+            tc_mma_bf16_el(acc, dv + uint64_t(128 * k), du + uint64_t(16 * k), id, (q || k) ? 1u : 0u);
+        } else {
 #pragma unroll
-          for (int i = 0; i < NS; ++i)
-            tc_mma_bf16_el(acc, dv + uint64_t(128 * k),
-                           du + uint64_t(16 * k) + uint64_t(i * (u_bytes >> 4)), id,
-                           (q || k || i) ? 1u : 0u);
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int i = NS - 1; i >= 0; --i)
+              tc_mma_bf16_el(acc, dv + uint64_t(128 * k),
+                             du + uint64_t(16 * k) + uint64_t(i * (u_bytes >> 4)), id,
+                             (q || k || i < NS - 1) ? 1u : 0u);
+        }
         tc_commit_el(&empty[st]);
       }
       if (!ok) break;
@@ -1318,73 +1365,40 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
     for (int64_t s = w0; s < w1; ++seg) {
       const LoraSeg sg = lora_seg(a, s, w1);
       const LoraGradSide &sd = a.side[sg.side];
-      // a warp whose wait ran out goes on without waiting: the others meet it at the barriers
       if (ok) ok = warp_wait(&acc_full[seg & 1], uint32_t(seg >> 1) & 1u);
       tc_fence_after();
       const uint32_t acc = tmem + uint32_t(seg & 1) * acc_cols + (uint32_t(32 * (warp & 3)) << 16);
-      const int64_t f = sg.item0 / per, l = (sg.item0 + sg.total - 1) / per;   // CTAs of the item
-      OT *out = static_cast<OT *>(sd.out) + int64_t(sg.adapter) * a.R * sd.C;
-      bool join = f == l;
-      if (f != l) {
-        float *mine = a.part + int64_t(2 * int(blockIdx.x) + (s == w0 ? 0 : 1)) * a.Rp * LG_COLS;
-        for (int c0 = 0; c0 < a.Rp; c0 += 32) {
-          uint32_t v[32];
-          tmem_ld32(acc + c0, v);
+      const bool whole = sg.count == sg.total;
+      float *mine = a.part + int64_t(2 * int(blockIdx.x) + (s == w0 ? 0 : 1)) * a.R * LG_COLS + col;
+      for (int c0 = 0; c0 < a.R; c0 += 32) {
+        float v[32];
+        if (wide) {
+#pragma unroll
+          for (int i = NS - 1; i >= 0; --i) {        // the smallest parts first
+            uint32_t w[32];
+            tmem_ld32(acc + min(i * a.Rp + c0, int(acc_cols) - 32), w);
+            // (a part that ends less than 32 columns before the accumulator's end is read from
+            // further left)
+            const int back = max(0, i * a.Rp + c0 + 32 - int(acc_cols));
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+              const uint32_t at = back == 0 ? w[x] : x + 16 < 32 ? w[x + 16] : 0u;
+              v[x] = i == NS - 1 ? __uint_as_float(at) : v[x] + __uint_as_float(at);
+            }
+          }
+        } else {
+          uint32_t w[32];
+          tmem_ld32(acc + c0, w);
+#pragma unroll
+          for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(w[x]);
+        }
+        if (whole) {
+          lora_wgrad_store<OT>(sd, static_cast<OT *>(sd.out) + int64_t(sg.adapter) * a.R * sd.C, a.R,
+                               int64_t(sg.cb) * LG_COLS + col, c0, 32, v);
+        } else {
 #pragma unroll
           for (int x = 0; x < 32; ++x)
-            if (c0 + x < a.R) __stcg(mine + (c0 + x) * LG_COLS + col, __uint_as_float(v[x]));
-        }
-        __threadfence();
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (e4 == 0) last_s = atomicAdd(a.plan.tickets + f, 1) == int(l - f);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        join = last_s != 0;
-        if (join) __threadfence();
-      }
-      if (join) {
-        const int64_t c = int64_t(sg.cb) * LG_COLS + col;
-        for (int c0 = 0; c0 < a.Rp; c0 += 32) {
-          uint32_t v[32];
-          if (f == l) {
-            tmem_ld32(acc + c0, v);
-          } else {
-#pragma unroll
-            for (int x = 0; x < 32; ++x) v[x] = 0u;
-#pragma unroll 2
-            for (int64_t k = f; k <= l; ++k) {
-              const int sl = 2 * int(k) + (k == f && sg.item0 > f * per ? 1 : 0);
-              const float *src = a.part + int64_t(sl) * a.Rp * LG_COLS + col;
-#pragma unroll
-              for (int x = 0; x < 32; ++x)
-                if (c0 + x < a.R)
-                  v[x] = __float_as_uint(__uint_as_float(v[x]) + __ldcg(src + (c0 + x) * LG_COLS));
-            }
-          }
-          if (c < sd.C) {
-            if (sd.r_major) {
-#pragma unroll
-              for (int x = 0; x < 32; ++x)
-                if (c0 + x < a.R) out[int64_t(c0 + x) * sd.C + c] = OT(__uint_as_float(v[x]));
-            } else {
-#pragma unroll
-              for (int x = 0; x < 32; x += 8)
-                if (c0 + x < a.R) {
-                  OT *dst = out + c * a.R + c0 + x;
-                  if constexpr (sizeof(OT) == 4) {
-                    *reinterpret_cast<uint4 *>(dst) = make_uint4(v[x], v[x + 1], v[x + 2], v[x + 3]);
-                    *reinterpret_cast<uint4 *>(dst + 4) =
-                        make_uint4(v[x + 4], v[x + 5], v[x + 6], v[x + 7]);
-                  } else {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                      w[y] = uint32_t(f2bf_bits(__uint_as_float(v[x + 2 * y]))) |
-                             (uint32_t(f2bf_bits(__uint_as_float(v[x + 2 * y + 1]))) << 16);
-                    *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-                  }
-                }
-            }
-          }
+            if (c0 + x < a.R) mine[(c0 + x) * LG_COLS] = v[x];
         }
       }
       tc_fence_before();
@@ -1410,6 +1424,33 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
     tc_fence_after();
     tmem_dealloc(tmem, cols);
   }
+}
+
+// The items that a cut divides: block x adds those that begin in CTA x's piece and end in a later
+// one, eight r's a block; the partial sums in the order of the tokens.
+template <typename OT>
+__global__ void __launch_bounds__(LG_COLS) k_lora_join(const LoraWgrad a) {
+  pdl_wait();
+  const LoraCut cut(a);
+  const int64_t f = blockIdx.x, end = min((f + 1) * cut.per, cut.all);
+  if (f * cut.per >= end) return;
+  const LoraSeg sg = lora_seg(a, end - 1, end);
+  const int64_t item_end = sg.item0 + sg.total;
+  if (item_end <= end || sg.item0 < f * cut.per) return;
+  const int64_t l = (item_end - 1) / cut.per;
+  const LoraGradSide &sd = a.side[sg.side];
+  const int c0 = blockIdx.y * 8;
+  float v[32] = {};
+#pragma unroll 4
+  for (int64_t k = f; k <= l; ++k) {
+    // CTA k's piece of the item is its first one (place 0) unless the item begins inside it
+    const int64_t slot = 2 * k + (k == f && sg.item0 > f * cut.per ? 1 : 0);
+    const float *src = a.part + slot * a.R * LG_COLS + threadIdx.x;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] += __ldg(src + (c0 + x) * LG_COLS);
+  }
+  lora_wgrad_store<OT>(sd, static_cast<OT *>(sd.out) + int64_t(sg.adapter) * a.R * sd.C, a.R,
+                       int64_t(sg.cb) * LG_COLS + threadIdx.x, c0, 8, v);
 }
 
 }  // namespace dsv41
