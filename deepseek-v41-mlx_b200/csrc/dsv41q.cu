@@ -1063,21 +1063,30 @@ int lora_shrink_launch(LoraShrink a, int64_t T, cudaStream_t st) {
 int lora_expand_cpu(int64_t tiles, int64_t ncb, int64_t slots) {
   int64_t c = 1;
   while (c < ncb && c * c * slots < tiles * ncb) ++c;
-  return int(c);
+  return int(c + (c & 1));                       // an MMA takes two
+}
+
+template <bool WMN, typename OT, bool VEC>
+cudaError_t lora_expand_go(const LoraExpandMaps &maps, const LoraExpand &a, unsigned grid, size_t smem,
+                           cudaStream_t st) {
+  const cudaError_t e = max_dynamic_smem(k_lora_expand<WMN, OT, VEC>, smem);
+  if (e != cudaSuccess) return e;
+  return launch_pdl_if(true, k_lora_expand<WMN, OT, VEC>, dim3(grid), dim3(LE_THREADS), smem, st, maps,
+                       a);
 }
 
 // What the parts (two buffers if they fit) and W's blocks (four or two) leave of the shared memory
 // is the ring of base and output tiles.
 template <bool WMN, typename OT>
 int lora_expand_launch(LoraExpand a, int64_t T, cudaStream_t st) {
-  constexpr int CB = 128 / int(sizeof(OT)), NS = sizeof(OT) == 4 ? 3 : 2;
+  constexpr int CB = 128 / int(sizeof(OT)), MB = 2 * CB, NS = sizeof(OT) == 4 ? 3 : 2;
   a.Rp = lora_rp(a.R);
   a.pw = lora_pw(a.R);
   size_t rest = 0;
-  for (int choice = 0; choice < 3; ++choice) {
+  for (int choice = 0; choice < 4; ++choice) {
     a.abuf = choice < 2 ? 2 : 1;
-    a.wbuf = choice == 1 ? 2 : LE_BUF;
-    rest = size_t(a.abuf) * NS * a.Rp * 256 + size_t(a.wbuf) * CB * a.Rp * 2 + 1024;
+    a.wbuf = choice & 1 ? 2 : LE_BUF;
+    rest = size_t(a.abuf) * NS * a.Rp * 256 + size_t(a.wbuf) * MB * a.Rp * 2 + 1024;
     a.ring = rest > 193 * 1024 ? 0 : int(std::min<size_t>(LE_RING_MAX, (225 * 1024 - rest) / LE_TILE_BYTES));
     a.ring -= a.ring % LE_GROUPS;
     if (a.ring >= 2 * LE_GROUPS) break;
@@ -1086,21 +1095,19 @@ int lora_expand_launch(LoraExpand a, int64_t T, cudaStream_t st) {
   const int64_t slots = num_sms();
   a.ncb = int(ceil_div(a.N, CB));
   a.cpu = lora_expand_cpu(ceil_div(T, LR_TILE), a.ncb, slots);
-  a.vec = a.N * sizeof(OT) % 16 == 0 && aligned(a.base, 16) && aligned(a.y, 16);
+  const bool vec = a.N * sizeof(OT) % 16 == 0 && aligned(a.base, 16) && aligned(a.y, 16);
   LoraExpandMaps maps{};
   int rc = WMN ? lora_bank_map(&maps.w, a.w, a.n, a.R, a.N, CB, uint32_t(a.R))
-               : lora_bank_map(&maps.w, a.w, a.n, a.N, a.R, uint32_t(a.pw), CB);
+               : lora_bank_map(&maps.w, a.w, a.n, a.N, a.R, uint32_t(a.pw), MB);
   if (!rc) rc = lora_parts_map(&maps.parts, a.parts, lora_max_blocks(T, a.n), a.np, a.Rp);
-  if (!rc && a.vec && a.base) rc = lora_rows_maps(&maps.base, a.base, T, a.N, sizeof(OT));
-  if (!rc && a.vec) rc = lora_rows_maps(&maps.y, a.y, T, a.N, sizeof(OT));
+  if (!rc && vec && a.base) rc = lora_rows_maps(&maps.base, a.base, T, a.N, sizeof(OT));
+  if (!rc && vec) rc = lora_rows_maps(&maps.y, a.y, T, a.N, sizeof(OT));
   if (rc) return rc;
   const unsigned grid = unsigned(std::min<int64_t>(
       lora_max_tiles(T, a.n) * ceil_div(a.ncb, a.cpu), slots));
   ProfScope prof("lora_expand", st);
-  cudaError_t e = max_dynamic_smem(k_lora_expand<WMN, OT>, smem);
-  if (e == cudaSuccess) {
-    e = launch_pdl_if(true, k_lora_expand<WMN, OT>, dim3(grid), dim3(LE_THREADS), smem, st, maps, a);
-  }
+  const cudaError_t e = vec ? lora_expand_go<WMN, OT, true>(maps, a, grid, smem, st)
+                            : lora_expand_go<WMN, OT, false>(maps, a, grid, smem, st);
   return cuda_status(e, "lora_expand");
 }
 

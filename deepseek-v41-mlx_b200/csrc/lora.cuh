@@ -751,15 +751,14 @@ struct LoraExpand {
   const void *base;            // [T, N] or NULL
   void *y;                     // [T, N]
   LoraPlan plan;
-  int ncb, cpu;                // column blocks, and how many of them a work item takes
-  int vec;                     // rows of base and y are 16-byte aligned: TMA moves them
+  int ncb, cpu;                // column blocks of 128 bytes of a row, and how many (even) an item takes
   int ring;                    // tiles of 128 rows x 128 bytes in shared memory (of LE_GROUPS)
   int abuf, wbuf;              // buffers of the parts and of W's column blocks
   int pw;                      // !WMN: see LoraPieces
 };
 struct LoraExpandMaps {
   LoraRows base, y;
-  CUtensorMap w;               // [n][N][R], box pw x CB columns; WMN: [n][R][N], box CB columns x R
+  CUtensorMap w;               // [n][N][R], box pw x MB columns; WMN: [n][R][N], box CB columns x R
   CUtensorMap parts;           // [np Rp / 8][blocks][1 KB], box of a part's groups of two blocks
 };
 
@@ -770,8 +769,9 @@ constexpr int LE_TILE_BYTES = LR_TILE * 128;      // 16 KB
 constexpr int LE_RING_MAX = 9;
 constexpr int LE_EPI_LD = 36;                     // floats of a transposition row (odd rows only)
 
-// D[128 tokens x CB columns] in TMEM (tcgen05.mma kind::f16; CB columns are 128 bytes of a row of
-// y): the tile's parts are the A operand, contraction NS * Rp, staged once for a work item's
+// D[128 tokens x MB columns] in TMEM (tcgen05.mma kind::f16; MB = 2 CB columns, CB are 128 bytes
+// of a row of y; with CB alone the MMAs of R = 128, which read the parts from shared memory every
+// time, took longer than the stores): the tile's parts are the A operand, contraction NS * Rp, staged once for a work item's
 // column blocks; a block of W is the B operand, in its own order in memory (rows of r for B,
 // columns contiguous for A: the MMA takes either).  base comes in through a ring of 16 KB tiles,
 // the epilogue adds the accumulators to it in place, a thread a row, and the tile goes out the
@@ -780,16 +780,17 @@ constexpr int LE_EPI_LD = 36;                     // floats of a transposition r
 // the others are three epilogues that take turns (one's turn is about 2500 cycles a tile: two fell
 // behind HBM).  Row-wise plain loads and stores, through a
 // transposition in shared memory, kept the load/store pipe busy for twice the time that HBM
-// needs (135 us at T 8192, N 14336, R 32).  Rows that TMA cannot address (odd lengths) are still
-// moved that way.
-template <bool WMN, typename OT>
+// needs (135 us at T 8192, N 14336, R 32).  Rows that TMA cannot address (VEC false: odd lengths)
+// are still moved that way, by a kernel of their own (in one kernel its unrolled rows pushed the
+// hot loop out of the instruction cache).
+template <bool WMN, typename OT, bool VEC>
 __global__ void __launch_bounds__(LE_THREADS, 1)
     k_lora_expand(const __grid_constant__ LoraExpandMaps maps, const LoraExpand a) {
   constexpr int NS = sizeof(OT) == 4 ? 3 : 2;
-  constexpr int CB = 128 / int(sizeof(OT));       // columns of a block
+  constexpr int CB = 128 / int(sizeof(OT)), MB = 2 * CB;       // columns of a block, of an MMA
   extern __shared__ uint8_t le_raw[];
   uint8_t *smem = le_raw + ((1024u - (smem_u32(le_raw) & 1023u)) & 1023u);
-  const uint32_t w_bytes = uint32_t(CB) * a.Rp * 2;
+  const uint32_t w_bytes = uint32_t(MB) * a.Rp * 2;
   const uint32_t s_ring = smem_u32(smem), sw = s_ring + a.ring * LE_TILE_BYTES,
                  sa = sw + a.wbuf * w_bytes, a_bytes = uint32_t(NS) * a.Rp * 256;
   __shared__ uint64_t a_full[2], a_empty[2], w_full[LE_BUF], w_empty[LE_BUF], acc_full[LE_BUF],
@@ -805,7 +806,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
       mbar_init(&w_full[i], 1);
       mbar_init(&w_empty[i], 1);
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 4);
+      mbar_init(&acc_empty[i], 8);
     }
     for (int i = 0; i < a.ring; ++i) {
       mbar_init(&b_full[i], 4);
@@ -814,12 +815,16 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
     fence_barrier_init();
   }
   if (warp == 4) {
-    tmem_alloc(&tmem_slot, LE_BUF * CB);
+    tmem_alloc(&tmem_slot, LE_BUF * MB);
     tmem_relinquish();
   }
   if (a.Rp > a.R) {               // the contraction's padding: zero for good, no copy writes it
-    for (int e = tid; e < a.wbuf * CB; e += LE_THREADS)
-      st_shared16(sw + e / CB * w_bytes + uint32_t(a.R) * CB * 2 + e % CB * 16, make_uint4(0, 0, 0, 0));
+    // (WMN: in each of the two pieces of CB columns)
+    constexpr int PC = WMN ? CB : MB;
+    for (int e = tid; e < a.wbuf * MB; e += LE_THREADS)
+      st_shared16(sw + e / MB * w_bytes + e % MB / PC * (PC * a.Rp * 2) + uint32_t(a.R) * PC * 2 +
+                      e % PC * 16,
+                  make_uint4(0, 0, 0, 0));
     fence_proxy_async_smem();
   }
   tc_fence_before();
@@ -831,10 +836,10 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
   const int per_tile = (a.ncb + a.cpu - 1) / a.cpu, rg = a.Rp >> 3;
   const int64_t items = int64_t(a.plan.head[0]) * per_tile;
   bool ok = true;
-  int blk = 0, live = 0;          // column blocks (warps 4 and 5: of live tiles), live items so far
+  int blk = 0, live = 0;          // column blocks (warps 4, 5: MMA blocks of live tiles), live items
   if (warp < 4) {
     // -------------------------------------------------------------- base, 32 rows a warp
-    if (a.vec && a.base) {
+    if (VEC && a.base) {
       for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
         const int4 tl = a.plan.tiles[item / per_tile];
         const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
@@ -867,9 +872,9 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
     }
   } else if (warp == 4) {
     // -------------------------------------------------------------- MMA issuer
-    const uint32_t id = idesc_lora(CB, 0, WMN ? 1 : 0);
+    const uint32_t id = idesc_lora(MB, 0, WMN ? 1 : 0);
     const LoraPieces pc(WMN ? CB : a.pw);
-    const LoraSteps steps = WMN ? LoraSteps::mn(pc) : LoraSteps::k(pc, CB);
+    const LoraSteps steps = WMN ? LoraSteps::mn(pc) : LoraSteps::k(pc, MB);
     for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
       if (a.plan.tiles[item / per_tile].x >= a.n) continue;
       const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
@@ -877,7 +882,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
       if (!(ok = warp_wait(&a_full[ab], uint32_t(live / a.abuf) & 1u))) break;
       ++live;
       const uint64_t da = sdesc(sa + ab * a_bytes, 2048, 128, 0);
-      for (int cb = cb0; cb < cb1; ++cb, ++blk) {
+      for (int cb = cb0; cb < cb1; cb += 2, ++blk) {
         const int b = blk % LE_BUF, wb = blk % a.wbuf;
         if (!warp_wait(&acc_empty[b], (uint32_t(blk / LE_BUF) & 1u) ^ 1u) ||
             !warp_wait(&w_full[wb], uint32_t(blk / a.wbuf) & 1u)) {
@@ -886,16 +891,16 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
         }
         tc_fence_after();
         const uint32_t bw = sw + wb * w_bytes;
-        const uint64_t db = WMN ? pc.desc_mn(bw, a.Rp) : pc.desc_k(bw, CB);
+        const uint64_t db = WMN ? pc.desc_mn(bw, a.Rp) : pc.desc_k(bw, MB);
         switch (a.Rp) {
-          case 16: lora_issue<NS, 1>(tmem + b * CB, da, db, id, steps, rg); break;
-          case 32: lora_issue<NS, 2>(tmem + b * CB, da, db, id, steps, rg); break;
-          case 64: lora_issue<NS, 4>(tmem + b * CB, da, db, id, steps, rg); break;
-          case 128: lora_issue<NS, 8>(tmem + b * CB, da, db, id, steps, rg); break;
+          case 16: lora_issue<NS, 1>(tmem + b * MB, da, db, id, steps, rg); break;
+          case 32: lora_issue<NS, 2>(tmem + b * MB, da, db, id, steps, rg); break;
+          case 64: lora_issue<NS, 4>(tmem + b * MB, da, db, id, steps, rg); break;
+          case 128: lora_issue<NS, 8>(tmem + b * MB, da, db, id, steps, rg); break;
           default:
             for (int i = NS - 1; i >= 0; --i)
               for (int k = 0; k < a.Rp / 16; ++k)
-                tc_mma_bf16_el(tmem + b * CB, da + uint64_t(uint32_t(i * rg + 2 * k) * 128),
+                tc_mma_bf16_el(tmem + b * MB, da + uint64_t(uint32_t(i * rg + 2 * k) * 128),
                                db + uint64_t(steps.at(k) >> 4), id, (i < NS - 1 || k) ? 1u : 0u);
         }
         tc_commit_el(&w_empty[wb]);
@@ -920,17 +925,18 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
 #pragma unroll
       for (int i = 0; i < NS; ++i)
         tma_load_3d_el(sa + ab * a_bytes + i * a.Rp * 256, &maps.parts, &a_full[ab], 0, tl.w, i * rg);
-      for (int cb = cb0; cb < cb1; ++cb, ++blk) {
+      for (int cb = cb0; cb < cb1; cb += 2, ++blk) {
         const int b = blk % a.wbuf;
         if (!(ok = warp_wait(&w_empty[b], (uint32_t(blk / a.wbuf) & 1u) ^ 1u))) break;
         const uint32_t dw = sw + b * w_bytes;
-        if (lane == 0) mbar_arrive_expect_tx(&w_full[b], uint32_t(CB) * a.R * 2);
+        if (lane == 0) mbar_arrive_expect_tx(&w_full[b], uint32_t(MB) * a.R * 2);
         __syncwarp();
         if constexpr (WMN) {
           tma_load_3d_el(dw, &maps.w, &w_full[b], cb * CB, 0, tl.x);
+          tma_load_3d_el(dw + CB * a.Rp * 2, &maps.w, &w_full[b], cb * CB + CB, 0, tl.x);
         } else {
           for (int r = 0; r < a.R; r += a.pw)
-            tma_load_3d_el(dw + uint32_t(r) * CB * 2, &maps.w, &w_full[b], r, cb * CB, tl.x);
+            tma_load_3d_el(dw + uint32_t(r) * MB * 2, &maps.w, &w_full[b], r, cb * CB, tl.x);
         }
       }
     }
@@ -946,17 +952,19 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
     const int grp = (warp - 6) >> 2, q4 = warp & 3;      // TMEM lanes 32 q4 .. + 31
     const int row = 32 * q4 + lane;                      // this thread's row of the tile
     float *tp = reinterpret_cast<float *>(smem) + (warp - 6) * 32 * LE_EPI_LD;
-    int all = 0, prev = -1;                              // blocks so far; the tile last stored
+    int all = 0, turn = 0, prev = -1;                    // blocks so far; the tile last stored
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
       const int4 tl = a.plan.tiles[item / per_tile];
       const bool has = tl.x < a.n;
       const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
       const int tok = row < tl.z ? a.plan.perm[tl.y + row] : -1;
-      for (int cb = cb0; cb < cb1; ++cb, ++all, blk += has ? 1 : 0) {
-        if (all % LE_GROUPS != grp) continue;
-        const int b = blk % LE_BUF, s = all % a.ring;
-        const uint32_t tacc = tmem + (uint32_t(32 * q4) << 16) + b * CB;
-        if (a.vec) {
+      for (int cb = cb0; cb < cb1; ++cb, ++all, turn = turn == LE_GROUPS - 1 ? 0 : turn + 1) {
+        if (turn != grp) continue;
+        const int mb = blk + ((cb - cb0) >> 1), b = mb % LE_BUF, s = all % a.ring;
+        const uint32_t tacc = tmem + (uint32_t(32 * q4) << 16) + b * MB + ((cb - cb0) & 1) * CB;
+        // the accumulator is free when both its halves have been read; a missing half counts too
+        const bool lone = cb == cb1 - 1 && ((cb - cb0) & 1) == 0;
+        if constexpr (VEC) {
           // the tile of this warp's last turn has been read: the fetch may refill it
           if (prev >= 0) {
             bulk_wait_read_el();
@@ -966,10 +974,10 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
           // a warp whose wait ran out goes on without waiting
           if (base && ok) ok = warp_wait(&b_full[s], uint32_t(all / a.ring) & 1u);
         }
-        OT odd[CB / 32][32];                               // !vec: base, a row a register
-        if (!a.vec && base) {
+        OT odd[VEC ? 1 : CB / 32][32];                     // base, a row a register
+        if (!VEC && base) {
 #pragma unroll
-          for (int h = 0; h < CB / 32; ++h)
+          for (int h = 0; h < (VEC ? 1 : CB / 32); ++h)
 #pragma unroll
             for (int r = 0; r < 32; ++r) {
               const int tk = __shfl_sync(0xffffffffu, tok, r);
@@ -978,10 +986,10 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
             }
         }
         if (has) {
-          if (ok) ok = warp_wait(&acc_full[b], uint32_t(blk / LE_BUF) & 1u);
+          if (ok) ok = warp_wait(&acc_full[b], uint32_t(mb / LE_BUF) & 1u);
           tc_fence_after();
         }
-        if (a.vec) {
+        if constexpr (VEC) {
           uint8_t *trow = smem + s * LE_TILE_BYTES + row * 128;
 #pragma unroll
           for (int h = 0; h < CB; h += 32) {
@@ -1025,7 +1033,10 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
           if (has) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[b]);
+            if (lane == 0) {
+              mbar_arrive(&acc_empty[b]);
+              if (lone) mbar_arrive(&acc_empty[b]);
+            }
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -1078,7 +1089,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
             for (int r = 0; r < 32; ++r) {
               const int tk = __shfl_sync(0xffffffffu, tok, r);
               float f = has ? tp[r * LE_EPI_LD + lane] : 0.0f;
-              if (base) f += float(odd[h / 32][r]);
+              if (base) f += float(odd[VEC ? 0 : h / 32][r]);
               if (tk >= 0 && c < a.N) y[int64_t(tk) * a.N + c] = OT(f);
             }
             __syncwarp();
@@ -1086,10 +1097,14 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
           if (has) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[b]);
+            if (lane == 0) {
+              mbar_arrive(&acc_empty[b]);
+              if (lone) mbar_arrive(&acc_empty[b]);
+            }
           }
         }
       }
+      if (has) blk += (cb1 - cb0 + 1) >> 1;
     }
     bulk_wait_el();
   }
@@ -1097,7 +1112,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
   __syncthreads();
   if (warp == 4) {
     tc_fence_after();
-    tmem_dealloc(tmem, LE_BUF * CB);
+    tmem_dealloc(tmem, LE_BUF * MB);
   }
 }
 
