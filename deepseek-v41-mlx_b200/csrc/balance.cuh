@@ -80,8 +80,7 @@ __device__ __forceinline__ float rsqrt_approx(float x) {
 
 // sqrt(softplus(z)) and its derivative sigmoid(z) / (2 s).  softplus = max(z, 0) + log1p(u), u =
 // e^-|z| in (0, 1], with log1p(u) / u by a Chebyshev interpolant of degree 8 (relative error
-// 2e-7): the library's log1pf, sqrtf and divisions would bound the pass by issue slots (448 us
-// at T = 65536, E = 384 in the one-thread-a-value form against 31 us of HBM time).
+// 2e-7): the library's log1pf, sqrtf and divisions would bound the pass by issue slots.
 __device__ __forceinline__ void score_sqrtsoftplus(float z, float &s, float &ds) {
   const float u = exp_acc(-fabsf(z));
   float p = 5.126101896e-3f;
@@ -102,6 +101,33 @@ __device__ __forceinline__ void score_sqrtsoftplus(float z, float &s, float &ds)
     ds = 0.5f * s;
   }
 }
+// The same for two values at once, |z| <= 16 where z < 0: packed fp32 pairs halve the polynomial,
+// and the exponential needs no correction there (its argument's rounding costs |z| half steps).
+// temp_l2e = -log2(e) / temp.  (At T 65536, E 384 with routing weights: 107 us with the scalar
+// form above, bound by issue slots.)
+__device__ __forceinline__ void score2_sqrtsoftplus(float z0, float z1, float inv_temp,
+                                                    float temp_l2e, uint64_t &s, uint64_t &ds) {
+  float u0, u1;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(u0) : "f"(fabsf(z0) * temp_l2e));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(u1) : "f"(fabsf(z1) * temp_l2e));
+  const uint64_t u = f32x2(u0, u1);
+  uint64_t p = f32x2(5.126101896e-3f, 5.126101896e-3f);
+  p = f32x2_fma(p, u, f32x2(-2.907406539e-2f, -2.907406539e-2f));
+  p = f32x2_fma(p, u, f32x2(7.751608640e-2f, 7.751608640e-2f));
+  p = f32x2_fma(p, u, f32x2(-1.360224783e-1f, -1.360224783e-1f));
+  p = f32x2_fma(p, u, f32x2(1.907688081e-1f, 1.907688081e-1f));
+  p = f32x2_fma(p, u, f32x2(-2.483539879e-1f, -2.483539879e-1f));
+  p = f32x2_fma(p, u, f32x2(3.331812024e-1f, 3.331812024e-1f));
+  p = f32x2_fma(p, u, f32x2(-4.999944568e-1f, -4.999944568e-1f));
+  p = f32x2_fma(p, u, f32x2(9.999999404e-1f, 9.999999404e-1f));
+  const uint64_t m = f32x2_mul(f32x2(fmaxf(z0, 0.0f), fmaxf(z1, 0.0f)), f32x2(inv_temp, inv_temp));
+  const uint64_t sp = f32x2_fma(p, u, m), w = f32x2_add(u, f32x2(1.0f, 1.0f));
+  const uint64_t r = f32x2(rsqrt_approx(f32x2_lo(sp)), rsqrt_approx(f32x2_hi(sp)));
+  const uint64_t d = f32x2(rcp_approx(f32x2_lo(w)), rcp_approx(f32x2_hi(w)));
+  s = f32x2_mul(sp, r);
+  const uint64_t h = f32x2_mul(r, f32x2(z0 < 0.0f ? 0.5f * u0 : 0.5f, z1 < 0.0f ? 0.5f * u1 : 0.5f));
+  ds = f32x2_mul(h, d);
+}
 // 1 - s from the same exponential: s (1 - s) = u / (1 + u)^2 keeps its digits at both ends.
 __device__ __forceinline__ void score_sigmoid(float z, float &s, float &ds) {
   const float u = exp_acc(-fabsf(z)), d = rcp_approx(1.0f + u);
@@ -109,10 +135,21 @@ __device__ __forceinline__ void score_sigmoid(float z, float &s, float &ds) {
   ds = u * d * d;
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// The warp's sums of four values in 10 shuffles: half the values change lanes with half the
+// partners, then each quarter of the warp finishes one.
+__device__ __forceinline__ void warp_sum4(float &a, float &b, float &c, float &d) {
+  const int lane = threadIdx.x & 31;
+  const bool h = lane & 16, q = lane & 8;
+  const float x = (h ? c : a) + __shfl_xor_sync(0xffffffffu, h ? a : c, 16);
+  const float y = (h ? d : b) + __shfl_xor_sync(0xffffffffu, h ? b : d, 16);
+  float v = (q ? y : x) + __shfl_xor_sync(0xffffffffu, q ? x : y, 8);
+  v += __shfl_xor_sync(0xffffffffu, v, 4);
+  v += __shfl_xor_sync(0xffffffffu, v, 2);
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  a = __shfl_sync(0xffffffffu, v, 0);
+  b = __shfl_sync(0xffffffffu, v, 8);
+  c = __shfl_sync(0xffffffffu, v, 16);
+  d = __shfl_sync(0xffffffffu, v, 24);
 }
 
 __device__ __forceinline__ float bal_ld(const float *p) { return __ldg(p); }
@@ -120,220 +157,291 @@ __device__ __forceinline__ float bal_ld(const __nv_bfloat16 *p) {
   return bf_bits2f(__ldg(reinterpret_cast<const uint16_t *>(p)));
 }
 
-// A row's values as lane l holds them: VEC = 4: elements 4 (32 j + l) + v (E % 4 == 0, aligned
-// rows); VEC = 1: elements 32 j + l.
-template <typename IT, int NV, int VEC> struct BalRow;
-template <int NV> struct BalRow<float, NV, 4> {
-  float4 r[NV];
+// A row's values as lane l holds them, in NP pairs: VEC = 4 (E % 4 == 0, aligned rows): pairs 2 j
+// and 2 j + 1 are elements 4 (32 j + l) .. + 3; VEC = 1: pair j is elements 64 j + l and + 32.
+template <typename IT, int NP, int VEC> struct BalRow;
+template <int NP> struct BalRow<float, NP, 4> {
+  float4 r[NP / 2];
   __device__ __forceinline__ void load(const float *row, int E, int lane) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NP / 2; ++j)
       if (4 * (32 * j + lane) < E) r[j] = __ldg(reinterpret_cast<const float4 *>(row) + 32 * j + lane);
   }
-  __device__ __forceinline__ float at(int j, int v) const { return (&r[j].x)[v]; }
+  __device__ __forceinline__ float at(int p, int h) const { return (&r[p >> 1].x)[2 * (p & 1) + h]; }
 };
-template <int NV> struct BalRow<__nv_bfloat16, NV, 4> {
-  uint2 r[NV];
+template <int NP> struct BalRow<__nv_bfloat16, NP, 4> {
+  uint2 r[NP / 2];
   __device__ __forceinline__ void load(const __nv_bfloat16 *row, int E, int lane) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NP / 2; ++j)
       if (4 * (32 * j + lane) < E) r[j] = __ldg(reinterpret_cast<const uint2 *>(row) + 32 * j + lane);
   }
-  __device__ __forceinline__ float at(int j, int v) const {
-    const uint32_t w = v < 2 ? r[j].x : r[j].y;
-    return bf_bits2f(uint16_t(v & 1 ? w >> 16 : w));
+  __device__ __forceinline__ float at(int p, int h) const {
+    const uint32_t w = p & 1 ? r[p >> 1].y : r[p >> 1].x;
+    return __uint_as_float(h ? w & 0xFFFF0000u : w << 16);
   }
 };
-template <typename IT, int NV> struct BalRow<IT, NV, 1> {
-  float r[NV];
+template <typename IT, int NP> struct BalRow<IT, NP, 1> {
+  float r[2 * NP];
   __device__ __forceinline__ void load(const IT *row, int E, int lane) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (32 * j + lane < E) r[j] = bal_ld(row + 32 * j + lane);
+    for (int j = 0; j < 2 * NP; ++j) r[j] = 32 * j + lane < E ? bal_ld(row + 32 * j + lane) : 0.0f;
   }
-  __device__ __forceinline__ float at(int j, int) const { return r[j]; }
+  __device__ __forceinline__ float at(int p, int h) const { return r[2 * p + h]; }
 };
-
-template <typename IT, int VEC>
-__device__ __forceinline__ void bal_store(IT *row, int j, int lane, const float *v) {
+// Element h of pair p of lane l, and whether the row has it (VEC = 4: both or neither).
+template <int VEC> __device__ __forceinline__ int bal_elem(int p, int h, int lane) {
+  return VEC == 4 ? 4 * (32 * (p >> 1) + lane) + 2 * (p & 1) + h : 64 * p + 32 * h + lane;
+}
+// Pairs 2 j and 2 j + 1 (VEC = 4) or pair p (VEC = 1) of a row
+template <typename IT, int NP, int VEC>
+__device__ __forceinline__ void bal_store(IT *row, int E, int lane, const uint64_t (&v)[NP]) {
   if constexpr (VEC == 1) {
-    row[32 * j + lane] = IT(v[0]);
-  } else if constexpr (sizeof(IT) == 4) {
-    reinterpret_cast<float4 *>(row)[32 * j + lane] = make_float4(v[0], v[1], v[2], v[3]);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      if (bal_elem<1>(p, 0, lane) < E) row[bal_elem<1>(p, 0, lane)] = IT(f32x2_lo(v[p]));
+      if (bal_elem<1>(p, 1, lane) < E) row[bal_elem<1>(p, 1, lane)] = IT(f32x2_hi(v[p]));
+    }
   } else {
-    reinterpret_cast<uint2 *>(row)[32 * j + lane] =
-        make_uint2(uint32_t(f2bf_bits(v[0])) | (uint32_t(f2bf_bits(v[1])) << 16),
-                   uint32_t(f2bf_bits(v[2])) | (uint32_t(f2bf_bits(v[3])) << 16));
+#pragma unroll
+    for (int j = 0; j < NP / 2; ++j)
+      if (4 * (32 * j + lane) < E) {
+        const uint64_t a = v[2 * j], b = v[2 * j + 1];
+        if constexpr (sizeof(IT) == 4) {
+          reinterpret_cast<float4 *>(row)[32 * j + lane] =
+              make_float4(f32x2_lo(a), f32x2_hi(a), f32x2_lo(b), f32x2_hi(b));
+        } else {
+          const __nv_bfloat162 x = __floats2bfloat162_rn(f32x2_lo(a), f32x2_hi(a));
+          const __nv_bfloat162 y = __floats2bfloat162_rn(f32x2_lo(b), f32x2_hi(b));
+          reinterpret_cast<uint2 *>(row)[32 * j + lane] = make_uint2(
+              *reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
+        }
+      }
   }
 }
 
 // A warp's tokens [t0, t1), in order.  cnt / live: the sequences' counters (global or shared
-// memory).  add: this warp's row of E floats in shared memory, zero between tokens (the routing
-// weights' gradients on their way to the lanes that own the experts).  done(t, q, dot) takes
-// c . p of token t; it is also called with 0 at the first token of each sequence.
-template <typename IT, int NV, int VEC, bool GRAD, typename Done>
+// memory), ready after `ready()`.  add: this warp's row of E floats in shared memory, zero between
+// tokens (the routing weights' gradients on their way to the lanes that own the experts).
+// done(t, q, dot) takes c . p of token t; it is also called with 0 at the first token of each
+// sequence.  The next token's row, choices and weights' gradients are requested a token ahead.
+// NP pairs a lane; FUNC: the score function.
+template <typename IT, int NP, int VEC, bool GRAD, int FUNC, typename Ready, typename Done>
 __device__ __forceinline__ void balance_tokens(const BalArgs &p, int64_t t0, int64_t t1,
                                                const int *cnt, const int *live, float *add,
-                                               Done &&done) {
+                                               Ready &&ready, Done &&done) {
   const int lane = threadIdx.x & 31;
   const int E = p.E, k = p.topk;
-  const IT *logits = static_cast<const IT *>(p.logits);
-  IT *dl = static_cast<IT *>(p.dlogits);
+  const IT *z = static_cast<const IT *>(p.logits) + t0 * E;     // this token's row, choices, ...
+  IT *dl = static_cast<IT *>(p.dlogits) + t0 * E;
+  const int32_t *ip = p.indices + t0 * k;
+  const float *wp = p.dweights + (p.dweights ? t0 * k : 0);
+  const uint8_t *mp = p.mask + (p.mask ? t0 : 0);
+  const bool routed = GRAD && p.dweights, nrm = p.norm && k > 1, wide = k > 32;
+  const float temp_l2e = -1.44269504f * p.inv_temp;
   BalSeq sq{-1, 0, t0};
-  float c[NV][VEC], coef = 0.0f;
-  BalRow<IT, NV, VEC> nx;
-  if (t0 < t1 && !(p.mask && !p.mask[t0])) nx.load(logits + t0 * E, E, lane);
-  for (int64_t t = t0; t < t1; ++t) {
-    BalRow<IT, NV, VEC> row = nx;
-    if (t + 1 < t1 && !(p.mask && !p.mask[t + 1])) nx.load(logits + (t + 1) * E, E, lane);
+  uint64_t c[NP];
+  float coef = 0.0f;
+  BalRow<IT, NP, VEC> nx;
+  int idx_n[2] = {-1, -1};
+  float dw_n[2] = {0.f, 0.f};
+  bool on_n = false;
+  auto fetch = [&](const IT *zr, const int32_t *ir, const float *wr, const uint8_t *mr) {
+    on_n = !p.mask || *mr;
+    if (!on_n) return;
+    nx.load(zr, E, lane);
+    if (routed) {
+      if (lane < k) {
+        idx_n[0] = __ldg(ir + lane);
+        dw_n[0] = __ldg(wr + lane);
+      }
+      if (wide && lane + 32 < k) {
+        idx_n[1] = __ldg(ir + lane + 32);
+        dw_n[1] = __ldg(wr + lane + 32);
+      }
+    }
+  };
+  if (t0 < t1) fetch(z, ip, wp, mp);
+  ready();
+#pragma unroll 1
+  for (int64_t t = t0; t < t1; ++t, z += E, dl += E) {
+    const BalRow<IT, NP, VEC> row = nx;
+    int idx[2] = {idx_n[0], idx_n[1]};
+    float dw[2] = {dw_n[0], dw_n[1]};
+    const bool on = on_n;
+    ip += k;
+    wp += k;
+    ++mp;
+    if (t + 1 < t1) fetch(z + E, ip, wp, mp);
     if (t >= sq.b) {
       sq = balance_seq(p, t);
       if (sq.q >= 0) {
         done(t, sq.q, 0.0f);
         const float m = float(live[sq.q]);
         coef = (GRAD && p.grad_loss ? p.grad_loss[sq.q] : 0.0f) * (float(E) / (float(k) * m * m));
+        const int *cq = cnt + int64_t(sq.q) * E;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            const int e = VEC * (32 * j + lane) + v;
-            c[j][v] = e < E ? float(cnt[int64_t(sq.q) * E + e]) : 0.0f;
-          }
+        for (int i = 0; i < NP; ++i) {
+          const int e0 = bal_elem<VEC>(i, 0, lane), e1 = bal_elem<VEC>(i, 1, lane);
+          c[i] = f32x2(e0 < E ? float(cq[e0]) : 0.0f, e1 < E ? float(cq[e1]) : 0.0f);
+        }
       }
     }
-    if (sq.q < 0 || (p.mask && !p.mask[t])) {
+    if (sq.q < 0 || !on) {
       if constexpr (GRAD) {
-        const float z4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-          if (VEC * (32 * j + lane) < E) bal_store<IT, VEC>(dl + t * E, j, lane, z4);
+        const uint64_t zero[NP] = {};
+        bal_store<IT, NP, VEC>(dl, E, lane, zero);
       }
       continue;
     }
     // the chosen experts' logits, read again while the row is in the cache
-    int idx[2] = {-1, -1};
-    float dw[2] = {0.f, 0.f}, zs[2] = {0.f, 0.f};
-    const bool routed = GRAD && p.dweights;
+    float zs[2] = {0.f, 0.f};
     if (routed) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (lane + 32 * u < k) {
-          const int i = p.indices[t * k + lane + 32 * u];
-          if (i >= 0 && i < E) {
-            idx[u] = i;
-            dw[u] = p.dweights[t * k + lane + 32 * u];
-            zs[u] = bal_ld(logits + t * E + i) * p.inv_temp;
-          }
+      if (lane >= k || idx[0] < 0 || idx[0] >= E) {
+        idx[0] = -1;
+        dw[0] = 0.0f;
+      } else {
+        zs[0] = bal_ld(z + idx[0]) * p.inv_temp;
+      }
+      if (wide) {
+        if (lane + 32 >= k || idx[1] < 0 || idx[1] >= E) {
+          idx[1] = -1;
+          dw[1] = 0.0f;
+        } else {
+          zs[1] = bal_ld(z + idx[1]) * p.inv_temp;
         }
+      }
     }
-    float s[NV][VEC], d[NV][VEC];                    // scores and their derivatives
-    float sum = 0.0f, cs = 0.0f, mx = 0.0f, rs = 0.0f;
-    if (p.func == DSV41_SCORE_SOFTMAX) {
+    uint64_t s[NP], d[NP];                           // scores and their derivatives
+    float mx = 0.0f;
+    if constexpr (FUNC == DSV41_SCORE_SOFTMAX) {
       mx = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (VEC * (32 * j + lane) < E)
+      for (int i = 0; i < NP; ++i)
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) mx = fmaxf(mx, row.at(j, v));
+        for (int h = 0; h < 2; ++h)
+          if (bal_elem<VEC>(i, h, lane) < E) mx = fmaxf(mx, row.at(i, h));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       mx *= p.inv_temp;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int i = 0; i < NP; ++i) {
+        float e[2];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const bool in = VEC * (32 * j + lane) < E && mx > -INFINITY;
-          s[j][v] = in ? exp_acc(row.at(j, v) * p.inv_temp - mx) : 0.0f;
-          sum += s[j][v];
-        }
-      sum = warp_sum(sum);
-      rs = mx > -INFINITY ? __fdividef(1.0f, sum) : 0.0f;
-      sum = 0.0f;
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) s[j][v] *= rs;
-    } else if (p.func == DSV41_SCORE_SIGMOID) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          s[j][v] = d[j][v] = 0.0f;
-          if (VEC * (32 * j + lane) < E) score_sigmoid(row.at(j, v) * p.inv_temp, s[j][v], d[j][v]);
-        }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          s[j][v] = d[j][v] = 0.0f;
-          if (VEC * (32 * j + lane) < E)
-            score_sqrtsoftplus(row.at(j, v) * p.inv_temp, s[j][v], d[j][v]);
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        sum += s[j][v];
-        cs = fmaf(c[j][v], s[j][v], cs);
+        for (int h = 0; h < 2; ++h)
+          e[h] = bal_elem<VEC>(i, h, lane) < E && mx > -INFINITY ? exp_acc(row.at(i, h) * p.inv_temp - mx)
+                                                                 : 0.0f;
+        s[i] = d[i] = f32x2(e[0], e[1]);
       }
-    sum = warp_sum(sum);
-    cs = warp_sum(cs);
-    const float rz = __fdividef(1.0f, sum + 1e-20f), dot = cs * rz;
+    } else {
+      bool fast = false;
+      if constexpr (FUNC == DSV41_SCORE_SQRTSOFTPLUS && VEC == 4) {
+        float mn = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+          if (bal_elem<VEC>(i, 0, lane) < E) mn = fminf(mn, fminf(row.at(i, 0), row.at(i, 1)));
+        fast = !__any_sync(0xffffffffu, mn * p.inv_temp < -16.0f);
+        if (fast) {
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            s[i] = d[i] = 0;
+            if (bal_elem<VEC>(i, 0, lane) < E)
+              score2_sqrtsoftplus(row.at(i, 0), row.at(i, 1), p.inv_temp, temp_l2e, s[i], d[i]);
+          }
+        }
+      }
+      if (!fast) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          float e[2] = {0.f, 0.f}, f[2] = {0.f, 0.f};
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (bal_elem<VEC>(i, h, lane) < E) {
+              if (FUNC == DSV41_SCORE_SIGMOID) score_sigmoid(row.at(i, h) * p.inv_temp, e[h], f[h]);
+              else score_sqrtsoftplus(row.at(i, h) * p.inv_temp, e[h], f[h]);
+            }
+          s[i] = f32x2(e[0], e[1]);
+          d[i] = f32x2(f[0], f[1]);
+        }
+      }
+    }
+    uint64_t sum2 = s[0], cs2 = f32x2_mul(c[0], s[0]);
+#pragma unroll
+    for (int i = 1; i < NP; ++i) {
+      sum2 = f32x2_add(sum2, s[i]);
+      cs2 = f32x2_fma(c[i], s[i], cs2);
+    }
+    float sum = f32x2_lo(sum2) + f32x2_hi(sum2), cs = f32x2_lo(cs2) + f32x2_hi(cs2);
+    // the sums over the row, and those of the routing weights with them
+    float ss[2] = {0.f, 0.f}, dd[2] = {0.f, 0.f}, sel = 0.0f, dws = 0.0f;
+    if (routed) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (u && !wide) break;
+        if (idx[u] >= 0) {
+          if (FUNC == DSV41_SCORE_SOFTMAX) ss[u] = dd[u] = mx > -INFINITY ? exp_acc(zs[u] - mx) : 0.0f;
+          else if (FUNC == DSV41_SCORE_SIGMOID) score_sigmoid(zs[u], ss[u], dd[u]);
+          else score_sqrtsoftplus(zs[u], ss[u], dd[u]);
+        }
+        sel += ss[u];
+        dws = fmaf(dw[u], ss[u], dws);
+      }
+    }
+    warp_sum4(sum, cs, sel, dws);
+    float rs = 1.0f, rz;                             // 1 / sum of the exponentials, of the scores
+    if constexpr (FUNC == DSV41_SCORE_SOFTMAX) {
+      // s, d, ss, dd still lack the factor rs (a row of -inf: zeros; NaN stays NaN)
+      rs = mx > -INFINITY ? __fdividef(1.0f, sum) : (mx == -INFINITY ? 0.0f : mx);
+      rz = 1.0f;
+      cs *= rs;
+      sel *= rs;
+      dws *= rs;
+    } else {
+      rz = __fdividef(1.0f, sum + 1e-20f);
+    }
+    const float dot = cs * rz;
     done(t, sq.q, dot);
     if constexpr (GRAD) {
-      const float ca = coef * rz;
-      float R = 0.0f;
+      float R = 0.0f;                                // softmax: sum of the weights' ds times s
       if (routed) {
-        float ss[2], dd[2], sel = 0.0f, dws = 0.0f;
+        const float rsel = nrm ? __fdividef(1.0f, sel + 1e-20f) : 1.0f;
+        const float mean = nrm ? dws * rsel : 0.0f, sc = p.route_scale * rsel;
+        R = sc * (dws - mean * sel);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          ss[u] = dd[u] = 0.0f;
-          if (idx[u] >= 0) {
-            if (p.func == DSV41_SCORE_SOFTMAX) ss[u] = dd[u] = mx > -INFINITY ? exp_acc(zs[u] - mx) * rs : 0.0f;
-            else if (p.func == DSV41_SCORE_SIGMOID) score_sigmoid(zs[u], ss[u], dd[u]);
-            else score_sqrtsoftplus(zs[u], ss[u], dd[u]);
-          }
-          sel += ss[u];
-          dws = fmaf(dw[u], ss[u], dws);
-        }
-        const bool nrm = p.norm && k > 1;
-        float rsel = 1.0f, mean = 0.0f;
-        if (nrm) {
-          rsel = __fdividef(1.0f, warp_sum(sel) + 1e-20f);
-          mean = warp_sum(dws) * rsel;
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (u && k <= 32) break;
-          const float g = p.route_scale * (dw[u] - mean) * rsel;
-          R += idx[u] >= 0 ? g * ss[u] : 0.0f;
+          if (u && !wide) break;
+          const float g = sc * (dw[u] - mean) * (dd[u] * rs) * p.inv_temp;
           // the same expert twice: one after another, in lane order
           const unsigned same = __match_any_sync(0xffffffffu, idx[u] >= 0 ? idx[u] : -1 - lane);
           const int turn = __popc(same & ((1u << lane) - 1));
-          for (int o = 0; __any_sync(0xffffffffu, turn >= o); ++o) {
-            if (turn == o && idx[u] >= 0) add[idx[u]] += g * dd[u] * p.inv_temp;
+          if (turn == 0 && idx[u] >= 0) add[idx[u]] += g;
+          __syncwarp();
+          for (int o = 1; __any_sync(0xffffffffu, turn >= o); ++o) {
+            if (turn == o && idx[u] >= 0) add[idx[u]] += g;
             __syncwarp();
           }
         }
-        if (p.func == DSV41_SCORE_SOFTMAX) R = warp_sum(R);
       }
+      // d loss / d s = ca (c - dot); times the derivative (softmax: s (ds - sum ds s), whose loss
+      // part has no sum: sum_e p_e (c_e - dot) = 0)
+      const float ca = coef * rz * p.inv_temp * rs;
+      const float cb = -dot * ca - (FUNC == DSV41_SCORE_SOFTMAX ? R * p.inv_temp * rs : 0.0f);
+      uint64_t o[NP];
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (VEC * (32 * j + lane) < E) {
-          float o[VEC];
+      for (int i = 0; i < NP; ++i)
+        o[i] = f32x2_mul(f32x2_fma(c[i], f32x2(ca, ca), f32x2(cb, cb)), d[i]);
+      if (routed) {
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            const float g = ca * (c[j][v] - dot);
-            o[v] = (p.func == DSV41_SCORE_SOFTMAX ? s[j][v] * (g - R) : g * d[j][v]) * p.inv_temp;
+        for (int i = 0; i < NP; ++i) {
+          const int e0 = bal_elem<VEC>(i, 0, lane), e1 = bal_elem<VEC>(i, 1, lane);
+          if constexpr (VEC == 4) {
+            if (e0 < E) o[i] = f32x2_add(o[i], *reinterpret_cast<const uint64_t *>(add + e0));
+          } else {
+            o[i] = f32x2_add(o[i], f32x2(e0 < E ? add[e0] : 0.0f, e1 < E ? add[e1] : 0.0f));
           }
-          if (routed) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) o[v] += add[VEC * (32 * j + lane) + v];
-          }
-          bal_store<IT, VEC>(dl + t * E, j, lane, o);
         }
+      }
+      bal_store<IT, NP, VEC>(dl, E, lane, o);
       if (routed) {
         __syncwarp();
 #pragma unroll
@@ -346,8 +454,7 @@ __device__ __forceinline__ void balance_tokens(const BalArgs &p, int64_t t0, int
 }
 
 // ------------------------------------------------------------------ counts
-// This thread's choices of the tokens [t0, t1), counted into hist (shared, [S][E]) and live
-// (shared, [S]); rows strided over the block.
+// This block's choices of the tokens [t0, t1), counted into hist ([S][E]) and live ([S]).
 __device__ __forceinline__ void balance_count_shared(const BalArgs &p, int64_t t0, int64_t t1,
                                                      int *hist, int *live) {
   BalSeq sq{-1, 0, 0};
@@ -359,7 +466,7 @@ __device__ __forceinline__ void balance_count_shared(const BalArgs &p, int64_t t
     for (int j = 0; j < p.topk; ++j) {
       const int e = __ldg(p.indices + t * p.topk + j);
       if (e >= p.E) dev_flag(DSV41_DEVST_BAD_INDEX);
-      else if (e >= 0) atomicAdd(hist + sq.q * p.E + e, 1);
+      else if (e >= 0) atomicAdd(hist + int64_t(sq.q) * p.E + e, 1);
     }
   }
 }
@@ -368,6 +475,7 @@ __device__ __forceinline__ void balance_count_shared(const BalArgs &p, int64_t t
 // the counters over the cluster's shared memories: no counter has to be zeroed in memory first.
 __global__ void __launch_bounds__(1024, 1) k_balance_count(const BalArgs p) {
   extern __shared__ int bc_smem[];
+  pdl_trigger();
   int *hist = bc_smem, *live = bc_smem + p.S * p.E;
   const int C = gridDim.x, rank = blockIdx.x, n = p.S * p.E + p.S;
   for (int i = threadIdx.x; i < n; i += 1024) hist[i] = 0;
@@ -384,18 +492,34 @@ __global__ void __launch_bounds__(1024, 1) k_balance_count(const BalArgs p) {
   cluster_sync();
 }
 
-// More counters than a CTA's shared memory holds: straight to memory (zeroed before).
-__global__ void __launch_bounds__(256) k_balance_count_global(const BalArgs p) {
-  const int64_t t = blockIdx.x * (int64_t)256 + threadIdx.x;
-  if (t >= p.T || (p.mask && !p.mask[t])) return;
-  const BalSeq sq = balance_seq(p, t);
-  if (sq.q < 0) return;
-  atomicAdd(p.live + sq.q, 1);
-  for (int j = 0; j < p.topk; ++j) {
-    const int e = p.indices[t * p.topk + j];
-    if (e >= p.E) dev_flag(DSV41_DEVST_BAD_INDEX);
-    else if (e >= 0) atomicAdd(p.counts + int64_t(sq.q) * p.E + e, 1);
+// Many choices: every SM counts a slice of the tokens and adds what it counted to counters in
+// memory (zeroed by k_balance_zero).  Counted in shared memory first where all counters fit (straight
+// to memory took 45 us more at T 65536: a sequence's choices meet in a few cache lines).
+__global__ void __launch_bounds__(256) k_balance_zero(const BalArgs p) {
+  pdl_trigger();
+  const int64_t n = int64_t(p.S) * p.E, step = int64_t(gridDim.x) * 256;
+  for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < n; i += step) p.counts[i] = 0;
+  for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i <= p.S; i += step) p.live[i] = 0;
+}
+__global__ void __launch_bounds__(256) k_balance_count_wide(const BalArgs p, int shared) {
+  extern __shared__ int bc_smem[];
+  const int64_t t0 = p.T * blockIdx.x / gridDim.x, t1 = p.T * (blockIdx.x + 1) / gridDim.x;
+  const int n = shared ? p.S * p.E + p.S : 0;
+  int *hist = bc_smem, *live = bc_smem + p.S * p.E;
+  for (int i = threadIdx.x; i < n; i += 256) hist[i] = 0;
+  __syncthreads();
+  if (shared) {
+    balance_count_shared(p, t0, t1, hist, live);
+    __syncthreads();
   }
+  pdl_wait();                                       // the zeros
+  pdl_trigger();
+  if (!shared) {
+    balance_count_shared(p, t0, t1, p.counts, p.live);
+    return;
+  }
+  for (int i = threadIdx.x; i < n; i += 256)
+    if (hist[i]) atomicAdd(i < p.S * p.E ? p.counts + i : p.live + (i - p.S * p.E), hist[i]);
 }
 
 // ------------------------------------------------------------------ loss and gradient
@@ -407,12 +531,13 @@ __device__ __forceinline__ float balance_scale(const BalArgs &p, double sum, int
 // A run of tokens a warp, its row of the next token in flight while it works on one.  The sum
 // of a run's tokens of sequence q goes to part[run index + q]: runs and sequences both ascend
 // with the tokens, so no two share a place.  The last CTA adds each sequence's places in order.
-template <typename IT, int NV, int VEC, bool GRAD>
-__global__ void __launch_bounds__(32 * BL_WARPS) k_balance(const BalArgs p) {
-  extern __shared__ float bl_add[];                // [BL_WARPS][E], with routing weights
+template <typename IT, int NP, int VEC, bool GRAD, int FUNC>
+__global__ void __launch_bounds__(32 * BL_WARPS, NP <= 4 ? 3 : NP <= 8 ? 2 : 1)
+    k_balance(const BalArgs p) {
+  extern __shared__ __align__(16) float bl_add[];  // [BL_WARPS][E], with routing weights
   __shared__ int last_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float *add = bl_add + warp * p.E;
+  float *add = bl_add + warp * ((p.E + 3) & ~3);
   if (GRAD && p.dweights) {
     for (int e = lane; e < p.E; e += 32) add[e] = 0.0f;
     __syncwarp();
@@ -421,7 +546,7 @@ __global__ void __launch_bounds__(32 * BL_WARPS) k_balance(const BalArgs p) {
   const int64_t t0 = min(r * p.run, p.T), t1 = min(t0 + p.run, p.T);
   double sum = 0.0;
   int cur = -1;
-  balance_tokens<IT, NV, VEC, GRAD>(p, t0, t1, p.counts, p.live, add,
+  balance_tokens<IT, NP, VEC, GRAD, FUNC>(p, t0, t1, p.counts, p.live, add, [] { pdl_wait(); },
                                     [&](int64_t, int q, float dot) {
     if (q != cur) {
       if (cur >= 0 && lane == 0) p.part[r + cur] = sum;
@@ -453,15 +578,16 @@ __global__ void __launch_bounds__(32 * BL_WARPS) k_balance(const BalArgs p) {
 
 // The whole pass in one launch, for few tokens: one cluster whose CTAs each count all choices in
 // shared memory and take a share of the rows; the rows' c . p meet in rank 0's shared memory.
-template <typename IT, int NV, int VEC, bool GRAD>
+template <typename IT, int NP, int VEC, bool GRAD, int FUNC>
 __global__ void __launch_bounds__(32 * BL_WARPS) k_balance_small(const BalArgs p) {
-  extern __shared__ int bs_smem[];
+  extern __shared__ __align__(16) int bs_smem[];
   const int C = gridDim.x, rank = blockIdx.x, n = p.S * p.E;
-  int *hist = bs_smem, *live = hist + n;
-  float *dots = reinterpret_cast<float *>(live + p.S);         // [T], rank 0's is used
+  int *hist = bs_smem, *live = hist + ((n + 3) & ~3);
+  float *dots = reinterpret_cast<float *>(live + ((p.S + 3) & ~3));    // [T], rank 0's is used
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float *add = dots + p.T + warp * p.E;
-  for (int i = threadIdx.x; i < n + p.S; i += blockDim.x) hist[i] = 0;
+  float *add = dots + ((p.T + 3) & ~3) + warp * ((p.E + 3) & ~3);
+  for (int i = threadIdx.x; i < n; i += blockDim.x) hist[i] = 0;
+  for (int i = threadIdx.x; i < p.S; i += blockDim.x) live[i] = 0;
   for (int i = threadIdx.x; i < p.T; i += blockDim.x) dots[i] = 0.0f;
   if (GRAD && p.dweights)
     for (int e = lane; e < p.E; e += 32) add[e] = 0.0f;
@@ -471,7 +597,7 @@ __global__ void __launch_bounds__(32 * BL_WARPS) k_balance_small(const BalArgs p
   for (int i = rank * blockDim.x + threadIdx.x; i < n; i += C * blockDim.x) p.counts[i] = hist[i];
   const int64_t w = rank * BL_WARPS + warp, W = C * BL_WARPS;
   const uint32_t dots0 = mapa_rank(dots, 0);
-  balance_tokens<IT, NV, VEC, GRAD>(p, p.T * w / W, p.T * (w + 1) / W, hist, live, add,
+  balance_tokens<IT, NP, VEC, GRAD, FUNC>(p, p.T * w / W, p.T * (w + 1) / W, hist, live, add, [] {},
                                     [&](int64_t t, int, float dot) {
     if (lane == 0)
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dots0 + uint32_t(t) * 4), "f"(dot)

@@ -740,49 +740,62 @@ constexpr int64_t BL_SMALL_T = 512;
 bool balance_is_small(int64_t T, int64_t E, int64_t S) {
   return T > 0 && T <= BL_SMALL_T && S * E <= BL_SMALL_INTS;
 }
-// Tokens of a warp's run: two CTAs an SM share the tokens in one wave.
-int64_t balance_run(int64_t T) { return std::max<int64_t>(1, ceil_div(T, 2 * num_sms() * BL_WARPS)); }
+// Tokens of a warp's run: as many CTAs as run at once share the tokens.
+int64_t balance_run(int64_t T, int64_t E) {
+  const int64_t ctas = (E <= 256 ? 3 : E <= 512 ? 2 : 1) * int64_t(num_sms());
+  return std::max<int64_t>(1, ceil_div(T, ctas * BL_WARPS));
+}
+// Choices up to which one cluster counts them all (it needs no zeroed memory; beyond, its eight SMs'
+// shared-memory atomics take longer than a launch that zeroes and a count on every SM).
+constexpr int64_t BL_CLUSTER_CHOICES = 65536;
 
 struct BalShape {
   unsigned grid, cluster;      // cluster: 0 for the several-launch form
   size_t smem;
 };
 
-template <typename IT, int NV, int VEC, bool GRAD>
+template <typename IT, int NP, int VEC, bool GRAD, int FUNC>
 cudaError_t balance_go(const BalArgs &p, const BalShape &sh, cudaStream_t st) {
-  if (sh.cluster) {
-    cudaError_t e = max_dynamic_smem(k_balance_small<IT, NV, VEC, GRAD>, sh.smem);
-    if (e != cudaSuccess) return e;
-    return launch_cluster(false, k_balance_small<IT, NV, VEC, GRAD>, sh.grid, sh.cluster, 32 * BL_WARPS,
-                          sh.smem, st, p);
-  }
-  k_balance<IT, NV, VEC, GRAD><<<sh.grid, 32 * BL_WARPS, sh.smem, st>>>(p);
-  return cudaGetLastError();
+  return launch_pdl_if(true, k_balance<IT, NP, VEC, GRAD, FUNC>, dim3(sh.grid), dim3(32 * BL_WARPS),
+                       sh.smem, st, p);
 }
-template <typename IT, int NV, int VEC>
-cudaError_t balance_grad(const BalArgs &p, const BalShape &sh, cudaStream_t st) {
-  return p.dlogits ? balance_go<IT, NV, VEC, true>(p, sh, st) : balance_go<IT, NV, VEC, false>(p, sh, st);
+template <typename IT, int NP, int VEC, bool GRAD, int FUNC>
+cudaError_t balance_small_go(const BalArgs &p, const BalShape &sh, cudaStream_t st) {
+  const cudaError_t e = max_dynamic_smem(k_balance_small<IT, NP, VEC, GRAD, FUNC>, sh.smem);
+  if (e != cudaSuccess) return e;
+  return launch_cluster(false, k_balance_small<IT, NP, VEC, GRAD, FUNC>, sh.grid, sh.cluster,
+                        32 * BL_WARPS, sh.smem, st, p);
 }
-// Rows of E % 4 == 0 values move in pieces of four, others one by one.
-template <typename IT>
+// Rows of E % 4 == 0 values move in pieces of four, others one by one; a lane holds the next size
+// of 8, 12, 16 or 32 values.  Few tokens: the largest size for all (its empty pairs are skipped).
+template <typename IT, bool GRAD, int FUNC>
 cudaError_t balance_rows(const BalArgs &p, const BalShape &sh, cudaStream_t st) {
   const bool vec = p.E % 4 == 0 && aligned(p.logits, 4 * sizeof(IT)) && aligned(p.dlogits, 4 * sizeof(IT));
-  if (!vec)
-    return p.E <= 256 ? balance_grad<IT, 8, 1>(p, sh, st) : balance_grad<IT, 32, 1>(p, sh, st);
-  switch ((p.E + 127) / 128) {
-    case 1: return balance_grad<IT, 1, 4>(p, sh, st);
-    case 2: return balance_grad<IT, 2, 4>(p, sh, st);
-    case 3: return balance_grad<IT, 3, 4>(p, sh, st);
-    case 4: return balance_grad<IT, 4, 4>(p, sh, st);
-    default: return balance_grad<IT, 8, 4>(p, sh, st);
-  }
+  if (sh.cluster)
+    return vec ? balance_small_go<IT, 16, 4, GRAD, FUNC>(p, sh, st)
+               : balance_small_go<IT, 16, 1, GRAD, FUNC>(p, sh, st);
+  if (!vec) return balance_go<IT, 16, 1, GRAD, FUNC>(p, sh, st);
+  if (p.E <= 256) return balance_go<IT, 4, 4, GRAD, FUNC>(p, sh, st);
+  if (p.E <= 384) return balance_go<IT, 6, 4, GRAD, FUNC>(p, sh, st);
+  if (p.E <= 512) return balance_go<IT, 8, 4, GRAD, FUNC>(p, sh, st);
+  return balance_go<IT, 16, 4, GRAD, FUNC>(p, sh, st);
+}
+template <typename IT, bool GRAD>
+cudaError_t balance_func(const BalArgs &p, const BalShape &sh, cudaStream_t st) {
+  if (p.func == DSV41_SCORE_SOFTMAX) return balance_rows<IT, GRAD, DSV41_SCORE_SOFTMAX>(p, sh, st);
+  if (p.func == DSV41_SCORE_SIGMOID) return balance_rows<IT, GRAD, DSV41_SCORE_SIGMOID>(p, sh, st);
+  return balance_rows<IT, GRAD, DSV41_SCORE_SQRTSOFTPLUS>(p, sh, st);
+}
+template <typename IT>
+cudaError_t balance_launch(const BalArgs &p, const BalShape &sh, cudaStream_t st) {
+  return p.dlogits ? balance_func<IT, true>(p, sh, st) : balance_func<IT, false>(p, sh, st);
 }
 
 }  // namespace
 
 extern "C" size_t dsv41_moe_balance_workspace_size(int64_t T, int64_t E, int64_t S) {
   if (T < 0 || E <= 0 || S < 0 || balance_is_small(T, E, S)) return 0;
-  return align_up(size_t(S + 1) * 4, 256) + size_t(ceil_div(T, balance_run(T)) + S) * 8 + 256;
+  return align_up(size_t(S + 1) * 4, 256) + size_t(ceil_div(T, balance_run(T, E)) + S) * 8 + 256;
 }
 
 extern "C" int dsv41_moe_balance(const void *logits, int dtype, int64_t T, int64_t E,
@@ -817,36 +830,39 @@ extern "C" int dsv41_moe_balance(const void *logits, int dtype, int64_t T, int64
             grad_loss, dweights, norm_topk_prob, route_scale, loss, counts, dlogits, nullptr,
             nullptr, 0};
   BalShape sh{};
-  const size_t add = dweights ? size_t(BL_WARPS) * E * 4 : 0;
+  const size_t add = dweights ? size_t(BL_WARPS) * align_up(E, 4) * 4 : 0;
   if (balance_is_small(T, E, S)) {
     sh.cluster = sh.grid = unsigned(std::min<int64_t>(8, ceil_div(T, BL_WARPS)));
-    sh.smem = size_t(S * E + S + T) * 4 + add;
+    sh.smem = (align_up(S * E, 4) + align_up(S, 4) + align_up(T, 4)) * 4 + add;
   } else {
     DSV41_REQUIRE(workspace && workspace_bytes >= dsv41_moe_balance_workspace_size(T, E, S),
                   DSV41_ERR_WORKSPACE, "workspace too small");
     DSV41_REQUIRE(aligned(workspace, 8), DSV41_ERR_MISALIGNED, "workspace must be 8-byte aligned");
     WsCarve ws{static_cast<uint8_t *>(workspace), workspace_bytes, 0};
     p.live = ws.take<int>(S + 1);
-    p.run = int(balance_run(T));
+    p.run = int(balance_run(T, E));
     p.part = ws.take<double>(ceil_div(T, p.run) + S);
     sh.grid = unsigned(ceil_div(ceil_div(T, p.run), BL_WARPS));
     sh.smem = add;
     const int64_t n = S * E + S;
     ProfScope prof("balance_count", st);
-    if (n <= BL_COUNT_INTS) {
+    if (n <= BL_COUNT_INTS && T * topk <= BL_CLUSTER_CHOICES) {
       DSV41_LAUNCH(max_dynamic_smem(k_balance_count, n * 4), "balance_count");
       DSV41_LAUNCH(launch_cluster(false, k_balance_count, 8, 8, 1024, size_t(n) * 4, st, p),
                    "balance_count");
     } else {
-      DSV41_LAUNCH(cudaMemsetAsync(p.live, 0, (S + 1) * 4, st), "balance memset");
-      DSV41_LAUNCH(cudaMemsetAsync(counts, 0, S * E * 4, st), "balance memset");
-      k_balance_count_global<<<unsigned(ceil_div(T, 256)), 256, 0, st>>>(p);
-      DSV41_CHECK_LAUNCH("balance_count");
+      const unsigned grid = unsigned(num_sms());
+      const int shared = n <= BL_COUNT_INTS;
+      k_balance_zero<<<unsigned(std::min<int64_t>(grid, ceil_div(n + 1, 256))), 256, 0, st>>>(p);
+      DSV41_CHECK_LAUNCH("balance_zero");
+      DSV41_LAUNCH(max_dynamic_smem(k_balance_count_wide, shared ? n * 4 : 0), "balance_count");
+      DSV41_LAUNCH(launch_pdl_if(true, k_balance_count_wide, dim3(grid), dim3(256),
+                                 shared ? size_t(n) * 4 : 0, st, p, shared), "balance_count");
     }
   }
   ProfScope prof("balance", st);
-  return cuda_status(dtype == DSV41_F32 ? balance_rows<float>(p, sh, st)
-                                        : balance_rows<__nv_bfloat16>(p, sh, st), "balance");
+  return cuda_status(dtype == DSV41_F32 ? balance_launch<float>(p, sh, st)
+                                        : balance_launch<__nv_bfloat16>(p, sh, st), "balance");
 }
 
 extern "C" int dsv41_moe_logits(const void *x, int64_t T, int64_t D, const void *gate_w, int64_t E,

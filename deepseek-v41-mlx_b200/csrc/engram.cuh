@@ -159,11 +159,6 @@ __device__ __forceinline__ bool gs_row(int64_t id, const uint8_t *&rt, const uin
   return in;
 }
 
-__device__ __forceinline__ uint64_t f32x2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
 
 // The row scale 2^(sb - 127) as the accumulation takes it: the f16 bits of the scale when it
 // is an f16 (sb in [103, 142], the scales real tables use), else 0x10000 | sb.
