@@ -12,7 +12,6 @@ from __future__ import annotations
 import ctypes as C
 import os
 import threading
-from contextlib import nullcontext
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB_NAME = "libdsv41q.so"
@@ -223,10 +222,22 @@ def stream_of(t) -> int:
     return torch().cuda.current_stream(t.device).cuda_stream
 
 
-def on(device):
-    """Context in which ``device`` is the current device (nothing to do when it already is)."""
-    t = torch()
-    return nullcontext() if t.cuda.current_device() == device.index else t.cuda.device(device)
+def call_on(device, name: str, *args):
+    """``call`` with ``device`` as the current device (the library launches on the current one)."""
+    fn = getattr(load(), name)
+    if torch().cuda.current_device() == device.index:
+        status = fn(*args)
+    else:
+        with torch().cuda.device(device):
+            status = fn(*args)
+    if status:
+        check(status, name)
+
+
+def ready(v, dtype, device) -> bool:
+    """v is a contiguous torch tensor of ``dtype`` on ``device``: nothing to check or convert."""
+    return type(v) is _torch.Tensor and v.dtype is dtype and v.device == device \
+        and v.is_contiguous()
 
 
 def dtype_code(dt) -> int:

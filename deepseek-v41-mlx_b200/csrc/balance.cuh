@@ -435,7 +435,10 @@ __device__ __forceinline__ void balance_tokens(const BalArgs &p, int64_t t0, int
         for (int i = 0; i < NP; ++i) {
           const int e0 = bal_elem<VEC>(i, 0, lane), e1 = bal_elem<VEC>(i, 1, lane);
           if constexpr (VEC == 4) {
-            if (e0 < E) o[i] = f32x2_add(o[i], *reinterpret_cast<const uint64_t *>(add + e0));
+            if (e0 < E) {
+              const uint4 *at = reinterpret_cast<const uint4 *>(add + (e0 & ~3));
+              o[i] = f32x2_add(o[i], i & 1 ? (uint64_t(at->w) << 32) | at->z : (uint64_t(at->y) << 32) | at->x);
+            }
           } else {
             o[i] = f32x2_add(o[i], f32x2(e0 < E ? add[e0] : 0.0f, e1 < E ? add[e1] : 0.0f));
           }

@@ -15,30 +15,42 @@ multiple of 8.  Ids at or past n count as none and raise bit 1 of ``dsv41_device
 
 from __future__ import annotations
 
+import functools
+
 from . import _lib as L
 
 
-def _tensor(v, name, dtype, device=None):
-    """A contiguous CUDA tensor of ``dtype``, on ``device`` where one is given."""
+@functools.lru_cache(maxsize=1024)
+def _workspace_size(device, T, K, N, n, R, backward):
+    # (by device too: the grids follow its number of SMs)
+    with L.torch().cuda.device(device):
+        return L.load().dsv41_lora_workspace_size(T, K, N, n, R, backward)
+
+
+def _tensor(v, name, dtype, device):
+    """v as a contiguous CUDA tensor of ``dtype`` on ``device``."""
+    if L.ready(v, dtype, device):
+        return v
     v = L.cuda_tensor(v, name)
     if v.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, not {v.dtype}")
-    if device is not None and v.device != device:
+    if v.device != device:
         raise ValueError(f"{name} is on {v.device}, x on {device}")
     return v
 
 
 def _operands(x, a, b, ids, scaling):
-    """x bf16, the bank, the ids int32, and the sizes (T, K, N, n, R)."""
+    """x bf16, the bank, the ids int32, the device and the sizes T, K, N, n, R."""
     t = L.torch()
     x = L.cuda_tensor(x, "x")
     if x.dtype != t.bfloat16:
         x = x.to(t.bfloat16)
     dev = x.device
     a, b = _tensor(a, "a", t.bfloat16, dev), _tensor(b, "b", t.bfloat16, dev)
-    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+    sa, sb = a.shape, b.shape
+    if len(sa) != 3 or len(sb) != 3 or sa[0] != sb[0] or sa[1] != sb[2]:
         raise ValueError("a must be [n, R, K] and b [n, N, R]")
-    n, R, K = a.shape
+    n, R, K = sa
     if scaling is not None:
         scaling = _tensor(scaling, "scaling", t.float32, dev)
         if scaling.shape != (n,):
@@ -46,13 +58,14 @@ def _operands(x, a, b, ids, scaling):
     if x.dim() == 0 or x.shape[-1] != K or K == 0:
         raise ValueError(f"x must be [..., {K}]")
     T = x.numel() // K
-    ids = L.as_tensor(ids)
-    if ids.dtype == t.int64:             # ids that int32 cannot hold are no adapter's
-        ids = ids.clamp(-1, 0x7FFFFFFF).to(t.int32)
-    ids = _tensor(ids, "ids", t.int32, dev)
+    if not L.ready(ids, t.int32, dev):
+        ids = L.as_tensor(ids)
+        if ids.dtype == t.int64:             # ids that int32 cannot hold are no adapter's
+            ids = ids.clamp(-1, 0x7FFFFFFF).to(t.int32)
+        ids = _tensor(ids, "ids", t.int32, dev)
     if ids.numel() != T:
         raise ValueError(f"ids must name the adapter of each of the {T} tokens")
-    return x, a, b, ids, scaling, (T, K, b.shape[1], n, R)
+    return x, a, b, ids, scaling, dev, T, K, sb[1], n, R
 
 
 def _rows(v, name, rows, cols, dtype, device):
@@ -83,22 +96,25 @@ def lora_forward(x, a, b, ids, scaling=None, base=None, out_dtype=None, out=None
     out's dtype, else bf16.  With ``return_h`` also h = x @ a[i].T, float32 [..., R], which
     ``lora_backward`` takes."""
     t = L.torch()
-    x, a, b, ids, scaling, (T, K, N, n, R) = _operands(x, a, b, ids, scaling)
-    dev, lead = x.device, x.shape[:-1]
+    x, a, b, ids, scaling, dev, T, K, N, n, R = _operands(x, a, b, ids, scaling)
+    lead = x.shape[:-1]
     like = base if base is not None else out
     odt = out_dtype or (t.bfloat16 if like is None else like.dtype)
     code = _code(odt)
     base = _rows(base, "base", T, N, odt, dev)
     if out is None:
-        out = t.empty(lead + (N,), dtype=odt, device=dev)
+        if base is not None and base.shape[:-1] == lead:
+            out = t.empty_like(base)
+        else:
+            out = x.new_empty(lead + (N,), dtype=odt)
     elif _rows(out, "out", T, N, odt, dev) is not out:
         raise ValueError("out must be a contiguous CUDA tensor")
-    h = t.empty(lead + (R,), dtype=t.float32, device=dev) if return_h else None
-    with L.on(dev):
-        nb = L.load().dsv41_lora_workspace_size(T, K, N, n, R, 0)
-        ws = L.workspace(nb, dev) if nb else None
-        L.call("dsv41_lora_forward", L.ptr(x), T, K, L.ptr(a), L.ptr(b), n, R, N, L.ptr(scaling),
-               L.ptr(ids), L.ptr(base), code, L.ptr(out), L.ptr(h), L.ptr(ws), nb, L.stream_of(x))
+    h = x.new_empty(lead + (R,), dtype=t.float32) if return_h else None
+    nb = _workspace_size(dev, T, K, N, n, R, 0)
+    ws = L.workspace(nb, dev) if nb else None
+    L.call_on(dev, "dsv41_lora_forward", x.data_ptr(), T, K, a.data_ptr(), b.data_ptr(), n, R, N,
+              L.ptr(scaling), ids.data_ptr(), L.ptr(base), code, out.data_ptr(), L.ptr(h),
+              L.ptr(ws), nb, L.stream_of(x))
     return (out, h) if return_h else out
 
 
@@ -111,23 +127,20 @@ def lora_backward(dy, x, h, a, b, ids, scaling=None, dx_base=None, dx_dtype=None
     dtype, else bf16.  da [n, R, K] and db [n, N, R] are ``grad_dtype`` (default: a's) and whole:
     zeros for adapters without tokens.  base's gradient is dy itself."""
     t = L.torch()
-    x, a, b, ids, scaling, (T, K, N, n, R) = _operands(x, a, b, ids, scaling)
-    dev = x.device
+    x, a, b, ids, scaling, dev, T, K, N, n, R = _operands(x, a, b, ids, scaling)
     dy = _rows(dy, "dy", T, N, t.bfloat16, dev)
     h = _rows(h, "h", T, R, t.float32, dev)
     xdt = dx_dtype or (t.bfloat16 if dx_base is None else dx_base.dtype)
-    gdt = grad_dtype or a.dtype
+    gdt = grad_dtype or t.bfloat16
     xcode, gcode = _code(xdt), _code(gdt)
     dx_base = _rows(dx_base, "dx_base", T, K, xdt, dev)
-    dx = t.empty(x.shape, dtype=xdt, device=dev)
-    da = t.empty(a.shape, dtype=gdt, device=dev)
-    db = t.empty(b.shape, dtype=gdt, device=dev)
-    with L.on(dev):
-        nb = L.load().dsv41_lora_workspace_size(T, K, N, n, R, 1)
-        ws = L.workspace(nb, dev) if nb else None
-        L.call("dsv41_lora_backward", L.ptr(dy), L.ptr(x), L.ptr(h), L.ptr(a), L.ptr(b), T, K, N,
-               n, R, L.ptr(scaling), L.ptr(ids), L.ptr(dx_base), xcode, L.ptr(dx), gcode,
-               L.ptr(da), L.ptr(db), L.ptr(ws), nb, L.stream_of(x))
+    dx = t.empty_like(x, dtype=xdt)
+    da, db = t.empty_like(a, dtype=gdt), t.empty_like(b, dtype=gdt)
+    nb = _workspace_size(dev, T, K, N, n, R, 1)
+    ws = L.workspace(nb, dev) if nb else None
+    L.call_on(dev, "dsv41_lora_backward", dy.data_ptr(), x.data_ptr(), h.data_ptr(), a.data_ptr(),
+              b.data_ptr(), T, K, N, n, R, L.ptr(scaling), ids.data_ptr(), L.ptr(dx_base), xcode,
+              dx.data_ptr(), gcode, da.data_ptr(), db.data_ptr(), L.ptr(ws), nb, L.stream_of(x))
     return dx, da, db
 
 

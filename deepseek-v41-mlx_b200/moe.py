@@ -23,6 +23,7 @@ intermediate in fp32 (``round_bf16=False``).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import gc
 
 from . import _lib as L
@@ -96,7 +97,7 @@ class Gate:
         if xt.shape[-1] != D or w.device != xt.device:
             raise ValueError(f"x must be [..., {D}] on the weight's device")
         out = t.empty(tuple(xt.shape[:-1]) + (E,), dtype=t.float32, device=xt.device)
-        with L.on(xt.device):
+        with t.cuda.device(xt.device):
             ws = L.workspace(L.load().dsv41_moe_route_workspace_size(T, D, E), xt.device)
             L.call("dsv41_moe_logits", L.ptr(xt), T, D, L.ptr(w), E, L.ptr(out), L.ptr(ws),
                    ws.numel(), L.stream_of(xt))
@@ -107,6 +108,12 @@ class Gate:
         """``balance_loss`` with this router's score function, temperature and scale."""
         return balance_loss(logits, indices, offsets, mask, self.score_func, self.gate_temp,
                             grad_loss, dweights, self.norm_topk_prob, self.route_scale)
+
+
+@functools.lru_cache(maxsize=1024)
+def _balance_workspace_size(device, T, E, S):
+    with _torch().cuda.device(device):
+        return L.load().dsv41_moe_balance_workspace_size(T, E, S)
 
 
 def balance_loss(logits, indices, offsets=None, mask=None, score_func="sqrtsoftplus",
@@ -136,7 +143,8 @@ def balance_loss(logits, indices, offsets=None, mask=None, score_func="sqrtsoftp
     T = z.numel() // E
 
     def arg(v, name, dtype, count, cols=0):
-        v = L.cuda_tensor(v, name)
+        if not L.ready(v, dtype, dev):
+            v = L.cuda_tensor(v, name)
         if v.dtype != dtype:
             raise ValueError(f"{name} must be {dtype}, not {v.dtype}")
         if v.device != dev:
@@ -165,17 +173,16 @@ def balance_loss(logits, indices, offsets=None, mask=None, score_func="sqrtsoftp
         dweights = arg(dweights, "dweights", t.float32, T * topk, topk)
     if score_func not in L.SCORE_FUNCS:
         raise ValueError(f"unknown score_func {score_func!r}")
-    loss = t.empty((S,), dtype=t.float32, device=dev)
-    counts = t.empty((S, E), dtype=t.int32, device=dev)
+    loss = z.new_empty((S,), dtype=t.float32)
+    counts = z.new_empty((S, E), dtype=t.int32)
     dz = t.empty_like(z) if grad_loss is not None or dweights is not None else None
-    with L.on(dev):
-        nb = L.load().dsv41_moe_balance_workspace_size(T, E, S)
-        ws = L.workspace(nb, dev) if nb else None
-        code = L.F32 if z.dtype == t.float32 else L.BF16
-        L.call("dsv41_moe_balance", L.ptr(z), code, T, E, L.ptr(idx), topk,
-               L.ptr(offsets), S, L.ptr(mask), L.SCORE_FUNCS[score_func], float(gate_temp),
-               L.ptr(grad_loss), L.ptr(dweights), int(norm_topk_prob), float(route_scale),
-               L.ptr(loss), L.ptr(counts), L.ptr(dz), L.ptr(ws), nb, L.stream_of(z))
+    nb = _balance_workspace_size(dev, T, E, S)
+    ws = L.workspace(nb, dev) if nb else None
+    L.call_on(dev, "dsv41_moe_balance", z.data_ptr(), L.F32 if z.dtype == t.float32 else L.BF16, T,
+              E, idx.data_ptr(), topk, L.ptr(offsets), S, L.ptr(mask), L.SCORE_FUNCS[score_func],
+              float(gate_temp), L.ptr(grad_loss), L.ptr(dweights), int(norm_topk_prob),
+              float(route_scale), loss.data_ptr(), counts.data_ptr(), L.ptr(dz), L.ptr(ws), nb,
+              L.stream_of(z))
     return loss, counts, dz
 
 
