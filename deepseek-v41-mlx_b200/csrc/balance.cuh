@@ -135,21 +135,14 @@ __device__ __forceinline__ void score_sigmoid(float z, float &s, float &ds) {
   ds = u * d * d;
 }
 
-// The warp's sums of four values in 10 shuffles: half the values change lanes with half the
-// partners, then each quarter of the warp finishes one.
-__device__ __forceinline__ void warp_sum4(float &a, float &b, float &c, float &d) {
-  const int lane = threadIdx.x & 31;
-  const bool h = lane & 16, q = lane & 8;
-  const float x = (h ? c : a) + __shfl_xor_sync(0xffffffffu, h ? a : c, 16);
-  const float y = (h ? d : b) + __shfl_xor_sync(0xffffffffu, h ? b : d, 16);
-  float v = (q ? y : x) + __shfl_xor_sync(0xffffffffu, q ? x : y, 8);
-  v += __shfl_xor_sync(0xffffffffu, v, 4);
-  v += __shfl_xor_sync(0xffffffffu, v, 2);
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
+// The warp's sums of two values in 7 shuffles: half the lanes go on with one, half with the other.
+__device__ __forceinline__ void warp_sum2(float &a, float &b) {
+  const bool h = threadIdx.x & 16;
+  float v = (h ? b : a) + __shfl_xor_sync(0xffffffffu, h ? a : b, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   a = __shfl_sync(0xffffffffu, v, 0);
-  b = __shfl_sync(0xffffffffu, v, 8);
-  c = __shfl_sync(0xffffffffu, v, 16);
-  d = __shfl_sync(0xffffffffu, v, 24);
+  b = __shfl_sync(0xffffffffu, v, 16);
 }
 
 __device__ __forceinline__ float bal_ld(const float *p) { return __ldg(p); }
@@ -220,6 +213,49 @@ __device__ __forceinline__ void bal_store(IT *row, int E, int lane, const uint64
   }
 }
 
+// The routing weights' side of 32 / k tokens at once, a lane a choice (k <= 32): what a token's
+// choices need of one another is summed here, and a choice of an expert that an earlier lane of
+// the same token has chosen too is left to that lane.  (One token at a time, most lanes idle, was a
+// third of the pass: 28 of 83 us at T 65536, E 384, k 6.)
+template <typename IT, int FUNC> struct BalChoices {
+  int seg, idx;                // token of the batch, expert (-1: none here)
+  float dw, n, e, d, sum, dsum, top;
+  // idx_in, dw_in: this lane's choice; z: the tokens' rows from the batch's first on
+  __device__ __forceinline__ void make(const BalArgs &p, const IT *z, int k, int idx_in, float dw_in) {
+    const int lane = threadIdx.x & 31;
+    idx = idx_in < p.E ? idx_in : -1;
+    dw = idx >= 0 ? dw_in : 0.0f;
+    const float zs = idx >= 0 ? bal_ld(z + int64_t(seg) * p.E + idx) * p.inv_temp : -INFINITY;
+    e = d = top = 0.0f;
+    const int first = min(seg * k, 32 - k);          // (idle lanes read a token that exists)
+    if constexpr (FUNC == DSV41_SCORE_SOFTMAX) {
+      top = -INFINITY;
+      for (int j = 0; j < k; ++j) top = fmaxf(top, __shfl_sync(0xffffffffu, zs, first + j));
+      if (idx >= 0) e = d = top > -INFINITY ? exp_acc(zs - top) : 0.0f;
+    } else if (idx >= 0) {
+      if (FUNC == DSV41_SCORE_SIGMOID) score_sigmoid(zs, e, d);
+      else score_sqrtsoftplus(zs, e, d);
+    }
+    sum = dsum = 0.0f;
+    for (int j = 0; j < k; ++j) {
+      sum += __shfl_sync(0xffffffffu, e, first + j);
+      dsum += __shfl_sync(0xffffffffu, dw * e, first + j);
+    }
+    n = 1.0f;
+    const unsigned same = __match_any_sync(0xffffffffu, idx >= 0 ? (seg << 16) | idx : -1 - lane);
+    if (__any_sync(0xffffffffu, __popc(same) > 1)) {
+      float all = 0.0f;
+      for (int j = 0; j < 32; ++j) {
+        const float v = __shfl_sync(0xffffffffu, dw, j);
+        if (same >> j & 1) all += v;
+      }
+      dw = all;
+      n = float(__popc(same));
+      if (lane != __ffs(same) - 1) idx = -1;
+    }
+  }
+};
+
 // A warp's tokens [t0, t1), in order.  cnt / live: the sequences' counters (global or shared
 // memory), ready after `ready()`.  add: this warp's row of E floats in shared memory, zero between
 // tokens (the routing weights' gradients on their way to the lanes that own the experts).
@@ -243,36 +279,44 @@ __device__ __forceinline__ void balance_tokens(const BalArgs &p, int64_t t0, int
   uint64_t c[NP];
   float coef = 0.0f;
   BalRow<IT, NP, VEC> nx;
-  int idx_n[2] = {-1, -1};
-  float dw_n[2] = {0.f, 0.f};
   bool on_n = false;
-  auto fetch = [&](const IT *zr, const int32_t *ir, const float *wr, const uint8_t *mr) {
+  const int G = wide ? 1 : 32 / k;                  // tokens of a batch of choices
+  BalChoices<IT, FUNC> bc;
+  bc.seg = wide ? 0 : lane / k;
+  int at = G - 1, ch_idx = -1;                      // token of the batch; the next batch's choices
+  float ch_dw = 0.0f;
+  auto fetch = [&](const IT *zr, const uint8_t *mr) {
     on_n = !p.mask || *mr;
-    if (!on_n) return;
-    nx.load(zr, E, lane);
-    if (routed) {
-      if (lane < k) {
-        idx_n[0] = __ldg(ir + lane);
-        dw_n[0] = __ldg(wr + lane);
-      }
-      if (wide && lane + 32 < k) {
-        idx_n[1] = __ldg(ir + lane + 32);
-        dw_n[1] = __ldg(wr + lane + 32);
-      }
+    if (on_n) nx.load(zr, E, lane);
+  };
+  // this lane's choice of the batch that begins at token t (ip, wp, mp: that token's)
+  auto fetch_choices = [&](int64_t t) {
+    ch_idx = -1;
+    if (bc.seg < G && t + bc.seg < t1 && (!p.mask || mp[bc.seg])) {
+      ch_idx = __ldg(ip + lane);
+      ch_dw = __ldg(wp + lane);
     }
   };
-  if (t0 < t1) fetch(z, ip, wp, mp);
+  if (t0 < t1) fetch(z, mp);
+  if (routed && !wide) fetch_choices(t0);
   ready();
 #pragma unroll 1
   for (int64_t t = t0; t < t1; ++t, z += E, dl += E) {
     const BalRow<IT, NP, VEC> row = nx;
-    int idx[2] = {idx_n[0], idx_n[1]};
-    float dw[2] = {dw_n[0], dw_n[1]};
     const bool on = on_n;
-    ip += k;
-    wp += k;
-    ++mp;
-    if (t + 1 < t1) fetch(z + E, ip, wp, mp);
+    if (routed && !wide && ++at >= G) {
+      const int ci = ch_idx;
+      const float cw = ch_dw;
+      const int64_t left = t1 - t;
+      at = 0;
+      // ip, wp and mp run a batch ahead of z
+      ip += G * k;
+      wp += G * k;
+      mp += G;
+      if (left > G) fetch_choices(t + G);
+      bc.make(p, z, k, ci, cw);
+    }
+    if (t + 1 < t1) fetch(z + E, p.mask + (p.mask ? t + 1 : 0));
     if (t >= sq.b) {
       sq = balance_seq(p, t);
       if (sq.q >= 0) {
@@ -293,24 +337,6 @@ __device__ __forceinline__ void balance_tokens(const BalArgs &p, int64_t t0, int
         bal_store<IT, NP, VEC>(dl, E, lane, zero);
       }
       continue;
-    }
-    // the chosen experts' logits, read again while the row is in the cache
-    float zs[2] = {0.f, 0.f};
-    if (routed) {
-      if (lane >= k || idx[0] < 0 || idx[0] >= E) {
-        idx[0] = -1;
-        dw[0] = 0.0f;
-      } else {
-        zs[0] = bal_ld(z + idx[0]) * p.inv_temp;
-      }
-      if (wide) {
-        if (lane + 32 >= k || idx[1] < 0 || idx[1] >= E) {
-          idx[1] = -1;
-          dw[1] = 0.0f;
-        } else {
-          zs[1] = bal_ld(z + idx[1]) * p.inv_temp;
-        }
-      }
     }
     uint64_t s[NP], d[NP];                           // scores and their derivatives
     float mx = 0.0f;
@@ -372,54 +398,64 @@ __device__ __forceinline__ void balance_tokens(const BalArgs &p, int64_t t0, int
       cs2 = f32x2_fma(c[i], s[i], cs2);
     }
     float sum = f32x2_lo(sum2) + f32x2_hi(sum2), cs = f32x2_lo(cs2) + f32x2_hi(cs2);
-    // the sums over the row, and those of the routing weights with them
-    float ss[2] = {0.f, 0.f}, dd[2] = {0.f, 0.f}, sel = 0.0f, dws = 0.0f;
-    if (routed) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (u && !wide) break;
-        if (idx[u] >= 0) {
-          if (FUNC == DSV41_SCORE_SOFTMAX) ss[u] = dd[u] = mx > -INFINITY ? exp_acc(zs[u] - mx) : 0.0f;
-          else if (FUNC == DSV41_SCORE_SIGMOID) score_sigmoid(zs[u], ss[u], dd[u]);
-          else score_sqrtsoftplus(zs[u], ss[u], dd[u]);
-        }
-        sel += ss[u];
-        dws = fmaf(dw[u], ss[u], dws);
-      }
-    }
-    warp_sum4(sum, cs, sel, dws);
+    warp_sum2(sum, cs);
     float rs = 1.0f, rz;                             // 1 / sum of the exponentials, of the scores
     if constexpr (FUNC == DSV41_SCORE_SOFTMAX) {
-      // s, d, ss, dd still lack the factor rs (a row of -inf: zeros; NaN stays NaN)
+      // s and d still lack the factor rs (a row of -inf: zeros; NaN stays NaN)
       rs = mx > -INFINITY ? __fdividef(1.0f, sum) : (mx == -INFINITY ? 0.0f : mx);
       rz = 1.0f;
       cs *= rs;
-      sel *= rs;
-      dws *= rs;
     } else {
       rz = __fdividef(1.0f, sum + 1e-20f);
     }
     const float dot = cs * rz;
     done(t, sq.q, dot);
     if constexpr (GRAD) {
-      float R = 0.0f;                                // softmax: sum of the weights' ds times s
-      if (routed) {
-        const float rsel = nrm ? __fdividef(1.0f, sel + 1e-20f) : 1.0f;
-        const float mean = nrm ? dws * rsel : 0.0f, sc = p.route_scale * rsel;
-        R = sc * (dws - mean * sel);
+      // the routing weights: with S = sum s and D = sum dw s over the choices, a choice adds scale
+      // (dw - D / S) / S ds/dz (not normalised: scale dw ds/dz); softmax also takes R = sum ds s
+      // off every element.  Its e are scaled to the choices' largest: s = phi e.
+      float R = 0.0f;
+      if (routed && !wide) {
+        float phi = 1.0f, S = bc.sum, D = bc.dsum;
+        if constexpr (FUNC == DSV41_SCORE_SOFTMAX) {
+          const int from = at * k;
+          S = __shfl_sync(0xffffffffu, bc.sum, from);
+          D = __shfl_sync(0xffffffffu, bc.dsum, from);
+          const float top = __shfl_sync(0xffffffffu, bc.top, from);
+          phi = top > -INFINITY ? exp_acc(top - mx) * rs : 0.0f;
+        }
+        const float w = nrm ? __fdividef(phi, fmaf(phi, S, 1e-20f)) : phi, mean = nrm ? D * w : 0.0f;
+        if (FUNC == DSV41_SCORE_SOFTMAX) R = p.route_scale * w * (nrm ? fmaf(-mean, S, D) : D);
+        if (bc.seg == at && bc.idx >= 0)
+          add[bc.idx] = p.route_scale * w * fmaf(-bc.n, mean, bc.dw) * bc.d * p.inv_temp;
+        __syncwarp();
+      } else if (routed) {
+        // more than 32 choices: two a lane, added one after another
+        float e[2], f[2], w[2], S = 0.0f, D = 0.0f;
+        int id[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          if (u && !wide) break;
-          const float g = sc * (dw[u] - mean) * (dd[u] * rs) * p.inv_temp;
-          // the same expert twice: one after another, in lane order
-          const unsigned same = __match_any_sync(0xffffffffu, idx[u] >= 0 ? idx[u] : -1 - lane);
-          const int turn = __popc(same & ((1u << lane) - 1));
-          if (turn == 0 && idx[u] >= 0) add[idx[u]] += g;
-          __syncwarp();
-          for (int o = 1; __any_sync(0xffffffffu, turn >= o); ++o) {
-            if (turn == o && idx[u] >= 0) add[idx[u]] += g;
-            __syncwarp();
+          e[u] = f[u] = w[u] = 0.0f;
+          id[u] = lane + 32 * u < k ? p.indices[t * k + lane + 32 * u] : -1;
+          if (id[u] >= E) id[u] = -1;
+          if (id[u] >= 0) {
+            const float zi = bal_ld(z + id[u]) * p.inv_temp;
+            w[u] = p.dweights[t * k + lane + 32 * u];
+            if (FUNC == DSV41_SCORE_SOFTMAX) e[u] = f[u] = mx > -INFINITY ? exp_acc(zi - mx) * rs : 0.0f;
+            else if (FUNC == DSV41_SCORE_SIGMOID) score_sigmoid(zi, e[u], f[u]);
+            else score_sqrtsoftplus(zi, e[u], f[u]);
           }
+          S += e[u];
+          D = fmaf(w[u], e[u], D);
+        }
+        warp_sum2(S, D);
+        const float r = nrm ? __fdividef(1.0f, S + 1e-20f) : 1.0f, mean = nrm ? D * r : 0.0f;
+        if (FUNC == DSV41_SCORE_SOFTMAX) R = p.route_scale * r * fmaf(-mean, S, D);
+        for (int j = 0; j < k; ++j) {
+          const int u = j >> 5;
+          const float g = p.route_scale * r * ((u ? w[1] : w[0]) - mean) * (u ? f[1] : f[0]) * p.inv_temp;
+          if (lane == (j & 31) && (u ? id[1] : id[0]) >= 0) add[u ? id[1] : id[0]] += g;
+          __syncwarp();
         }
       }
       // d loss / d s = ca (c - dot); times the derivative (softmax: s (ds - sum ds s), whose loss
@@ -447,9 +483,11 @@ __device__ __forceinline__ void balance_tokens(const BalArgs &p, int64_t t0, int
       bal_store<IT, NP, VEC>(dl, E, lane, o);
       if (routed) {
         __syncwarp();
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (idx[u] >= 0) add[idx[u]] = 0.0f;
+        if (!wide) {
+          if (bc.seg == at && bc.idx >= 0) add[bc.idx] = 0.0f;
+        } else {
+          for (int e = lane; e < E; e += 32) add[e] = 0.0f;
+        }
         __syncwarp();
       }
     }
