@@ -84,17 +84,18 @@ __global__ void __launch_bounds__(1024, 1)
   extern __shared__ int lp_smem[];                                    // [n + 1] each
   int *cnt = lp_smem, *pos = cnt + (n + 1), *tile0 = pos + (n + 1), *first = tile0 + (n + 1),
       *block0 = first + (n + 1);
-  __shared__ int wsum[32][3];
+  __shared__ int wsum[32][3], bin_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = gridDim.x, rank = blockIdx.x;
   pdl_trigger();
   const int per = (((T + C - 1) / C) + 1023) & ~1023;
   const int t0 = int(min(int64_t(rank) * per, int64_t(T)));
   const int t1 = int(min(int64_t(t0) + per, int64_t(T)));
+  int bin_1 = t0 + tid < t1 ? lora_bin(ids[t0 + tid], n) : -1;        // of the first batch
   for (int i = tid; i <= n; i += 1024) cnt[i] = 0;
   __syncthreads();
   for (int b0 = t0; b0 < t1; b0 += 1024) {
-    const int bin = b0 + tid < t1 ? lora_bin(ids[b0 + tid], n) : -1;
+    const int bin = b0 == t0 ? bin_1 : b0 + tid < t1 ? lora_bin(ids[b0 + tid], n) : -1;
     const unsigned same = __match_any_sync(0xffffffffu, bin);         // runs: one add a warp
     if (bin >= 0 && lane == __ffs(same) - 1) atomicAdd(&cnt[bin], __popc(same));
   }
@@ -130,6 +131,7 @@ __global__ void __launch_bounds__(1024, 1)
     used += __syncthreads_count(b < n && total > 0);
     for (int i = 0; i < 3; ++i) run[i] += tot[i];
   }
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");      // histograms read
   if (rank == 0 && tid == 0) {
     p.head[0] = run[1];
     p.head[1] = used;
@@ -148,8 +150,11 @@ __global__ void __launch_bounds__(1024, 1)
   }
   // scatter: batches of 1024 tokens, their warps one after another
   for (int b0 = t0; b0 < t1; b0 += 1024) {
-    const int t = b0 + tid, bin0 = lora_bin(ids[b0], n);
-    const int bin = t < t1 ? lora_bin(ids[t], n) : -1;
+    const int t = b0 + tid;
+    const int bin = b0 == t0 ? bin_1 : t < t1 ? lora_bin(ids[t], n) : -1;
+    if (tid == 0) bin_s = bin;
+    __syncthreads();
+    const int bin0 = bin_s;
     if (__syncthreads_and(bin < 0 || bin == bin0)) {                  // a run on one adapter
       if (bin >= 0) p.perm[pos[bin0] + tid] = t;
       __syncthreads();
@@ -171,7 +176,7 @@ __global__ void __launch_bounds__(1024, 1)
     }
     __syncthreads();
   }
-  cluster_sync();                               // the others have read this histogram
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // ------------------------------------------------------------------ operand staging
@@ -431,6 +436,9 @@ __global__ void __launch_bounds__(LS_THREADS, 2)
   const int C = int(cluster_nctas()), rank = int(cluster_rank());
   const uint32_t cols = a.Rp <= 32 ? 32u : a.Rp <= 64 ? 64u : 128u;
   if (tid == 0) {
+    prefetch_tmap(&maps.w);
+    prefetch_tmap(&maps.x.run);
+    prefetch_tmap(&maps.x.gather);
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 4);
       mbar_init(&empty[s], 1);
@@ -798,6 +806,10 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
   __shared__ uint32_t tmem_slot;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
+    prefetch_tmap(&maps.w);
+    prefetch_tmap(&maps.parts);
+    prefetch_tmap(&maps.base.run);
+    prefetch_tmap(&maps.y.run);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&a_full[i], 1);
       mbar_init(&a_empty[i], 1);
@@ -1246,6 +1258,8 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
   const uint32_t mma_n = wide ? NS * a.Rp : a.Rp;
   const uint32_t acc_cols = lg_acc_cols(int(mma_n)), cols = 2 * acc_cols;
   if (tid == 0) {
+    prefetch_tmap(&maps.v[0].run);
+    prefetch_tmap(&maps.v[1].run);
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
