@@ -1027,18 +1027,33 @@ int lora_plan_launch(const int32_t *ids, int64_t T, int64_t n, const LoraPlan &p
   return DSV41_OK;
 }
 
-// Up to this many tokens a forward call is one launch (k_lora_decode).
-constexpr int64_t LORA_DECODE_T = 64;
+// A forward call of few tokens is one launch (k_lora_decode): a cluster of C CTAs a token.  A
+// round of CTAs takes about 5 us and 1 us for every 50 KB of its share of an adapter; C is the one
+// with the least of it, and 0 where plan, shrink and expand (23 us and up) are expected to be
+// faster.  (Measured at R 16, K 7168, N 4096: 32 tokens 8.3 us with C = 8, 96 10.8 us with 4, 192
+// 15.7 us with 2, against 30 to 35 us.)
+unsigned lora_decode_ctas(int64_t T, int64_t K, int64_t N, int64_t R) {
+  const int64_t slots = int64_t(num_sms()) * (R <= 32 ? 3 : 1);
+  double best = 24.0;
+  unsigned c_best = 0;
+  for (unsigned c = 8; c >= 2; c >>= 1) {
+    const double cost = double(ceil_div(T * c, slots)) * (5.0 + double(R * (K + N)) * 2.0 / c / 50e3);
+    if (cost < best) {
+      best = cost;
+      c_best = c;
+    }
+  }
+  return c_best;
+}
 
 template <typename OT>
-cudaError_t lora_decode_launch(const LoraDecode &p, int64_t T, cudaStream_t st) {
-  const unsigned C = 8;
+cudaError_t lora_decode_launch(const LoraDecode &p, int64_t T, unsigned C, cudaStream_t st) {
   const unsigned grid = unsigned(T) * C;
-  if (p.R <= 8) return launch_cluster(false, k_lora_decode<OT, 1, 1>, grid, C, LD_THREADS, 0, st, p);
-  if (p.R <= 16) return launch_cluster(false, k_lora_decode<OT, 2, 2>, grid, C, LD_THREADS, 0, st, p);
-  if (p.R <= 32) return launch_cluster(false, k_lora_decode<OT, 4, 4>, grid, C, LD_THREADS, 0, st, p);
-  if (p.R <= 64) return launch_cluster(false, k_lora_decode<OT, 8, 8>, grid, C, LD_THREADS, 0, st, p);
-  return launch_cluster(false, k_lora_decode<OT, 16, 16>, grid, C, LD_THREADS, 0, st, p);
+  if (p.R <= 8) return launch_cluster(false, k_lora_decode<OT, 256, 1, 1>, grid, C, 256, 0, st, p);
+  if (p.R <= 16) return launch_cluster(false, k_lora_decode<OT, 256, 2, 2>, grid, C, 256, 0, st, p);
+  if (p.R <= 32) return launch_cluster(false, k_lora_decode<OT, 256, 4, 4>, grid, C, 256, 0, st, p);
+  if (p.R <= 64) return launch_cluster(false, k_lora_decode<OT, 512, 4, 8>, grid, C, 512, 0, st, p);
+  return launch_cluster(false, k_lora_decode<OT, 512, 8, 16>, grid, C, 512, 0, st, p);
 }
 
 template <bool WMN, bool VEC, int S>
@@ -1155,7 +1170,7 @@ cudaError_t lora_wgrad_launch(const LoraWgradMaps &m, const LoraWgrad &a, const 
 extern "C" size_t dsv41_lora_workspace_size(int64_t T, int64_t K, int64_t N, int64_t n, int64_t R,
                                             int backward) {
   if (T < 0 || K <= 0 || N <= 0 || n <= 0 || R <= 0) return 0;
-  if (T == 0 || (!backward && T <= LORA_DECODE_T)) return 0;
+  if (T == 0 || (!backward && lora_decode_ctas(T, K, N, R))) return 0;
   return lora_carve(nullptr, ~size_t(0), T, K, N, n, R, backward != 0).used;
 }
 
@@ -1172,13 +1187,13 @@ extern "C" int dsv41_lora_forward(const void *x, int64_t T, int64_t K, const voi
   DSV41_REQUIRE(x && a && b && ids && y, DSV41_ERR_BAD_ARG, "NULL pointer");
   DSV41_REQUIRE(aligned(x, 16) && aligned(a, 16) && aligned(b, 16) && aligned(h_out, 16),
                 DSV41_ERR_MISALIGNED, "x, a, b and h_out must be 16-byte aligned");
-  if (T <= LORA_DECODE_T) {
+  if (const unsigned C = lora_decode_ctas(T, K, N, R)) {
     const LoraDecode d{static_cast<const __nv_bfloat16 *>(x), static_cast<const __nv_bfloat16 *>(a),
                        static_cast<const __nv_bfloat16 *>(b), K, N, int(R), int(n), scaling, ids,
                        base, y, h_out};
     ProfScope prof("lora_decode", STREAM(stream));
-    return cuda_status(out_dtype == DSV41_F32 ? lora_decode_launch<float>(d, T, STREAM(stream))
-                                              : lora_decode_launch<__nv_bfloat16>(d, T, STREAM(stream)),
+    return cuda_status(out_dtype == DSV41_F32 ? lora_decode_launch<float>(d, T, C, STREAM(stream))
+                                              : lora_decode_launch<__nv_bfloat16>(d, T, C, STREAM(stream)),
                        "lora_decode");
   }
   LoraWs w = lora_carve(workspace, workspace_bytes, T, K, N, n, R, false);

@@ -644,17 +644,16 @@ __device__ __forceinline__ float dot8(uint4 u, uint4 v, float acc) {
   return acc;
 }
 
-constexpr int LD_THREADS = 256, LD_WARPS = 8;
-
 // Both products of a token in one launch, no plan: a cluster per token.  Each CTA takes a slice
 // of K (its warps R / 8 ranks each), the partial h meet in distributed shared memory in rank
 // order, then each CTA takes a slice of the columns, a row of B per group of LPR lanes.  The
 // first rows of B are requested before the cluster meets.  Bound by the latency of one pass
 // over an adapter (360 KB at K 7168, N 4096, R 16), which tokens on the same adapter find in L2.
-// RW: ranks a warp; LPR: lanes a row of B, the power of two at or above R / 8.
-template <typename OT, int RW, int LPR>
-__global__ void __launch_bounds__(LD_THREADS) k_lora_decode(const LoraDecode p) {
-  constexpr int COLS = LD_THREADS / LPR;            // columns a pass
+// TH threads; RW: ranks a warp; LPR: lanes a row of B, the power of two at or above R / 8.
+template <typename OT, int TH, int RW, int LPR>
+__global__ void __launch_bounds__(TH) k_lora_decode(const LoraDecode p) {
+  constexpr int LD_WARPS = TH / 32;
+  constexpr int COLS = TH / LPR;                    // columns a pass
   constexpr int PF = 8;                             // passes requested ahead
   __shared__ float part[LD_WARPS * RW];
   __shared__ float hs[LD_WARPS * RW];
@@ -666,10 +665,10 @@ __global__ void __launch_bounds__(LD_THREADS) k_lora_decode(const LoraDecode p) 
   const int i = lora_bin(p.ids[t], p.n);
   const int64_t c0 = p.N * rank / C, c1 = p.N * (rank + 1) / C;
   if (i == p.n) {                                   // uniform over the cluster
-    for (int64_t c = c0 + tid; c < c1; c += LD_THREADS)
+    for (int64_t c = c0 + tid; c < c1; c += TH)
       y[c] = base ? base[t * p.N + c] : OT(0.0f);
     if (p.h && rank == 0)
-      for (int r = tid; r < p.R; r += LD_THREADS) p.h[t * p.R + r] = 0.0f;
+      for (int r = tid; r < p.R; r += TH) p.h[t * p.R + r] = 0.0f;
     return;
   }
   const uint4 z = make_uint4(0, 0, 0, 0);
@@ -992,6 +991,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
           for (int h = 0; h < (VEC ? 1 : CB / 32); ++h)
 #pragma unroll
             for (int r = 0; r < 32; ++r) {
+              if (r % 8 == 0 && 32 * q4 + r >= tl.z) break;        // only rows that are there
               const int tk = __shfl_sync(0xffffffffu, tok, r);
               const int64_t c = int64_t(cb) * CB + h * 32 + lane;
               odd[h][r] = tk >= 0 && c < a.N ? base[int64_t(tk) * a.N + c] : OT(0.0f);
@@ -1099,6 +1099,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
             const int64_t c = int64_t(cb) * CB + h + lane;
 #pragma unroll
             for (int r = 0; r < 32; ++r) {
+              if (r % 8 == 0 && 32 * q4 + r >= tl.z) break;
               const int tk = __shfl_sync(0xffffffffu, tok, r);
               float f = has ? tp[r * LE_EPI_LD + lane] : 0.0f;
               if (base) f += float(odd[VEC ? 0 : h / 32][r]);
