@@ -183,6 +183,7 @@ def call(name: str, *args):
 # ---------------------------------------------------------------- torch glue --
 
 _torch = None
+_raw_stream = None
 
 
 def torch():
@@ -216,10 +217,12 @@ def ptr(t) -> int:
 
 def stream_of(t) -> int:
     """The current stream of t's device, as an integer."""
-    raw = getattr(torch()._C, "_cuda_getCurrentRawStream", None)   # no Stream object is built
-    if raw is not None:
-        return raw(t.device.index)
-    return torch().cuda.current_stream(t.device).cuda_stream
+    global _raw_stream
+    if _raw_stream is None:
+        cuda = torch().cuda                          # the raw form builds no Stream object
+        _raw_stream = getattr(_torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda index: cuda.current_stream(index).cuda_stream)
+    return _raw_stream(t.device.index)
 
 
 def call_on(device, name: str, *args):

@@ -29,7 +29,8 @@ def _workspace_size(device, T, K, N, n, R, backward):
 
 def _tensor(v, name, dtype, device):
     """v as a contiguous CUDA tensor of ``dtype`` on ``device``."""
-    if L.ready(v, dtype, device):
+    if type(v) is L.torch().Tensor and v.dtype is dtype and v.device == device \
+            and v.is_contiguous():
         return v
     v = L.cuda_tensor(v, name)
     if v.dtype != dtype:
@@ -58,11 +59,9 @@ def _operands(x, a, b, ids, scaling):
     if x.dim() == 0 or x.shape[-1] != K or K == 0:
         raise ValueError(f"x must be [..., {K}]")
     T = x.numel() // K
-    if not L.ready(ids, t.int32, dev):
-        ids = L.as_tensor(ids)
-        if ids.dtype == t.int64:             # ids that int32 cannot hold are no adapter's
-            ids = ids.clamp(-1, 0x7FFFFFFF).to(t.int32)
-        ids = _tensor(ids, "ids", t.int32, dev)
+    if ids.dtype is t.int64:             # ids that int32 cannot hold are no adapter's
+        ids = L.as_tensor(ids).clamp(-1, 0x7FFFFFFF).to(t.int32)
+    ids = _tensor(ids, "ids", t.int32, dev)
     if ids.numel() != T:
         raise ValueError(f"ids must name the adapter of each of the {T} tokens")
     return x, a, b, ids, scaling, dev, T, K, sb[1], n, R
