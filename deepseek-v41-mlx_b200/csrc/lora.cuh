@@ -412,7 +412,7 @@ struct LoraShrinkMaps {
 };
 
 constexpr int LS_THREADS = 160;
-constexpr int LS_BATCH = 4;
+constexpr int LS_BATCH = 2;
 constexpr int LS_X_BYTES = LR_TILE * LR_KB * 2;     // 16 KB
 
 // D[128 tokens x Rp] in TMEM: tcgen05.mma kind::f16, M = 128, N = Rp.  A cluster of C CTAs
@@ -543,10 +543,11 @@ __global__ void __launch_bounds__(LS_THREADS, 2)
       __syncwarp();
     }
     it += kb1 - kb0;
-    // ------------------------------------------------------------ the C partial sums: every
-    // thread sends its row to the CTA that adds that row, red[rank][row of the owner][Rp]
+    // ------------------------------------------------------------ the C partial sums: each CTA
+    // adds 128 / C rows, which it reads from the others' shared memories, neighbouring lanes along
+    // a row.  (Rows sent to their adder straight from TMEM, a lane a row, took 10 us at R 128.)
     float *red = reinterpret_cast<float *>(smem);
-    const int ld = a.Rp + 4, own = LR_TILE / C;      // rows a CTA adds
+    const int ld = a.Rp + 4, own = LR_TILE / C;
     const int q4 = a.Rp >> 2;
     const float sc = a.scaling ? a.scaling[tl.adapter] : 1.0f;
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -565,54 +566,60 @@ __global__ void __launch_bounds__(LS_THREADS, 2)
     if (warp < 4) {
       if (ok) ok = warp_wait(&acc_full, uint32_t(done) & 1u);
       tc_fence_after();
-    }
-    ++done;
-    cluster_sync();                       // nobody's stages are in use any more
-    if (warp < 4) {
-      const uint32_t to = mapa_rank(red + (rank * own + tid % own) * ld, tid / own);
       for (int c0 = 0; c0 < a.Rp; c0 += 32) {
         uint32_t v[32];
         tmem_ld32(tmem + (uint32_t(32 * warp) << 16) + c0, v);
+        float *dst = red + tid * ld + c0;
 #pragma unroll
         for (int e = 0; e < 32; e += 4)
           if (c0 + e < a.Rp)
-            asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (c0 + e) * 4),
-                         "r"(v[e]), "r"(v[e + 1]), "r"(v[e + 2]), "r"(v[e + 3])
-                         : "memory");
+            *reinterpret_cast<uint4 *>(dst + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
       }
       tc_fence_before();
     }
+    ++done;
     cluster_sync();
     tc_fence_after();
 #pragma unroll 1
     for (int e0 = tid; e0 < own * q4; e0 += LS_BATCH * LS_THREADS) {
       if (e0 != tid) load_h(e0);
+      float4 v[LS_BATCH][8];                         // all requests in flight
 #pragma unroll
       for (int u = 0; u < LS_BATCH; ++u) {
-        const int e = e0 + u * LS_THREADS;
-        const int lrow = e / q4, row = rank * own + lrow, c4 = (e % q4) * 4;
-        if (lrow >= own || row >= ((tl.rows + 63) & ~63)) break;
+        const int e = e0 + u * LS_THREADS, row = rank * own + e / q4, c4 = (e % q4) * 4;
+        const bool in = e < own * q4 && c4 < a.R && row < tl.rows;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          v[u][q] = zero;
+          if (in && q < C)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v[u][q].x), "=f"(v[u][q].y), "=f"(v[u][q].z), "=f"(v[u][q].w)
+                         : "r"(mapa_rank(red + row * ld + c4, q))
+                         : "memory");
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < LS_BATCH; ++u) {
+        const int e = e0 + u * LS_THREADS, row = rank * own + e / q4, c4 = (e % q4) * 4;
+        if (e >= own * q4 || row >= ((tl.rows + 63) & ~63)) break;
         const bool in = c4 < a.R && row < tl.rows;   // the padding of Rp and of the block: zeros
         float4 s = zero;
-        if (in)
-          for (int q = 0; q < C; ++q) {
-            const float4 v = *reinterpret_cast<const float4 *>(red + (q * own + lrow) * ld + c4);
-            s.x += v.x;
-            s.y += v.y;
-            s.z += v.z;
-            s.w += v.w;
-          }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {                // in rank order
+          s.x += v[u][q].x;
+          s.y += v[u][q].y;
+          s.z += v[u][q].z;
+          s.w += v[u][q].w;
+        }
         if (a.out && in) *reinterpret_cast<float4 *>(a.out + int64_t(rows_s[row]) * a.R + c4) = s;
         // (zeros are not scaled: an infinite scaling would make them NaN)
         store_parts(a.parts, a.np, a.Rp, tl.block, row, c4, s, in ? sc : 1.0f);
         if (a.h) store_parts(a.h_parts, a.np, a.Rp, tl.block, row, c4, hv[u], in ? sc : 1.0f);
       }
     }
-    __syncthreads();                      // before the stages are written again
-    // the copies' writes come after these reads and the peers' stores
+    cluster_sync();                       // the others have read; before the stages are written again
     fence_proxy_async_smem();
   }
-  cluster_sync();                         // no peer's stores are on their way
   tc_fence_before();
   __syncthreads();
   if (warp == 4) {
