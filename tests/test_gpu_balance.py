@@ -145,6 +145,49 @@ def test_ragged_sequences(cuda, T, S):
     assert (dz[out | ~mask] == 0).all()
 
 
+@pytest.mark.parametrize("T", [20, 4000])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_unaligned_rows(cuda, T, dtype):
+    g, z, idx, dw = _inputs(8, T, 96, 5, dtype)
+    flat = torch.empty(T * 96 + 1, dtype=dtype, device="cuda")
+    flat[1:] = z.reshape(-1)
+    _check(flat[1:].view(T, 96), idx, gl=torch.ones(1, device="cuda"), dw=dw)
+
+
+@pytest.mark.parametrize("k", [1, 3, 32, 33, 64])
+@pytest.mark.parametrize("func", FUNCS)
+def test_choices_repeated_and_missing(cuda, k, func):
+    """Any number of choices a token, with the same expert more than twice and with none."""
+    T, E = 300, 70
+    g, z, _, dw = _inputs(k, T, E, k)
+    idx = torch.randint(-2, 9, (T, k), generator=g, device="cuda").int()
+    idx[7] = -1
+    gl = torch.ones(1, device="cuda")
+    for norm in (True, False):
+        _check(z, idx, func=func, gl=gl, dw=dw, norm=norm)
+    mask = torch.rand(T, generator=g, device="cuda") > 0.4
+    _check(z, idx, mask=mask, func=func, dw=dw)
+
+
+def test_more_than_2_31_values(cuda):
+    """Offsets into the logits past 32 bits: the last rows' gradients against the formula."""
+    T, E, k = 2_150_000, 1000, 4
+    g = torch.Generator(device="cuda").manual_seed(2)
+    z = torch.randn(1000, E, generator=g, device="cuda").repeat(T // 1000, 1)
+    idx = torch.randint(0, E, (T, k), generator=g, device="cuda").int()
+    loss, cnt, dz = q.moe.balance_loss(z, idx, grad_loss=1e6)
+    assert _eq(cnt[0], torch.bincount(idx.reshape(-1).long(), minlength=E).int())
+    zl = z[-50:].to(D).requires_grad_(True)
+    s = _score(zl, "sqrtsoftplus")
+    p = s / (s.sum(1, keepdim=True) + 1e-20)
+    coef = 1e6 * E / (k * T * T)
+    want = torch.autograd.grad((p * cnt[0].to(D)).sum() * coef, zl)[0]
+    ds = torch.autograd.grad(_score(zl, "sqrtsoftplus").sum(), zl)[0]
+    # terms c and sum c p, each about T k / E times coef ds / sum s
+    mag = 2 * cnt[0].to(D).max() * coef * ds / s.sum(1, keepdim=True)
+    assert ((dz[-50:].to(D) - want).abs() <= 32 * 2.0 ** -24 * mag.detach()).all()
+
+
 @pytest.mark.parametrize("T", [60, 3000])
 @pytest.mark.parametrize("func", FUNCS)
 def test_padding_may_hold_anything(cuda, T, func):

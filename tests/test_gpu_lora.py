@@ -131,6 +131,72 @@ def test_forward_long_rows(cuda, shape):
     _check_forward(c, ids, None, F32, y, h)
 
 
+@pytest.mark.parametrize("kind", ["mixed", "runs", "none"])
+@pytest.mark.parametrize("shape", [(3000, 72, 33, 8, 2), (2500, 264, 130, 24, 5),
+                                   (1300, 1032, 200, 104, 9), (1100, 520, 256, 48, 1),
+                                   (1030, 8, 1, 8, 3), (2049, 4096, 64, 128, 2)], ids=str)
+def test_forward_many_tokens(cuda, shape, kind):
+    """Sorted tiles: ranks of every piece width, odd and single columns, short contractions."""
+    T, K, N, R, n = shape
+    c = _case(sum(shape), *shape)
+    ids = _ids(kind, T, n, c["g"])
+    for odt in (BF, F32):
+        base = _randn(c["g"], T, N, dtype=odt)
+        y, h = q.lora.lora_forward(c["x"], c["a"], c["b"], ids, c["s"], base, odt, return_h=True)
+        _check_forward(c, ids, base, odt, y, h)
+        y = q.lora.lora_forward(c["x"], c["a"], c["b"], ids, c["s"], out_dtype=odt)
+        _check_forward(c, ids, None, odt, y)
+
+
+@pytest.mark.parametrize("T", [3, 1500])
+def test_unaligned_base_and_output(cuda, T):
+    """Rows of base and the output may start at any element."""
+    c = _case(14, T, 256, 128, 16, 3)
+    ids = _ids("mixed", T, 3, c["g"])
+    dy = _randn(c["g"], T, 128)
+    _, h = q.lora.lora_forward(c["x"], c["a"], c["b"], ids, c["s"], return_h=True)
+    for dt in (BF, F32):
+        flat = _randn(c["g"], T * 128 + 1, dtype=dt)
+        base = flat[1:].view(T, 128)
+        want = q.lora.lora_forward(c["x"], c["a"], c["b"], ids, c["s"], base.clone(), dt)
+        assert _eq(q.lora.lora_forward(c["x"], c["a"], c["b"], ids, c["s"], base, dt), want)
+        out = torch.empty(T * 128 + 1, dtype=dt, device="cuda")[1:].view(T, 128)
+        q.lora.lora_forward(c["x"], c["a"], c["b"], ids, c["s"], base, dt, out=out)
+        assert _eq(out, want)
+        xb = _randn(c["g"], T * 256 + 1, dtype=dt)[1:].view(T, 256)
+        g1 = q.lora.lora_backward(dy, c["x"], h, c["a"], c["b"], ids, c["s"], xb, dt)
+        g2 = q.lora.lora_backward(dy, c["x"], h, c["a"], c["b"], ids, c["s"], xb.clone(), dt)
+        assert all(_eq(u, v) for u, v in zip(g1, g2))
+
+
+def test_more_than_2_31_values(cuda):
+    """Offsets into x, y and their gradients past 32 bits: rows at both ends against the formula."""
+    T, K, N, R, n = 300_000, 7200, 7208, 8, 2
+    g = torch.Generator(device="cuda").manual_seed(3)
+    c = dict(a=_randn(g, n, R, K, scale=K ** -0.5), b=_randn(g, n, N, R), g=g,
+             s=torch.ones(n, device="cuda"))
+    x = torch.randn(1000, K, generator=g, device="cuda").to(BF).repeat(T // 1000, 1)
+    ids = _ids("mixed", T, n, g)
+    y, h = q.lora.lora_forward(x, c["a"], c["b"], ids, c["s"], return_h=True)
+    rows = torch.cat([torch.arange(200), torch.arange(T - 200, T)]).cuda()
+    _check_forward(dict(c, x=x[rows]), ids[rows], None, BF, y[rows], h[rows])
+    dx, da, db = q.lora.lora_backward(y, x, h, c["a"], c["b"], ids, c["s"])
+    (dx64, _, _), (mag, _, _) = _backward64(dict(c, x=x[rows]), ids[rows], y[rows], h[rows], None)
+    tol = (2.0 ** -23 * 4 * N ** 0.5 + 2.0 ** -17) * mag + _half_step(BF) * dx64.abs() * 1.01
+    assert ((dx[rows].to(D) - dx64).abs() <= tol).all()
+    # db in slices of the tokens: sums of 1.5e5 terms, in fp32 partial sums of 64-token stages
+    want, mag = torch.zeros(n, N, R, dtype=D, device="cuda"), torch.zeros(n, N, R, device="cuda")
+    for t0 in range(0, T, 20000):
+        t = slice(t0, t0 + 20000)
+        for i in range(n):
+            k = torch.nonzero(ids[t] == i)[:, 0]
+            yi, hi = y[t][k], h[t][k]
+            want[i] += yi.to(D).T @ hi.to(D)
+            mag[i] += yi.float().abs().T @ hi.abs()
+    tol = (2.0 ** -23 * 4 * T ** 0.5 + 2.0 ** -17) * mag + _half_step(BF) * want.abs() * 1.01
+    assert ((db.to(D) - want).abs() <= tol).all()
+
+
 def test_forward_in_place_leading_shape_and_int64_ids(cuda):
     c = _case(9, 24, 256, 120, 16, 4)
     ids = _ids("mixed", 24, 4, c["g"])
