@@ -355,8 +355,16 @@ cudaError_t max_dynamic_smem(void (*kernel)(KArgs...), size_t bytes) {
       }
     }
   if (slot && slot->bytes[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
-  e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-  if (e == cudaSuccess && slot) slot->bytes[dev].store(bytes, std::memory_order_release);
+  // The attribute only ever grows: two threads on their first calls with different sizes would
+  // else leave the larger one's launch without its memory.
+  static std::mutex growing;
+  const std::lock_guard<std::mutex> lock(growing);
+  cudaFuncAttributes at;
+  e = cudaFuncGetAttributes(&at, f);
+  if (e == cudaSuccess && size_t(at.maxDynamicSharedSizeBytes) < bytes)
+    e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  if (e == cudaSuccess && slot && slot->bytes[dev].load(std::memory_order_relaxed) < bytes)
+    slot->bytes[dev].store(bytes, std::memory_order_release);
   return e;
 }
 

@@ -11,6 +11,7 @@ its type.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import pytest
 import torch
@@ -251,6 +252,41 @@ def test_non_finite_rows_stay_in_their_rows(cuda):
     y = q.lora.lora_forward(x2, c["a"], c["b"], ids, c["s"])
     rest = torch.arange(200, device="cuda") != 7
     assert _eq(y[rest], want[rest]) and not torch.isfinite(y[7]).all()
+
+
+def test_calls_from_several_threads(cuda):
+    """Each thread has a stream and sizes of its own; the results are those of calls in turn."""
+    jobs = []
+    for k, (T, R) in enumerate([(900, 128), (700, 16), (800, 64), (600, 32)]):
+        c = _case(40 + k, T, 264, 392, R, 5)
+        ids = _ids("mixed", T, 5, c["g"])
+        jobs.append((c, ids, _randn(c["g"], T, 392)))
+
+    def run(c, ids, dy):
+        y, h = q.lora.lora_forward(c["x"], c["a"], c["b"], ids, c["s"], return_h=True)
+        return (y, h) + q.lora.lora_backward(dy, c["x"], h, c["a"], c["b"], ids, c["s"])
+    got, errors = [[] for _ in jobs], []
+    start = threading.Barrier(len(jobs))
+    torch.cuda.synchronize()
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for _ in range(5):
+                    got[k].append(run(*jobs[k]))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                       # shown by the assertion below
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(jobs))]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors
+    for k, job in enumerate(jobs):
+        want = run(*job)
+        assert len(got[k]) == 5 and all(_eq(u, v) for r in got[k] for u, v in zip(r, want))
 
 
 def test_ids_past_the_bank_count_as_none(cuda):
