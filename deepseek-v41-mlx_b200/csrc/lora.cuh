@@ -971,6 +971,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
     const int row = 32 * q4 + lane;                      // this thread's row of the tile
     float *tp = reinterpret_cast<float *>(smem) + (warp - 6) * 32 * LE_EPI_LD;
     int all = 0, turn = 0, prev = -1;                    // blocks so far; the tile last stored
+    const uint32_t none = base ? 0x80000000u : 0u;       // no adapter's part: -0 leaves base as it is
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
       const int4 tl = a.plan.tiles[item / per_tile];
       const bool has = tl.x < a.n;
@@ -1017,7 +1018,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
               tmem_ld32(tacc + h, v);
             } else {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = 0u;
+              for (int e = 0; e < 32; ++e) v[e] = none;
             }
             if constexpr (sizeof(OT) == 4) {
 #pragma unroll
@@ -1108,7 +1109,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
             for (int r = 0; r < 32; ++r) {
               if (r % 8 == 0 && 32 * q4 + r >= tl.z) break;
               const int tk = __shfl_sync(0xffffffffu, tok, r);
-              float f = has ? tp[r * LE_EPI_LD + lane] : 0.0f;
+              float f = has ? tp[r * LE_EPI_LD + lane] : __uint_as_float(none);
               if (base) f += float(odd[VEC ? 0 : h / 32][r]);
               if (tk >= 0 && c < a.N) y[int64_t(tk) * a.N + c] = OT(f);
             }

@@ -198,8 +198,8 @@ int dsv41_gemv_affine(const void *x, int64_t M, int64_t K, const uint32_t *wq,
  * adapter get base (zeros when it is NULL).  h_out, if not NULL, receives h f32 [T, R] (zero
  * rows without an adapter) for the backward pass.  Sums are fp32, h is not rounded below 16
  * bits of mantissa, y is rounded once.  K a multiple of 8, R a multiple of 8 up to 128, n <=
- * 8192, T <= 2^30, N any; every tensor but y and the base 16-byte aligned, and the workspace.  An id at or past n counts as none and raises bit 1 of
- * dsv41_device_status.
+ * 8192, T <= 2^30, N any; every tensor but y, the base, ids and scaling 16-byte aligned, and the
+ * workspace.  An id at or past n counts as none and raises bit 1 of dsv41_device_status.
  *
  * dsv41_lora_backward: from dy bf16 [T, N], x and h of the forward pass, with g[t] =
  * scaling[i] * (dy[t] . b[i]):
@@ -249,8 +249,8 @@ int dsv41_moe_logits(const void *x, int64_t T, int64_t D, const void *gate_w, in
  * no sequence count nowhere, whatever they hold, and get zero gradients.  A row whose scores
  * are all zero (logits of -inf) adds nothing and gets a zero gradient from the loss.  loss f32
  * [S], counts int32 [S, E].  1 <= E <= 1024, 1 <= topk <= min(64, E).  An index at or past E
- * counts as no choice and raises bit 1 of dsv41_device_status.  The same bits every time.  T, S <= 2^30.
- * The workspace (8-byte aligned) may be NULL where its size is 0. */
+ * counts as no choice and raises bit 1 of dsv41_device_status.  The same bits every time.
+ * T, S <= 2^30.  The workspace (8-byte aligned) may be NULL where its size is 0. */
 size_t dsv41_moe_balance_workspace_size(int64_t T, int64_t E, int64_t S);
 int dsv41_moe_balance(const void *logits, int dtype, int64_t T, int64_t E, const int32_t *indices,
                       int topk, const int32_t *offsets, int64_t S, const uint8_t *mask,

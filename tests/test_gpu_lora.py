@@ -254,6 +254,19 @@ def test_non_finite_rows_stay_in_their_rows(cuda):
     assert _eq(y[rest], want[rest]) and not torch.isfinite(y[7]).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=str)
+@pytest.mark.parametrize("T, N", [(5, 64), (700, 64), (700, 65)])
+def test_rows_without_adapter_keep_every_bit_of_base(cuda, T, N, dtype):
+    c = _case(14, T, 64, N, 16, 3)
+    ids = _ids("mixed", T, 3, c["g"])
+    base = _randn(c["g"], T, N, dtype=dtype)
+    base[:, ::3] = -0.0
+    y = q.lora.lora_forward(c["x"], c["a"], c["b"], ids, c["s"], base=base)
+    bits = torch.int16 if dtype is BF else torch.int32
+    idle = ids < 0
+    assert idle.any() and _eq(y[idle].view(bits), base[idle].view(bits))
+
+
 def test_calls_from_several_threads(cuda):
     """Each thread has a stream and sizes of its own; the results are those of calls in turn."""
     jobs = []
