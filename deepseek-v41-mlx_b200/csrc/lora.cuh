@@ -765,10 +765,42 @@ struct LoraExpand {
   const void *base;            // [T, N] or NULL
   void *y;                     // [T, N]
   LoraPlan plan;
-  int ncb, cpu;                // column blocks of 128 bytes of a row, and how many (even) an item takes
+  int ncb;                     // column blocks of 128 bytes of a row; an MMA takes a pair
   int ring;                    // tiles of 128 rows x 128 bytes in shared memory (of LE_GROUPS)
   int abuf, wbuf;              // buffers of the parts and of W's column blocks
   int pw;                      // !WMN: see LoraPieces
+};
+
+// The work is one line, tile after tile, a tile's pairs of column blocks in order.  The CTAs go
+// along it in rounds of `turn` neighbouring pairs each; the last round shares what is left.  A
+// CTA's whole share at once, far from the other CTAs', reads DRAM worse; one pair at a time reloads
+// the parts for each: the square root of the share has the least of both.  (T 8192, N 14336, R 32,
+// 49 pairs a CTA: 115 us the call, 141 with 1, 124 with 49; T 4096, N 7168, R 128, 13 pairs: 47, 55
+// and 47 us.)  next() gives a CTA's stretches: column blocks [cb0, cb1) of one tile.
+struct LoraWalk {
+  int64_t work, at, end, round;
+  int ncb, turn, tile, cb0, cb1;
+  __device__ __forceinline__ explicit LoraWalk(const LoraExpand &a)
+      : work(int64_t(a.plan.head[0]) * ((a.ncb + 1) >> 1)), at(0), end(0), round(0), ncb(a.ncb) {
+    turn = max(1, int(rintf(sqrtf(float((work + gridDim.x - 1) / gridDim.x)))));
+  }
+  __device__ __forceinline__ bool next() {
+    while (at >= end) {
+      if (round >= work) return false;
+      const int64_t n = min(int64_t(turn), (work - round + gridDim.x - 1) / gridDim.x);
+      at = round + blockIdx.x * n;
+      end = min(at + n, work);
+      round += gridDim.x * n;
+    }
+    const int pairs = (ncb + 1) >> 1;
+    tile = int(at / pairs);
+    const int p = int(at - int64_t(tile) * pairs), q = int(min(int64_t(pairs), p + end - at));
+    cb0 = 2 * p;
+    cb1 = min(2 * q, ncb);
+    at += q - p;
+    return true;
+  }
+  __device__ __forceinline__ int pairs() const { return (cb1 - cb0 + 1) >> 1; }
 };
 struct LoraExpandMaps {
   LoraRows base, y;
@@ -785,16 +817,16 @@ constexpr int LE_EPI_LD = 36;                     // floats of a transposition r
 
 // D[128 tokens x MB columns] in TMEM (tcgen05.mma kind::f16; MB = 2 CB columns, CB are 128 bytes
 // of a row of y; with CB alone the MMAs of R = 128, which read the parts from shared memory every
-// time, took longer than the stores): the tile's parts are the A operand, contraction NS * Rp, staged once for a work item's
-// column blocks; a block of W is the B operand, in its own order in memory (rows of r for B,
-// columns contiguous for A: the MMA takes either).  base comes in through a ring of 16 KB tiles,
-// the epilogue adds the accumulators to it in place, a thread a row, and the tile goes out the
-// same way (128-byte swizzle: no bank conflicts); rows that follow one another move 16 an
-// instruction, others four.  Warps 0-3 fetch base, 4 issues the MMAs, 5 fetches W and the parts,
-// the others are three epilogues that take turns (one's turn is about 2500 cycles a tile: two fell
-// behind HBM).  Row-wise plain loads and stores, through a
-// transposition in shared memory, kept the load/store pipe busy for twice the time that HBM
-// needs (135 us at T 8192, N 14336, R 32).  Rows that TMA cannot address (VEC false: odd lengths)
+// time, took longer than the stores): the tile's parts are the A operand, contraction NS * Rp,
+// staged once for a stretch of column blocks; a block of W is the B operand, in its own order in
+// memory (rows of r for B, columns contiguous for A: the MMA takes either).  base comes in through
+// a ring of 16 KB tiles, the epilogue adds the accumulators to it in place, a thread a row, and
+// the tile goes out the same way (128-byte swizzle: no bank conflicts); rows that follow one
+// another move 16 an instruction, others four.  Warps 0-3 fetch base, 4 issues the MMAs, 5 fetches
+// W and the parts, the others are three epilogues that take turns (one's turn is about 2500 cycles
+// a tile: two fell behind HBM).  Row-wise plain loads and stores, through a transposition in shared
+// memory, kept the load/store pipe busy for twice the time that HBM needs (135 us at T 8192, N
+// 14336, R 32, against 79 us now: 5.9 TB/s).  Rows that TMA cannot address (VEC false: odd lengths)
 // are still moved that way, by a kernel of their own (in one kernel its unrolled rows pushed the
 // hot loop out of the instruction cache).
 template <bool WMN, typename OT, bool VEC>
@@ -851,16 +883,15 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
   const uint32_t tmem = tmem_slot;
   pdl_wait();                             // the parts
   pdl_trigger();
-  const int per_tile = (a.ncb + a.cpu - 1) / a.cpu, rg = a.Rp >> 3;
-  const int64_t items = int64_t(a.plan.head[0]) * per_tile;
+  const int rg = a.Rp >> 3;
+  LoraWalk st(a);
   bool ok = true;
-  int blk = 0, live = 0;          // column blocks (warps 4, 5: MMA blocks of live tiles), live items
+  int blk = 0, live = 0;          // column blocks (warps 4, 5: MMA blocks of live tiles), live stretches
   if (warp < 4) {
     // -------------------------------------------------------------- base, 32 rows a warp
     if (VEC && a.base) {
-      for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
-        const int4 tl = a.plan.tiles[item / per_tile];
-        const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
+      while (ok && st.next()) {
+        const int4 tl = a.plan.tiles[st.tile];
         int tok[2], rows[2];
         bool run[2];
         uint32_t tx = 0;
@@ -873,7 +904,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
           run[h] = rows[h] > 0 && last - __shfl_sync(0xffffffffu, tok[h], 0) == rows[h] - 1;
           tx += lora_rows_bytes(run[h], rows[h]);
         }
-        for (int cb = cb0; cb < cb1; ++cb, ++blk) {
+        for (int cb = st.cb0; cb < st.cb1; ++cb, ++blk) {
           const int s = blk % a.ring;
           if (!(ok = warp_wait(&b_empty[s], (uint32_t(blk / a.ring) & 1u) ^ 1u))) break;
           if (lane == 0) mbar_arrive_expect_tx(&b_full[s], tx);
@@ -893,14 +924,13 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
     const uint32_t id = idesc_lora(MB, 0, WMN ? 1 : 0);
     const LoraPieces pc(WMN ? CB : a.pw);
     const LoraSteps steps = WMN ? LoraSteps::mn(pc) : LoraSteps::k(pc, MB);
-    for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      if (a.plan.tiles[item / per_tile].x >= a.n) continue;
-      const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
+    while (ok && st.next()) {
+      if (a.plan.tiles[st.tile].x >= a.n) continue;
       const int ab = live % a.abuf;
       if (!(ok = warp_wait(&a_full[ab], uint32_t(live / a.abuf) & 1u))) break;
       ++live;
       const uint64_t da = sdesc(sa + ab * a_bytes, 2048, 128, 0);
-      for (int cb = cb0; cb < cb1; cb += 2, ++blk) {
+      for (int cb = st.cb0; cb < st.cb1; cb += 2, ++blk) {
         const int b = blk % LE_BUF, wb = blk % a.wbuf;
         if (!warp_wait(&acc_empty[b], (uint32_t(blk / LE_BUF) & 1u) ^ 1u) ||
             !warp_wait(&w_full[wb], uint32_t(blk / a.wbuf) & 1u)) {
@@ -929,10 +959,9 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
     __syncwarp();
   } else if (warp == 5) {
     // -------------------------------------------------------------- W and the parts
-    for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const int4 tl = a.plan.tiles[item / per_tile];
+    while (ok && st.next()) {
+      const int4 tl = a.plan.tiles[st.tile];
       if (tl.x >= a.n) continue;
-      const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
       // two 64-row blocks of parts (the second may be another adapter's: its rows reach only
       // accumulator rows that nobody reads)
       const int ab = live % a.abuf;
@@ -943,7 +972,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
 #pragma unroll
       for (int i = 0; i < NS; ++i)
         tma_load_3d_el(sa + ab * a_bytes + i * a.Rp * 256, &maps.parts, &a_full[ab], 0, tl.w, i * rg);
-      for (int cb = cb0; cb < cb1; cb += 2, ++blk) {
+      for (int cb = st.cb0; cb < st.cb1; cb += 2, ++blk) {
         const int b = blk % a.wbuf;
         if (!(ok = warp_wait(&w_empty[b], (uint32_t(blk / a.wbuf) & 1u) ^ 1u))) break;
         const uint32_t dw = sw + b * w_bytes;
@@ -972,10 +1001,10 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
     float *tp = reinterpret_cast<float *>(smem) + (warp - 6) * 32 * LE_EPI_LD;
     int all = 0, turn = 0, prev = -1;                    // blocks so far; the tile last stored
     const uint32_t none = base ? 0x80000000u : 0u;       // no adapter's part: -0 leaves base as it is
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-      const int4 tl = a.plan.tiles[item / per_tile];
+    while (st.next()) {
+      const int4 tl = a.plan.tiles[st.tile];
       const bool has = tl.x < a.n;
-      const int cb0 = int(item % per_tile) * a.cpu, cb1 = min(cb0 + a.cpu, a.ncb);
+      const int cb0 = st.cb0, cb1 = st.cb1;
       const int tok = row < tl.z ? a.plan.perm[tl.y + row] : -1;
       for (int cb = cb0; cb < cb1; ++cb, ++all, turn = turn == LE_GROUPS - 1 ? 0 : turn + 1) {
         if (turn != grp) continue;
@@ -1125,7 +1154,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
           }
         }
       }
-      if (has) blk += (cb1 - cb0 + 1) >> 1;
+      if (has) blk += st.pairs();
     }
     bulk_wait_el();
   }
