@@ -11,7 +11,7 @@
 //   ds_ij += scale / (sum_l s_il + 1e-20) (dw_j - sum_l dw_l w_l / scale).
 // The counts come first (they need the choices alone); then sum_e c_e p_te serves the loss and
 // the gradient alike, so one pass over the logits gives both: each row is read once and, with a
-// gradient, written once, and the bound is HBM.  Sums over a sequence's tokens are doubles.
+// gradient, written once.  Sums over a sequence's tokens are doubles.
 #pragma once
 #include "bsgemm.cuh"
 #include "common.cuh"
@@ -572,6 +572,8 @@ __device__ __forceinline__ float balance_scale(const BalArgs &p, double sum, int
 // A run of tokens a warp, its row of the next token in flight while it works on one.  The sum
 // of a run's tokens of sequence q goes to part[run index + q]: runs and sequences both ascend
 // with the tokens, so no two share a place.  The last CTA adds each sequence's places in order.
+// T 65536, E 384, k 6, fp32 with both gradients: 72 us, 2.8 TB/s, bound by instructions (an
+// element takes about 50, three of them special functions; 56% of the issue slots) and their latency.
 template <typename IT, int NP, int VEC, bool GRAD, int FUNC>
 __global__ void __launch_bounds__(32 * BL_WARPS, NP <= 4 ? 3 : NP <= 8 ? 2 : 1)
     k_balance(const BalArgs p) {

@@ -24,6 +24,7 @@
 #include "aqgemm.cuh"
 #include "bsgemm.cuh"
 #include "common.cuh"
+#include <type_traits>
 
 namespace dsv41 {
 
@@ -77,7 +78,8 @@ __device__ __forceinline__ void block_scan3(int (&v)[3], int (&tot)[3], int (*ws
 // One cluster of 1024-thread CTAs, each on a contiguous slice of the tokens: histogram in
 // shared memory, the other CTAs' histograms over distributed shared memory, one scan over the
 // adapters, then the stable scatter (warps of a 1024-token batch in order).  One launch; sorting
-// through global memory would take three.
+// through global memory would take three.  6 to 8 us for 500 to 8192 tokens, a chain of latencies:
+// ids, the cluster's meeting, scan, scatter.
 constexpr int LP_MAX_CTAS = 8;
 __global__ void __launch_bounds__(1024, 1)
     k_lora_plan(const int32_t *__restrict__ ids, int T, int n, LoraPlan p) {
@@ -420,7 +422,8 @@ constexpr int LS_X_BYTES = LR_TILE * LR_KB * 2;     // 16 KB
 // shared memory and are added in rank order.  Warps 0-3 fetch 32 token rows each, 64 values a
 // stage, warp 0 also the adapter's values, all by TMA; warp 4 issues the MMAs.  (Both went
 // through cp.async first: 512 bytes cost about 20 shared-memory cycles that way, which all but
-// caps an SM at its share of HBM.)  What stands in the rows past the tile's only reaches
+// caps an SM at its share of HBM.)  T 8192, K 7168, R 32: 26 us, 4.5 TB/s, of which some 7 are the
+// start behind the plan and the join.  What stands in the rows past the tile's only reaches
 // accumulator rows that nobody reads.  Rows that TMA cannot address, of odd lengths, are staged
 // by the threads.
 template <bool WMN, bool VEC, int S>
@@ -655,7 +658,8 @@ __device__ __forceinline__ float dot8(uint4 u, uint4 v, float acc) {
 // of K (its warps R / 8 ranks each), the partial h meet in distributed shared memory in rank
 // order, then each CTA takes a slice of the columns, a row of B per group of LPR lanes.  The
 // first rows of B are requested before the cluster meets.  Bound by the latency of one pass
-// over an adapter (360 KB at K 7168, N 4096, R 16), which tokens on the same adapter find in L2.
+// over an adapter (360 KB at K 7168, N 4096, R 16: 7 us for one token, 10 us for 64), which tokens
+// on the same adapter find in L2.
 // TH threads; RW: ranks a warp; LPR: lanes a row of B, the power of two at or above R / 8.
 template <typename OT, int TH, int RW, int LPR>
 __global__ void __launch_bounds__(TH) k_lora_decode(const LoraDecode p) {
@@ -827,8 +831,8 @@ constexpr int LE_EPI_LD = 36;                     // floats of a transposition r
 // a tile: two fell behind HBM).  Row-wise plain loads and stores, through a transposition in shared
 // memory, kept the load/store pipe busy for twice the time that HBM needs (135 us at T 8192, N
 // 14336, R 32, against 79 us now: 5.9 TB/s).  Rows that TMA cannot address (VEC false: odd lengths)
-// are still moved that way, by a kernel of their own (in one kernel its unrolled rows pushed the
-// hot loop out of the instruction cache).
+// are still moved that way, by a kernel of their own (in one kernel its rows pushed the hot loop
+// out of the instruction cache).
 template <bool WMN, typename OT, bool VEC>
 __global__ void __launch_bounds__(LE_THREADS, 1)
     k_lora_expand(const __grid_constant__ LoraExpandMaps maps, const LoraExpand a) {
@@ -1022,18 +1026,21 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
           // a warp whose wait ran out goes on without waiting
           if (base && ok) ok = warp_wait(&b_full[s], uint32_t(all / a.ring) & 1u);
         }
-        OT odd[VEC ? 1 : CB / 32][32];                     // base, a row a register
-        if (!VEC && base) {
+        // odd rows: 16 rows of 32 columns at a time, a lane a column, the first ones of base ahead
+        // of the wait
+        using Bits = std::conditional_t<sizeof(OT) == 4, uint32_t, uint16_t>;
+        Bits odd[VEC ? 1 : 16];
+        const int64_t col = int64_t(cb) * CB + lane;
+        auto load_odd = [&](int64_t c, int r0) {           // (missing rows and columns read others')
+          const Bits *from = reinterpret_cast<const Bits *>(base) + min(c, a.N - 1);
+          const int any = __shfl_sync(0xffffffffu, tok, 0);
+          if (base && any >= 0) {
 #pragma unroll
-          for (int h = 0; h < (VEC ? 1 : CB / 32); ++h)
-#pragma unroll
-            for (int r = 0; r < 32; ++r) {
-              if (r % 8 == 0 && 32 * q4 + r >= tl.z) break;        // only rows that are there
-              const int tk = __shfl_sync(0xffffffffu, tok, r);
-              const int64_t c = int64_t(cb) * CB + h * 32 + lane;
-              odd[h][r] = tk >= 0 && c < a.N ? base[int64_t(tk) * a.N + c] : OT(0.0f);
-            }
-        }
+            for (int r = 0; r < (VEC ? 1 : 16); ++r)
+              odd[r] = from[int64_t(max(__shfl_sync(0xffffffffu, tok, r0 + r), any)) * a.N];
+          }
+        };
+        if (!VEC) load_odd(col, 0);
         if (has) {
           if (ok) ok = warp_wait(&acc_full[b], uint32_t(mb / LE_BUF) & 1u);
           tc_fence_after();
@@ -1121,8 +1128,11 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
           bulk_commit_el();
           prev = s;
         } else {
-          // rows that start anywhere: 32 x 32 pieces turned in shared memory, a lane a column
-#pragma unroll
+          // rows that start anywhere: 32 x 32 pieces turned in shared memory.  (Loads without a
+          // condition, 16 in flight, in loops that stay small: unrolled over all rows, each load
+          // behind a test, T 4000, N 5884 took 172 us, now 71.)
+          const int rows = min(32, tl.z - 32 * q4);
+#pragma unroll 1
           for (int h = 0; h < CB; h += 32) {
             if (has) {
               uint32_t v[32];
@@ -1133,14 +1143,31 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
                     make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
             }
             __syncwarp();
-            const int64_t c = int64_t(cb) * CB + h + lane;
+            const int64_t c = col + h;
+#pragma unroll 1
+            for (int r0 = 0; r0 < 32; r0 += 16) {
+              float f[16];
+              if (has) {
 #pragma unroll
-            for (int r = 0; r < 32; ++r) {
-              if (r % 8 == 0 && 32 * q4 + r >= tl.z) break;
-              const int tk = __shfl_sync(0xffffffffu, tok, r);
-              float f = has ? tp[r * LE_EPI_LD + lane] : __uint_as_float(none);
-              if (base) f += float(odd[VEC ? 0 : h / 32][r]);
-              if (tk >= 0 && c < a.N) y[int64_t(tk) * a.N + c] = OT(f);
+                for (int r = 0; r < 16; ++r) f[r] = tp[(r0 + r) * LE_EPI_LD + lane];
+              } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) f[r] = __uint_as_float(none);
+              }
+              if (base) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                  f[r] += sizeof(OT) == 4 ? __uint_as_float(odd[VEC ? 0 : r])
+                                          : __uint_as_float(uint32_t(odd[VEC ? 0 : r]) << 16);
+              }
+              if (r0 == 0 && rows > 16) load_odd(c, 16);
+              else if (h + 32 < CB && r0 + 16 >= rows) load_odd(c + 32, 0);
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const int tk = __shfl_sync(0xffffffffu, tok, r0 + r);
+                if (tk >= 0 && c < a.N) y[int64_t(tk) * a.N + c] = OT(f[r]);
+              }
+              if (r0 + 16 >= rows) break;
             }
             __syncwarp();
           }
@@ -1280,7 +1307,8 @@ __device__ __forceinline__ void lora_wgrad_store(const LoraGradSide &sd, OT *out
 // arrive did that first: 17 us of one CTA's time behind 41 us of work at T 8192, R 64).  Warps
 // 0-3 fetch v's rows (missing ones repeat one of the adapter's own, against zero rows of u) and
 // u's block, each every fourth stage; 4 issues the MMAs, 5-8 read TMEM; accumulators are
-// double-buffered, so an item's stores overlap the next one.
+// double-buffered, so an item's stores overlap the next one.  T 8192, K 7168, N 4096, R 64: 38 us,
+// 4.9 TB/s (pieces of 256 bytes a row, and u once for every 128 columns), and 7 us the join.
 template <typename OT, int S>
 __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_wgrad(
     const __grid_constant__ LoraWgradMaps maps, const LoraWgrad a) {
