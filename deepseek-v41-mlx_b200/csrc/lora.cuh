@@ -1306,13 +1306,20 @@ __device__ __forceinline__ void lora_wgrad_store(const LoraGradSide &sd, OT *out
 // as fp32 partial sums, at most two per CTA, which k_lora_join adds in order (the last CTA to
 // arrive did that first: 17 us of one CTA's time behind 41 us of work at T 8192, R 64).  Warps
 // 0-3 fetch v's rows (missing ones repeat one of the adapter's own, against zero rows of u) and
-// u's block, each every fourth stage; 4 issues the MMAs, 5-8 read TMEM; accumulators are
+// u's block, the stages dealt in turn to four of them, or to three where the ring has three stages
+// (see P); 4 issues the MMAs, 5-8 read TMEM; accumulators are
 // double-buffered, so an item's stores overlap the next one.  T 8192, K 7168, N 4096, R 64: 38 us,
 // 4.9 TB/s (pieces of 256 bytes a row, and u once for every 128 columns), and 7 us the join.
 template <typename OT, int S>
 __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_wgrad(
     const __grid_constant__ LoraWgradMaps maps, const LoraWgrad a) {
   constexpr int NS = sizeof(OT) == 4 ? 3 : 2;
+  // Warps that deal the stages.  A dealer goes from stage i to stage i + P, whose slot it may have
+  // once stage i + P - S is released.  The wait's one-bit parity tells that release from the slot's
+  // previous one, stage i + P - 2 S, only if that one is known to be over: it is, since the dealer
+  // has waited for stage i - S and releases come in order, as long as P <= S.
+  constexpr int P = S < 4 ? S : 4;
+  static_assert(P <= S, "the parities of the ring's waits would be ambiguous");
   extern __shared__ uint8_t lg_raw[];
   uint8_t *smem = lg_raw + ((1024u - (smem_u32(lg_raw) & 1023u)) & 1023u);
   const uint32_t sx = smem_u32(smem), su = sx + S * LG_X_BYTES;
@@ -1365,15 +1372,15 @@ __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_w
       const int64_t C = sd.C;
       const __nv_bfloat16 *u = sd.u + int64_t(a.plan.stages[sg.adapter] + sg.first) * a.np * a.Rp * 64;
       const int c0 = sg.cb * LG_COLS;
-      // every fourth stage is this warp's; its 64 rows as two tokens a lane, one turn ahead
-      int q = (warp - it) & 3;
+      // every P-th stage is this warp's; its 64 rows as two tokens a lane, one turn ahead
+      int q = warp < P ? (warp + P - it % P) % P : sg.count;
       int tn0 = a.plan.perm[min(p0 + q * LR_KB + lane, pn - 1)];
       int tn1 = a.plan.perm[min(p0 + q * LR_KB + 32 + lane, pn - 1)];
-      for (; q < sg.count; q += 4) {
+      for (; q < sg.count; q += P) {
         const int i = it + q, st = i % S;
         const int tok[2] = {tn0, tn1};
-        tn0 = a.plan.perm[min(p0 + (q + 4) * LR_KB + lane, pn - 1)];
-        tn1 = a.plan.perm[min(p0 + (q + 4) * LR_KB + 32 + lane, pn - 1)];
+        tn0 = a.plan.perm[min(p0 + (q + P) * LR_KB + lane, pn - 1)];
+        tn1 = a.plan.perm[min(p0 + (q + P) * LR_KB + 32 + lane, pn - 1)];
         if (!(ok = warp_wait(&empty[st], (uint32_t(i / S) & 1u) ^ 1u))) break;
         const uint32_t dv = sx + st * LG_X_BYTES;
         const int left = pn - p0 - q * LR_KB;              // rows of the adapter from here on

@@ -364,6 +364,30 @@ def test_backward(cuda, shape, kind):
         assert all(_eq(u, v) for u, v in zip(got, again))
 
 
+# the weight gradients' ring has 5, 4, 6, 5, 4 stages for these ranks with bf16 gradients and
+# 5, 6, 5, 4, 3, 3, 3 with fp32
+@pytest.mark.parametrize("N", [1000, 1001])
+@pytest.mark.parametrize("kind, n", [("one", 1), ("mixed", 3)])
+@pytest.mark.parametrize("R, dt", [(16, BF), (32, BF), (64, BF), (96, BF), (128, BF), (8, F32),
+                                   (32, F32), (64, F32), (96, F32), (104, F32), (112, F32),
+                                   (128, F32)], ids=str)
+def test_backward_pieces_of_many_rings(cuda, R, dt, kind, n, N):
+    """13 stages of 64 tokens a CTA or more: every slot of its ring is used more than twice."""
+    T, K = 14000, 2048
+    c = _case(R + N + n, T, K, N, R, n)
+    ids = _ids(kind, T, n, c["g"])
+    dy, h = _randn(c["g"], T, N), _randn(c["g"], T, R, dtype=F32)
+    got = q.lora.lora_backward(dy, c["x"], h, c["a"], c["b"], ids, c["s"], None, dt, dt)
+    want, mag = _backward64(c, ids, dy, h, None)
+    parts = 2.0 ** -17 if dt is BF else 0.0      # fp32 results keep all of g's and h's 24 bits
+    for g, w, m, terms in zip(got, want, mag, (N + R, N + T, T)):
+        tol = (2.0 ** -23 * 4 * terms ** 0.5 + parts) * m + _half_step(dt) * w.abs() * 1.01
+        assert ((g.to(D) - w).abs() <= tol + 1e-30).all()
+    for _ in range(3):
+        again = q.lora.lora_backward(dy, c["x"], h, c["a"], c["b"], ids, c["s"], None, dt, dt)
+        assert all(_eq(u, v) for u, v in zip(got, again))
+
+
 def test_gradients_by_differences(cuda):
     """d sum(y * dy) / d(x, a, b) along a direction, from two forward passes.  y is linear in
     each of x, a and b, so the difference quotient is exact but for rounding."""
