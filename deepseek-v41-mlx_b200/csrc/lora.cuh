@@ -1004,7 +1004,6 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
     const int row = 32 * q4 + lane;                      // this thread's row of the tile
     float *tp = reinterpret_cast<float *>(smem) + (warp - 6) * 32 * LE_EPI_LD;
     int all = 0, turn = 0, prev = -1;                    // blocks so far; the tile last stored
-    const uint32_t none = base ? 0x80000000u : 0u;       // no adapter's part: -0 leaves base as it is
     while (st.next()) {
       const int4 tl = a.plan.tiles[st.tile];
       const bool has = tl.x < a.n;
@@ -1046,16 +1045,18 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
           tc_fence_after();
         }
         if constexpr (VEC) {
+          // (no adapter: the tile of base goes out as it came, every bit of it, or zeros)
           uint8_t *trow = smem + s * LE_TILE_BYTES + row * 128;
+          if (!has && !base) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              *reinterpret_cast<uint4 *>(trow + ((k ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+          }
 #pragma unroll
           for (int h = 0; h < CB; h += 32) {
+            if (!has) break;
             uint32_t v[32];
-            if (has) {
-              tmem_ld32(tacc + h, v);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = none;
-            }
+            tmem_ld32(tacc + h, v);
             if constexpr (sizeof(OT) == 4) {
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
@@ -1147,25 +1148,27 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
 #pragma unroll 1
             for (int r0 = 0; r0 < 32; r0 += 16) {
               float f[16];
-              if (has) {
+              // (no adapter: base's bits alone, or zeros)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) f[r] = tp[(r0 + r) * LE_EPI_LD + lane];
-              } else {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) f[r] = __uint_as_float(none);
-              }
+              for (int r = 0; r < 16; ++r) f[r] = has ? tp[(r0 + r) * LE_EPI_LD + lane] : 0.0f;
               if (base) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                  f[r] += sizeof(OT) == 4 ? __uint_as_float(odd[VEC ? 0 : r])
-                                          : __uint_as_float(uint32_t(odd[VEC ? 0 : r]) << 16);
+                for (int r = 0; r < 16; ++r) {
+                  const uint32_t in = odd[VEC ? 0 : r];
+                  const float o = __uint_as_float(sizeof(OT) == 4 ? in : in << 16);
+                  f[r] = has ? f[r] + o : o;
+                }
               }
               if (r0 == 0 && rows > 16) load_odd(c, 16);
               else if (h + 32 < CB && r0 + 16 >= rows) load_odd(c + 32, 0);
 #pragma unroll
               for (int r = 0; r < 16; ++r) {
                 const int tk = __shfl_sync(0xffffffffu, tok, r0 + r);
-                if (tk >= 0 && c < a.N) y[int64_t(tk) * a.N + c] = OT(f[r]);
+                const Bits raw = Bits(__float_as_uint(f[r]) >> (32 - 8 * sizeof(OT)));
+                const OT o = OT(f[r]);
+                if (tk >= 0 && c < a.N)
+                  reinterpret_cast<Bits *>(y)[int64_t(tk) * a.N + c] =
+                      has ? *reinterpret_cast<const Bits *>(&o) : raw;
               }
               if (r0 + 16 >= rows) break;
             }

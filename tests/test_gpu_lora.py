@@ -267,6 +267,36 @@ def test_rows_without_adapter_keep_every_bit_of_base(cuda, T, N, dtype):
     assert idle.any() and _eq(y[idle].view(bits), base[idle].view(bits))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=str)
+@pytest.mark.parametrize("T, N", [(5, 64), (5, 65), (3000, 64), (3000, 65)])
+def test_rows_without_adapter_keep_nan_payloads(cuda, T, N, dtype):
+    """Few tokens and sorted tiles alike: base's NaN of both kinds, infinities and zeros of both
+    signs come out as they are, and zeros where there is no base."""
+    c = _case(15, T, 64, N, 16, 3)
+    ids = _ids("mixed", T, 3, c["g"])
+    ids[0], ids[T // 2:] = -1, -1                  # whole tiles without an adapter among them
+    bits, shift = (torch.int16, 0) if dtype is BF else (torch.int32, 16)
+    words = [0x7F81, 0x7FC5, 0x7F80, 0x0000, 0x7FFF, 0x0001, 0x3F80]
+    words = [w << shift | (3 if shift and w & 0x7F else 0) for w in words]
+    top = 16 + shift
+    words += [w - (1 << (top - 1)) for w in words]     # the same with the sign bit
+    base = torch.tensor(words, dtype=bits, device="cuda").repeat(T * N // len(words) + 1)
+    base = base[:T * N].view(T, N).view(dtype)
+    idle = ids < 0
+    y = q.lora.lora_forward(c["x"], c["a"], c["b"], ids, c["s"], base=base)
+    assert _eq(y[idle].view(bits), base[idle].view(bits))
+    y = base.clone()
+    q.lora.lora_forward(c["x"], c["a"], c["b"], ids, c["s"], base=y, out=y)
+    assert _eq(y[idle].view(bits), base[idle].view(bits))
+    y = q.lora.lora_forward(c["x"], c["a"], c["b"], ids, c["s"], out_dtype=dtype)
+    assert (y[idle].view(bits) == 0).all()
+    dy, h = _randn(c["g"], T, N), _randn(c["g"], T, 16, dtype=F32)
+    xb = torch.tensor(words, dtype=bits, device="cuda").repeat(T * 64 // len(words) + 1)
+    xb = xb[:T * 64].view(T, 64).view(dtype)
+    dx = q.lora.lora_backward(dy, c["x"], h, c["a"], c["b"], ids, c["s"], xb)[0]
+    assert _eq(dx[idle].view(bits), xb[idle].view(bits))
+
+
 def test_calls_from_several_threads(cuda):
     """Each thread has a stream and sizes of its own; the results are those of calls in turn."""
     jobs = []
