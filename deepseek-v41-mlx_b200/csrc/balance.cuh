@@ -349,6 +349,15 @@ __device__ __forceinline__ void balance_tokens(const BalArgs &p, int64_t t0, int
           if (bal_elem<VEC>(i, h, lane) < E) mx = fmaxf(mx, row.at(i, h));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (mx == -INFINITY) {                         // (fmaxf passes over NaN: a row of nothing else)
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (bal_elem<VEC>(i, h, lane) < E) nan |= isnan(row.at(i, h));
+        if (__any_sync(0xffffffffu, nan)) mx = __int_as_float(0x7FFFFFFF);
+      }
       mx *= p.inv_temp;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {

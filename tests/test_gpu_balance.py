@@ -233,6 +233,30 @@ def test_extreme_logits(cuda, func):
     assert torch.isnan(loss).all() and rows[9] and int(rows.sum()) == 1
 
 
+@pytest.mark.parametrize("T", [60, 3000])
+@pytest.mark.parametrize("E, k", [(64, 4), (33, 4), (64, 40)])
+@pytest.mark.parametrize("func", FUNCS)
+def test_a_row_of_nan_is_seen(cuda, func, E, k, T):
+    """A live token whose logits are all NaN, or NaN and -inf, makes its sequence's loss and its own
+    gradient NaN; the other sequences and rows keep their bits."""
+    g, z, idx, dw = _inputs(T + E, T, E, k)
+    offsets = torch.tensor([0, T // 2, T], dtype=torch.int32, device="cuda")
+    gl = torch.ones(2, device="cuda")
+    z2 = z.clone()
+    z2[9] = float("nan")
+    z2[11] = float("-inf")
+    z2[11, E - 1] = float("nan")
+    rest = torch.ones(T, dtype=torch.bool, device="cuda")
+    rest[9] = rest[11] = False
+    for kw in (dict(), dict(grad_loss=gl), dict(dweights=dw), dict(grad_loss=gl, dweights=dw)):
+        want = q.moe.balance_loss(z, idx, offsets, score_func=func, **kw)
+        loss, cnt, dz = q.moe.balance_loss(z2, idx, offsets, score_func=func, **kw)
+        assert torch.isnan(loss[0]) and loss[1] == want[0][1] and _eq(cnt, want[1])
+        if kw:
+            assert torch.isnan(dz[9]).all() and torch.isnan(dz[11]).any()
+            assert _eq(dz[rest], want[2][rest])
+
+
 def test_same_expert_twice_and_missing_choices(cuda):
     T, E, k = 500, 40, 5
     g, z, _, dw = _inputs(4, T, E, k)
