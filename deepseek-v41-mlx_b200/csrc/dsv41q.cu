@@ -748,9 +748,16 @@ constexpr int64_t BL_SMALL_T = 128;
 bool balance_is_small(int64_t T, int64_t E, int64_t S) {
   return T > 0 && T <= BL_SMALL_T && S * E <= BL_SMALL_INTS;
 }
-// Tokens of a warp's run: as many CTAs as run at once share the tokens.
-int64_t balance_run(int64_t T, int64_t E) {
-  const int64_t ctas = (E <= 256 ? 3 : E <= 512 ? 2 : 1) * int64_t(num_sms());
+// Rows that move in pieces of four values (see balance_rows)
+bool balance_vec(const BalArgs &p, size_t esize) {
+  return p.E % 4 == 0 && aligned(p.logits, 4 * esize) && aligned(p.dlogits, 4 * esize);
+}
+// Tokens of a warp's run: as many CTAs as run at once share the tokens, by the registers of the
+// kernel that takes such rows (k_balance's launch bounds).  Rows in single values have one CTA an SM
+// at any E.  (T 5000, E 383, fp32, both gradients: 37.0 us cut for two CTAs an SM, 30.8 for one; T
+// 65536, E 33: 215 us cut for three, 207 for one.)
+int64_t balance_run(int64_t T, int64_t E, bool vec) {
+  const int64_t ctas = (!vec ? 1 : E <= 256 ? 3 : E <= 512 ? 2 : 1) * int64_t(num_sms());
   return std::max<int64_t>(1, ceil_div(T, ctas * BL_WARPS));
 }
 // Choices up to which one cluster counts them all (it needs no zeroed memory; beyond, its eight SMs'
@@ -778,7 +785,7 @@ cudaError_t balance_small_go(const BalArgs &p, const BalShape &sh, cudaStream_t 
 // of 8, 12, 16 or 32 values.  Few tokens: the largest size for all (its empty pairs are skipped).
 template <typename IT, bool GRAD, int FUNC>
 cudaError_t balance_rows(const BalArgs &p, const BalShape &sh, cudaStream_t st) {
-  const bool vec = p.E % 4 == 0 && aligned(p.logits, 4 * sizeof(IT)) && aligned(p.dlogits, 4 * sizeof(IT));
+  const bool vec = balance_vec(p, sizeof(IT));
   if (sh.cluster)
     return vec ? balance_small_go<IT, 16, 4, GRAD, FUNC>(p, sh, st)
                : balance_small_go<IT, 16, 1, GRAD, FUNC>(p, sh, st);
@@ -803,7 +810,8 @@ cudaError_t balance_launch(const BalArgs &p, const BalShape &sh, cudaStream_t st
 
 extern "C" size_t dsv41_moe_balance_workspace_size(int64_t T, int64_t E, int64_t S) {
   if (T < 0 || E <= 0 || S < 0 || balance_is_small(T, E, S)) return 0;
-  return align_up(size_t(S + 1) * 4, 256) + size_t(ceil_div(T, balance_run(T, E)) + S) * 8 + 256;
+  // (the rows' alignment is not known here: the shorter runs are the more)
+  return align_up(size_t(S + 1) * 4, 256) + size_t(ceil_div(T, balance_run(T, E, true)) + S) * 8 + 256;
 }
 
 extern "C" int dsv41_moe_balance(const void *logits, int dtype, int64_t T, int64_t E,
@@ -848,7 +856,7 @@ extern "C" int dsv41_moe_balance(const void *logits, int dtype, int64_t T, int64
     DSV41_REQUIRE(aligned(workspace, 8), DSV41_ERR_MISALIGNED, "workspace must be 8-byte aligned");
     WsCarve ws{static_cast<uint8_t *>(workspace), workspace_bytes, 0};
     p.live = ws.take<int>(S + 1);
-    p.run = int(balance_run(T, E));
+    p.run = int(balance_run(T, E, balance_vec(p, dtype == DSV41_F32 ? 4 : 2)));
     p.part = ws.take<double>(ceil_div(T, p.run) + S);
     sh.grid = unsigned(ceil_div(ceil_div(T, p.run), BL_WARPS));
     sh.smem = add;
