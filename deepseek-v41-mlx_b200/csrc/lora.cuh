@@ -463,6 +463,7 @@ __global__ void __launch_bounds__(LS_THREADS, 2)
   const int kb0 = int(int64_t(nkb) * rank / C), kb1 = int(int64_t(nkb) * (rank + 1) / C);
   const int ntiles = a.plan.head[0];
   int it = 0, done = 0;                   // stages and tiles so far (barrier parities)
+  int sent = 0;                           // stages that this warp's copies were issued for
   bool ok = true;                         // no wait of this thread has run out
   for (int i = int(cluster_id_x()); i < ntiles; i += int(ncluster_x())) {
     const int4 tv = a.plan.tiles[i];
@@ -520,6 +521,7 @@ __global__ void __launch_bounds__(LS_THREADS, 2)
               tma_load_3d_el(dw + r * 128, &maps.w, &full[s], r, kb * LR_KB, tl.adapter);
           }
         }
+        sent = jt + 1;
       }
     } else {
       // ------------------------------------------------------------ MMA issuer
@@ -542,7 +544,7 @@ __global__ void __launch_bounds__(LS_THREADS, 2)
                          (kb > kb0 || k) ? 1u : 0u);
         tc_commit_el(&empty[s]);
       }
-      if (ok) tc_commit_el(&acc_full);
+      tc_commit_el(&acc_full);            // (after a wait that ran out too: TMEM outlives the MMAs)
       __syncwarp();
     }
     it += kb1 - kb0;
@@ -623,6 +625,8 @@ __global__ void __launch_bounds__(LS_THREADS, 2)
     cluster_sync();                       // the others have read; before the stages are written again
     fence_proxy_async_smem();
   }
+  // the last copies have landed before the CTA can end, after a wait that ran out too (bounded)
+  for (int e = max(0, sent - S); e < sent; ++e) warp_wait(&full[e % S], uint32_t(e / S) & 1u);
   tc_fence_before();
   __syncthreads();
   if (warp == 4) {
@@ -844,7 +848,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
   const uint32_t s_ring = smem_u32(smem), sw = s_ring + a.ring * LE_TILE_BYTES,
                  sa = sw + a.wbuf * w_bytes, a_bytes = uint32_t(NS) * a.Rp * 256;
   __shared__ uint64_t a_full[2], a_empty[2], w_full[LE_BUF], w_empty[LE_BUF], acc_full[LE_BUF],
-      acc_empty[LE_BUF], b_full[LE_RING_MAX], b_empty[LE_RING_MAX];
+      acc_empty[LE_BUF], b_full[LE_RING_MAX], b_empty[LE_RING_MAX], mma_done;
   __shared__ uint32_t tmem_slot;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -866,6 +870,7 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
       mbar_init(&b_full[i], 4);
       mbar_init(&b_empty[i], 4);
     }
+    mbar_init(&mma_done, 1);
     fence_barrier_init();
   }
   if (warp == 4) {
@@ -959,6 +964,10 @@ __global__ void __launch_bounds__(LE_THREADS, 1)
         tc_commit_el(&acc_full[b]);
       }
       if (ok) tc_commit_el(&a_empty[ab]);
+    }
+    if (!ok) {                            // TMEM and the operands outlive the MMAs (bounded)
+      tc_commit_el(&mma_done);
+      warp_wait(&mma_done, 0);
     }
     __syncwarp();
   } else if (warp == 5) {
