@@ -1560,8 +1560,9 @@ __global__ void __launch_bounds__(LG_COLS) k_lora_join(const LoraWgrad a) {
     // CTA k's piece of the item is its first one (place 0) unless the item begins inside it
     const int64_t slot = 2 * k + (k == f && sg.item0 > f * cut.per ? 1 : 0);
     const float *src = a.part + slot * a.R * LG_COLS + threadIdx.x;
+    // (not __ldg: this grid starts while k_lora_wgrad still writes, so the sums are not read-only)
 #pragma unroll
-    for (int x = 0; x < 8; ++x) v[x] += __ldg(src + (c0 + x) * LG_COLS);
+    for (int x = 0; x < 8; ++x) v[x] += __ldcg(src + (c0 + x) * LG_COLS);
   }
   lora_wgrad_store<OT>(sd, static_cast<OT *>(sd.out) + int64_t(sg.adapter) * a.R * sd.C, a.R,
                        int64_t(sg.cb) * LG_COLS + threadIdx.x, c0, 8, v);
