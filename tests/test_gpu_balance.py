@@ -325,6 +325,17 @@ def test_router_training_step(cuda, T, func):
     assert same[2].shape == (1, T, 64) and _eq(same[2][0], dz)
 
 
+@pytest.mark.parametrize("T, E, K", [(2400, 64, 256), (400, 384, 512), (1301, 100, 32)])
+def test_router_logits_of_many_tokens(cuda, T, E, K):
+    """Enough tiles for all SMs: the products are written by one launch, K not split."""
+    gate, gen = _gate(E, K)
+    x = torch.randn(T, K, generator=gen, device="cuda").to(BF)
+    z = gate.logits(x)
+    z64 = x.to(D) @ gate.weight.to(D).T
+    mag = x.to(D).abs() @ gate.weight.to(D).abs().T
+    assert z.shape == (T, E) and ((z.to(D) - z64).abs() <= 4 * K ** 0.5 * 2.0 ** -23 * mag).all()
+
+
 def test_graph_replay(cuda):
     graphs = []
     for T in (50, 4000):

@@ -418,6 +418,138 @@ def test_backward_pieces_of_many_rings(cuda, R, dt, kind, n, N):
         assert all(_eq(u, v) for u, v in zip(got, again))
 
 
+# Sums of a single term: what is left of an error is the rounding of scaling times h or g (half a
+# step of 2^-23), and at most one truncated or rounded step for each of the three additions that
+# join the parts.  (A result from two parts, 17 bits, would be off by up to 64 steps.)
+_SINGLE = 4 * 2.0 ** -23
+
+
+def _one_row_a_column(gen, rows, cols):
+    """bf16 [rows, cols] with one value in every column, in different rows."""
+    v = torch.zeros(rows, cols, dtype=BF, device="cuda")
+    at = torch.randperm(rows, generator=gen, device="cuda")[:cols]
+    v[at, torch.arange(cols, device="cuda")] = _randn(gen, cols) + 2
+    return v
+
+
+@pytest.mark.parametrize("R", [8, 24, 64, 96, 104, 128])
+@pytest.mark.parametrize("T, N", [(5, 200), (3000, 200), (3000, 201)])
+def test_fp32_results_keep_every_bit_of_h_and_g(cuda, T, N, R):
+    n, K = 3, 256
+    c = _case(R + T + N, T, K, N, R, n)
+    ids = _ids("mixed", T, n, c["g"])
+    for w in (c["b"], c["a"].transpose(1, 2)):     # one rank in every column
+        w *= torch.eye(R, device="cuda").repeat(w.shape[1] // R + 1, 1)[:w.shape[1]].to(BF)
+    full = torch.randn(n, R, K, generator=c["g"], device="cuda").to(BF)
+    y, h = q.lora.lora_forward(c["x"], full, c["b"], ids, c["s"], out_dtype=F32, return_h=True)
+    live = ids >= 0
+    hs = h.to(D) * (c["s"].to(D)[ids.clamp(min=0).long()] * live)[:, None]
+    want = torch.einsum("tr,tcr->tc", hs, _sel(c["b"], ids))
+    assert want[live].abs().min() > 0 and ((y.to(D) - want).abs() <= _SINGLE * want.abs()).all()
+    if T < K:
+        return
+    c["x"], dy = _one_row_a_column(c["g"], T, K), _one_row_a_column(c["g"], T, N)
+    c["b"] = _randn(c["g"], n, N, R)
+    h = _randn(c["g"], T, R, dtype=F32)
+    got = q.lora.lora_backward(dy, c["x"], h, c["a"], c["b"], ids, c["s"], None, F32, F32)
+    want, _ = _backward64(c, ids, dy, h, None)
+    for g, w in zip(got, want):
+        assert (w != 0).any() and ((g.to(D) - w).abs() <= _SINGLE * w.abs()).all()
+
+
+@pytest.mark.parametrize("shape", [(700, 512, 1000, 16, 4), (700, 512, 1001, 64, 4),
+                                   (3000, 264, 96, 128, 3), (130, 72, 33, 8, 2)], ids=str)
+def test_backward_of_mixed_types(cuda, shape):
+    """dx and the weights' gradients have types of their own: the bits of one do not depend on the
+    other's type."""
+    T, K, N, R, n = shape
+    c = _case(sum(shape), *shape)
+    ids = _ids("mixed", T, n, c["g"])
+    dy, h = _randn(c["g"], T, N), _randn(c["g"], T, R, dtype=F32)
+
+    def grads(xdt, gdt):
+        return q.lora.lora_backward(dy, c["x"], h, c["a"], c["b"], ids, c["s"], None, xdt, gdt)
+    same = {dt: grads(dt, dt) for dt in (BF, F32)}
+    for xdt, gdt in ((BF, F32), (F32, BF)):
+        dx, da, db = grads(xdt, gdt)
+        assert dx.dtype == xdt and da.dtype == db.dtype == gdt
+        assert _eq(dx, same[xdt][0]) and _eq(da, same[gdt][1]) and _eq(db, same[gdt][2])
+
+
+@pytest.mark.parametrize("dt", [BF, F32], ids=str)
+@pytest.mark.parametrize("T", [6, 3000])
+def test_infinities_stay_where_they_enter(cuda, T, dt):
+    """Exactly the elements whose sums an infinity enters are not finite (infinite, or NaN where
+    its products with the parts of h or g do not add up); all others keep their bits."""
+    inf, n, R, K, N = float("inf"), 3, 16, 136, 72
+    c = _case(90, T, K, N, R, n)
+    ids = _ids("mixed", T, n, c["g"])
+    ids[T - 1], ids[0] = 1, 0                      # the last row: the one that padding repeats
+    mine, t0 = ids == 1, T - 1
+    x, a, b, s = c["x"], c["a"], c["b"], c["s"]
+    dy, h = _randn(c["g"], T, N), _randn(c["g"], T, R, dtype=F32)
+
+    def put(v, *at):
+        v = v.clone()
+        v[at] = inf
+        return v
+
+    def fwd(x, a, b):
+        return q.lora.lora_forward(x, a, b, ids, s, out_dtype=dt, return_h=True)
+
+    def bwd(dy, x, a, b):
+        return q.lora.lora_backward(dy, x, h, a, b, ids, s, None, dt, dt)
+
+    def only(got, want, *where):
+        for v, w, at in zip(got, want, where):
+            bad = torch.zeros_like(v, dtype=torch.bool)
+            if at is not None:
+                bad[at] = True
+            assert _eq(torch.isfinite(v), ~bad) and _eq(v[~bad], w[~bad])
+    y, g = fwd(x, a, b), bwd(dy, x, a, b)
+    every = slice(None)
+    only(fwd(put(x, t0, 5), a, b), y, (t0,), (t0,))
+    only(fwd(x, put(a, 1, 2, 5), b), y, (mine,), (mine, 2))
+    only(fwd(x, a, put(b, 1, 7, 3)), y, (mine, 7), None)
+    only(bwd(dy, put(x, t0, 5), a, b), g, None, (1, every, 5), None)
+    only(bwd(dy, x, put(a, 1, 2, 5), b), g, (mine, 5), None, None)
+    only(bwd(put(dy, t0, 7), x, a, b), g, (t0,), (1,), (1, 7))
+    only(bwd(dy, x, a, put(b, 1, 7, 3)), g, (mine,), (1, 3), None)
+
+
+def test_two_captured_graphs_of_sorted_tiles_at_once(cuda):
+    cs = [_case(150 + i, T, 520, 264, R, 4) for i, (T, R) in enumerate(((2000, 16), (3000, 104)))]
+    graphs = []
+    for c, dt in zip(cs, (BF, F32)):
+        T = c["x"].shape[0]
+        c["ids"] = _ids("mixed", T, 4, c["g"])
+        c["dy"] = _randn(c["g"], T, 264)
+
+        def step(c=c, dt=dt):
+            y, h = q.lora.lora_forward(c["x"], c["a"], c["b"], c["ids"], c["s"], out_dtype=dt,
+                                       return_h=True)
+            return (y, h) + q.lora.lora_backward(c["dy"], c["x"], h, c["a"], c["b"], c["ids"],
+                                                 c["s"], None, dt, dt)
+        step()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = step()
+        graphs.append((g, outs, step, torch.cuda.Stream()))
+    for rnd in range(3):
+        for c in cs:
+            c["x"].copy_(_randn(c["g"], *c["x"].shape))
+            c["ids"].copy_(_ids(("mixed", "runs", "none")[rnd], c["x"].shape[0], 4, c["g"]))
+        torch.cuda.synchronize()
+        for g, _, _, st in graphs:
+            with torch.cuda.stream(st):
+                for _ in range(4):
+                    g.replay()
+        torch.cuda.synchronize()
+        for _, outs, step, _ in graphs:
+            assert all(_eq(o, w) for o, w in zip(outs, step()))
+
+
 def test_gradients_by_differences(cuda):
     """d sum(y * dy) / d(x, a, b) along a direction, from two forward passes.  y is linear in
     each of x, a and b, so the difference quotient is exact but for rounding."""
