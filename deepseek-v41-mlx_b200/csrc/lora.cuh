@@ -359,11 +359,13 @@ struct LoraSteps {
 };
 
 // v as bf16 parts; the rest after each part is exact in fp32 (and zero after an infinity or NaN).
+// A finite value that would round to an infinity gets the largest bf16 and its rest.
 template <int NS>
 __device__ __forceinline__ void split_bf16(float v, uint16_t (&p)[NS]) {
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
     p[i] = f2bf_bits(v);
+    if ((p[i] & 0x7F80) == 0x7F80 && fabsf(v) < INFINITY) p[i] -= 1;
     v = (p[i] & 0x7F80) == 0x7F80 ? 0.0f : v - bf_bits2f(p[i]);
   }
 }

@@ -517,6 +517,30 @@ def test_infinities_stay_where_they_enter(cuda, T, dt):
     only(bwd(dy, x, a, put(b, 1, 7, 3)), g, (mine,), (1, 3), None)
 
 
+@pytest.mark.parametrize("T", [6, 3000])
+def test_values_past_the_largest_bf16(cuda, T):
+    """h and g up to fp32's largest value, which a bf16 rounds to infinity: products that fit stay
+    finite and keep every bit (sums of single terms and powers of two: no rounding at all)."""
+    n, K, N, R = 2, 16, 24, 8
+    ids = (torch.arange(T, device="cuda") % n).int()
+    x, a = torch.zeros(T, K, dtype=BF, device="cuda"), torch.zeros(n, R, K, dtype=BF, device="cuda")
+    b = torch.zeros(n, N, R, dtype=BF, device="cuda")
+    x[:, 0], x[:, 1] = 2.0 ** 64, 2.0 ** 50
+    a[:, 0, 0], a[:, 0, 1] = 2.0 ** 63 * 255 / 128, 2.0 ** 69 * 1.25
+    a[1] *= -1
+    b[:, :, 0] = 2.0 ** -10
+    y, h = q.lora.lora_forward(x, a, b, ids, out_dtype=F32, return_h=True)
+    big = 2.0 ** 127 * (255 / 128 + 1.25 * 2.0 ** -8)          # past the middle to 2^128
+    sign = torch.where(ids == 0, 1.0, -1.0).to(D)[:, None]
+    assert (h[:, :1].to(D) == big * sign).all() and (y.to(D) == big * 2.0 ** -10 * sign).all()
+    y = q.lora.lora_forward(x, a, b, ids)
+    assert (y.to(D) == 2.0 ** 118 * sign).all()
+    dy = torch.zeros(T, N, dtype=BF, device="cuda")
+    dy[0, 3] = dy[1, 3] = 2.0 ** -20
+    dx, da, db = q.lora.lora_backward(dy, x, h, a, b, ids, dx_dtype=F32, grad_dtype=F32)
+    assert (db[:, 3, 0].to(D) == big * 2.0 ** -20 * sign[:2, 0]).all()
+
+
 def test_two_captured_graphs_of_sorted_tiles_at_once(cuda):
     cs = [_case(150 + i, T, 520, 264, R, 4) for i, (T, R) in enumerate(((2000, 16), (3000, 104)))]
     graphs = []
