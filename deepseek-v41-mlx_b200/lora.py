@@ -43,6 +43,8 @@ def _tensor(v, name, dtype, device):
 def _operands(x, a, b, ids, scaling):
     """x bf16, the bank, the ids int32, the device and the sizes T, K, N, n, R."""
     t = L.torch()
+    if ids is None:
+        raise ValueError("ids must name the adapter of each token (negative: none)")
     x = L.cuda_tensor(x, "x")
     if x.dtype != t.bfloat16:
         x = x.to(t.bfloat16)

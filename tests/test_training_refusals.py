@@ -71,3 +71,16 @@ def test_cpu_tensors_are_refused():
         q.lora.lora_forward(x, a, b, ids)
     with pytest.raises(q.DSV41Error):
         q.moe.balance_loss(torch.zeros(4, 8), ids.view(4, 1))
+
+
+def test_missing_ids_are_refused():
+    import pytest
+    import torch
+
+    import deepseek_v41_mlx_b200 as q
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    a, b = torch.zeros(2, 8, 64, dtype=torch.bfloat16), torch.zeros(2, 32, 8, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="ids"):
+        q.lora.lora_forward(x, a, b, None)
+    with pytest.raises(ValueError, match="ids"):
+        q.lora.LoRA(a, b).backward(x, x, x, None)
