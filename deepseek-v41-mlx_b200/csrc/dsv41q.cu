@@ -861,16 +861,18 @@ extern "C" int dsv41_moe_balance(const void *logits, int dtype, int64_t T, int64
     sh.grid = unsigned(ceil_div(ceil_div(T, p.run), BL_WARPS));
     sh.smem = add;
     const int64_t n = S * E + S;
-    ProfScope prof("balance_count", st);
     if (n <= BL_COUNT_INTS && T * topk <= BL_CLUSTER_CHOICES) {
+      ProfScope prof("balance_count", st);
       DSV41_LAUNCH(max_dynamic_smem(k_balance_count, n * 4), "balance_count");
       DSV41_LAUNCH(launch_cluster(false, k_balance_count, 8, 8, 1024, size_t(n) * 4, st, p),
                    "balance_count");
     } else {
       const unsigned grid = unsigned(num_sms());
       const int shared = n <= BL_COUNT_INTS;
+      { ProfScope prof("balance_zero", st);
       k_balance_zero<<<unsigned(std::min<int64_t>(grid, ceil_div(n + 1, 256))), 256, 0, st>>>(p);
-      DSV41_CHECK_LAUNCH("balance_zero");
+      DSV41_CHECK_LAUNCH("balance_zero"); }
+      ProfScope prof("balance_count", st);
       DSV41_LAUNCH(max_dynamic_smem(k_balance_count_wide, shared ? n * 4 : 0), "balance_count");
       DSV41_LAUNCH(launch_pdl_if(true, k_balance_count_wide, dim3(grid), dim3(256),
                                  shared ? size_t(n) * 4 : 0, st, p, shared), "balance_count");
@@ -1151,9 +1153,11 @@ cudaError_t lora_wgrad_go(const LoraWgradMaps &m, const LoraWgrad &a, const Lora
                           cudaStream_t st) {
   cudaError_t e = max_dynamic_smem(k_lora_wgrad<OT, S>, sh.smem);
   if (e != cudaSuccess) return e;
+  { ProfScope prof("lora_wgrad", st);
   e = launch_pdl_if(true, k_lora_wgrad<OT, S>, dim3(unsigned(sh.grid)), dim3(LG_THREADS), sh.smem, st,
-                    m, a);
+                    m, a); }
   if (e != cudaSuccess) return e;
+  ProfScope prof("lora_join", st);
   return launch_pdl_if(true, k_lora_join<OT>, dim3(unsigned(sh.grid), unsigned(a.R / 8)),
                        dim3(LG_COLS), 0, st, a);
 }
@@ -1297,12 +1301,9 @@ extern "C" int dsv41_lora_backward(const void *dy, const void *x, const float *h
   rc = lora_rows_maps(&maps.v[0], x, T, K, 2);
   if (!rc && N % 8 == 0) rc = lora_rows_maps(&maps.v[1], dy, T, N, 2);
   if (rc) return rc;
-  {
-    ProfScope prof("lora_wgrad", st);
-    const cudaError_t ge = grad_dtype == DSV41_F32 ? lora_wgrad_launch<float>(maps, g, sh, st)
-                                                   : lora_wgrad_launch<__nv_bfloat16>(maps, g, sh, st);
-    if (ge != cudaSuccess) return cuda_status(ge, "lora_wgrad");
-  }
+  const cudaError_t ge = grad_dtype == DSV41_F32 ? lora_wgrad_launch<float>(maps, g, sh, st)
+                                                 : lora_wgrad_launch<__nv_bfloat16>(maps, g, sh, st);
+  if (ge != cudaSuccess) return cuda_status(ge, "lora_wgrad");
   LoraExpand e{};
   e.parts = w.parts;
   e.np = s.np;

@@ -702,6 +702,35 @@ def test_side_stream(cuda):
     assert all(_eq(v, want) for v in got)
 
 
+def test_every_launch_is_counted(cuda):
+    """The launches that dsv41_prof_launches counts are the kernels that a call launches."""
+    def launches(fn):
+        fn()
+        L.prof_enable(True)
+        fn()
+        torch.cuda.synchronize()
+        report = {k: v[0] for k, v in L.prof_report().items()}
+        n = L.prof_launches()
+        L.prof_enable(False)
+        assert n == sum(report.values())
+        return report
+    c = _case(71, 3000, 264, 136, 16, 3)
+    ids = _ids("mixed", 3000, 3, c["g"])
+    dy, h = _randn(c["g"], 3000, 136), _randn(c["g"], 3000, 16, dtype=F32)
+    one = dict.fromkeys
+    assert launches(lambda: q.lora.lora_forward(c["x"][:4], c["a"], c["b"], ids[:4])) == \
+        one(["lora_decode"], 1)
+    assert launches(lambda: q.lora.lora_forward(c["x"], c["a"], c["b"], ids)) == \
+        one(["lora_plan", "lora_shrink", "lora_expand"], 1)
+    assert launches(lambda: q.lora.lora_backward(dy, c["x"], h, c["a"], c["b"], ids)) == \
+        one(["lora_plan", "lora_shrink", "lora_wgrad", "lora_join", "lora_expand"], 1)
+    for T, names in ((64, ["balance"]), (5000, ["balance_count", "balance"]),
+                     (20000, ["balance_zero", "balance_count", "balance"])):
+        z = torch.zeros(T, 64, device="cuda")
+        idx = torch.zeros(T, 4, dtype=torch.int32, device="cuda")
+        assert launches(lambda: q.moe.balance_loss(z, idx, grad_loss=1.0)) == one(names, 1)
+
+
 def test_no_tokens(cuda):
     c = _case(70, 0, 64, 40, 8, 3)
     ids = torch.empty(0, dtype=torch.int32, device="cuda")
