@@ -1045,17 +1045,65 @@ int lora_plan_launch(const int32_t *ids, int64_t T, int64_t n, const LoraPlan &p
   return DSV41_OK;
 }
 
-// A forward call of few tokens is one launch (k_lora_decode): a cluster of C CTAs a token.  A
-// round of CTAs takes about 5 us and 1 us for every 50 KB of its share of an adapter; C is the one
-// with the least of it, and 0 where plan, shrink and expand (23 us and up) are expected to be
-// faster.  (Measured at R 16, K 7168, N 4096: 32 tokens 8.3 us with C = 8, 96 10.8 us with 4, 192
-// 15.7 us with 2, against 30 to 35 us.)
-unsigned lora_decode_ctas(int64_t T, int64_t K, int64_t N, int64_t R) {
-  const int64_t slots = int64_t(num_sms()) * (R <= 32 ? 3 : 1);
-  double best = 24.0;
+// k_lora_decode's variant for a rank: ranks a warp and lanes a row of B follow R.
+template <typename OT, typename F>
+cudaError_t lora_decode_kernel(int64_t R, F &&f) {
+  if (R <= 8) return f(k_lora_decode<OT, 256, 1, 1>, 256u, 0);
+  if (R <= 16) return f(k_lora_decode<OT, 256, 2, 2>, 256u, 1);
+  if (R <= 32) return f(k_lora_decode<OT, 256, 4, 4>, 256u, 2);
+  if (R <= 64) return f(k_lora_decode<OT, 512, 4, 8>, 512u, 3);
+  return f(k_lora_decode<OT, 512, 8, 16>, 512u, 4);
+}
+
+// Clusters of c CTAs (2, 4 or 8) of k_lora_decode that the device holds at once, asked once a
+// device: fewer than its SMs over c, since a cluster stays within a part of the chip (of 8: 48 up to
+// R 32, 15 above, where the SMs alone would make 55 and 18).
+int64_t lora_decode_clusters(int64_t R, unsigned c, int dev, int sms) {
+  static std::atomic<int> known[16][5][3];
+  int n = 0;
+  const cudaError_t e = lora_decode_kernel<__nv_bfloat16>(R, [&](auto *kernel, unsigned block, int v) {
+    std::atomic<int> *slot = dev >= 0 && dev < 16 ? &known[dev][v][c == 8 ? 2 : c == 4 ? 1 : 0] : nullptr;
+    if (slot && (n = slot->load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c);
+    cfg.blockDim = dim3(block);
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {c, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t q = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    if (q == cudaSuccess && slot) slot->store(n, std::memory_order_relaxed);
+    return q;
+  });
+  if (e != cudaSuccess) cudaGetLastError();
+  return e == cudaSuccess && n > 0 ? n : std::max(1, sms * (R <= 32 ? 3 : 1) / int(c));
+}
+
+// A forward call of few tokens is one launch (k_lora_decode): a cluster of C CTAs a token; returns
+// C, or 0 for plan, shrink and expand, whichever is estimated to be faster.  A round of clusters
+// takes 4 us and its CTAs' shares of an adapter at 40 KB a us, or 55 KB a us and SM where they share
+// one; the three launches 19 us, 0.1 us a MB of the adapters used and 0.7 us a MB of tokens.  Timed
+// both ways at ten shapes (R 8 to 128, K and N 1000 to 14336), 4 and 32 adapters, T 1 to 512: the
+// choice is within 1% of the fastest on average and 23% at worst (6.4 against 5.2 us).  At K 7168, N
+// 14336, R 128 and 4 adapters: one launch 27.0 us at 8 tokens and 50.6 at 16, three 27.5 and 27.4; at
+// K 7168, N 4096, R 16: one launch 7 us at 1 token and 15 at 200, three 20 us and more.
+unsigned lora_decode_ctas(int64_t T, int64_t K, int64_t N, int64_t n, int64_t R) {
+  const double adapter = double(R) * double(K + N) * 2;
+  double best = 19.0 + double(std::min(n, T)) * adapter * 0.1e-6 +
+                double(T) * double(K + 2 * N) * 2 * 0.7e-6;
   unsigned c_best = 0;
+  int dev = -1;
+  cudaGetDevice(&dev);
+  const int sms = num_sms();
   for (unsigned c = 8; c >= 2; c >>= 1) {
-    const double cost = double(ceil_div(T * c, slots)) * (5.0 + double(R * (K + N)) * 2.0 / c / 50e3);
+    const int64_t slots = lora_decode_clusters(R, c, dev, sms);
+    auto round = [&](int64_t m) {
+      if (m == 0) return 0.0;
+      const double sharing = std::max(1.0, double(m * c) / sms);
+      return 4.0 + adapter / c * std::max(1 / 40e3, sharing / 55e3);
+    };
+    const double cost = double(T / slots) * round(slots) + round(T % slots);
     if (cost < best) {
       best = cost;
       c_best = c;
@@ -1066,12 +1114,9 @@ unsigned lora_decode_ctas(int64_t T, int64_t K, int64_t N, int64_t R) {
 
 template <typename OT>
 cudaError_t lora_decode_launch(const LoraDecode &p, int64_t T, unsigned C, cudaStream_t st) {
-  const unsigned grid = unsigned(T) * C;
-  if (p.R <= 8) return launch_cluster(false, k_lora_decode<OT, 256, 1, 1>, grid, C, 256, 0, st, p);
-  if (p.R <= 16) return launch_cluster(false, k_lora_decode<OT, 256, 2, 2>, grid, C, 256, 0, st, p);
-  if (p.R <= 32) return launch_cluster(false, k_lora_decode<OT, 256, 4, 4>, grid, C, 256, 0, st, p);
-  if (p.R <= 64) return launch_cluster(false, k_lora_decode<OT, 512, 4, 8>, grid, C, 512, 0, st, p);
-  return launch_cluster(false, k_lora_decode<OT, 512, 8, 16>, grid, C, 512, 0, st, p);
+  return lora_decode_kernel<OT>(p.R, [&](auto *kernel, unsigned block, int) {
+    return launch_cluster(false, kernel, unsigned(T) * C, C, block, 0, st, p);
+  });
 }
 
 template <bool WMN, bool VEC, int S>
@@ -1178,7 +1223,7 @@ cudaError_t lora_wgrad_launch(const LoraWgradMaps &m, const LoraWgrad &a, const 
 extern "C" size_t dsv41_lora_workspace_size(int64_t T, int64_t K, int64_t N, int64_t n, int64_t R,
                                             int backward) {
   if (T < 0 || K <= 0 || N <= 0 || n <= 0 || R <= 0) return 0;
-  if (T == 0 || (!backward && lora_decode_ctas(T, K, N, R))) return 0;
+  if (T == 0 || (!backward && lora_decode_ctas(T, K, N, n, R))) return 0;
   return lora_carve(nullptr, ~size_t(0), T, K, N, n, R, backward != 0).used;
 }
 
@@ -1195,7 +1240,7 @@ extern "C" int dsv41_lora_forward(const void *x, int64_t T, int64_t K, const voi
   DSV41_REQUIRE(x && a && b && ids && y, DSV41_ERR_BAD_ARG, "NULL pointer");
   DSV41_REQUIRE(aligned(x, 16) && aligned(a, 16) && aligned(b, 16) && aligned(h_out, 16),
                 DSV41_ERR_MISALIGNED, "x, a, b and h_out must be 16-byte aligned");
-  if (const unsigned C = lora_decode_ctas(T, K, N, R)) {
+  if (const unsigned C = lora_decode_ctas(T, K, N, n, R)) {
     const LoraDecode d{static_cast<const __nv_bfloat16 *>(x), static_cast<const __nv_bfloat16 *>(a),
                        static_cast<const __nv_bfloat16 *>(b), K, N, int(R), int(n), scaling, ids,
                        base, y, h_out};

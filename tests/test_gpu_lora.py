@@ -702,6 +702,21 @@ def test_side_stream(cuda):
     assert all(_eq(v, want) for v in got)
 
 
+@pytest.mark.parametrize("T, K, N, n, R, few", [
+    (1, 7168, 4096, 8, 16, True), (64, 7168, 4096, 32, 16, True), (8, 7168, 14336, 4, 64, True),
+    (16, 7168, 14336, 4, 128, False), (384, 4096, 4096, 4, 32, False),
+    (256, 7168, 14336, 4, 16, False)], ids=str)
+def test_few_token_form_where_it_is_faster(cuda, T, K, N, n, R, few):
+    """The one-launch form (no workspace) at sizes where the other takes 1.4 times as long or more,
+    and the other way round; either gives the formula."""
+    nb = L.load().dsv41_lora_workspace_size(T, K, N, n, R, 0)
+    assert (nb == 0) == few
+    c = _case(T + R, T, K, N, R, n)
+    ids = _ids("mixed", T, n, c["g"])
+    y, h = q.lora.lora_forward(c["x"], c["a"], c["b"], ids, c["s"], return_h=True)
+    _check_forward(c, ids, None, BF, y, h)
+
+
 def test_every_launch_is_counted(cuda):
     """The launches that dsv41_prof_launches counts are the kernels that a call launches."""
     def launches(fn):
