@@ -16,7 +16,9 @@
 // HBM.  All sums are fp32.  Where h or g is an operand of a bf16 tensor-core product it goes in
 // as a sum of bf16 parts (v = p0 + p1 + ..., each the rounding of what the earlier ones leave):
 // two parts keep 17 bits or more, below the rounding of a bf16 result, three keep all 24 for an
-// fp32 result.  Shrink writes the parts, in sorted order, for both consumers.
+// fp32 result.  Shrink writes the parts, in sorted order, for both consumers.  (Parts may differ in
+// sign or be zero, so an infinite weight, x or dy that they meet gives NaN where one factor would give
+// an infinity; both stay in the elements whose sums it enters.)
 //
 // k_lora_plan sorts the tokens by adapter first (a stable counting sort), so that a tile of
 // 128 token rows belongs to one adapter; tokens without one come last.
@@ -424,7 +426,7 @@ constexpr int LS_X_BYTES = LR_TILE * LR_KB * 2;     // 16 KB
 // shared memory and are added in rank order.  Warps 0-3 fetch 32 token rows each, 64 values a
 // stage, warp 0 also the adapter's values, all by TMA; warp 4 issues the MMAs.  (Both went
 // through cp.async first: 512 bytes cost about 20 shared-memory cycles that way, which all but
-// caps an SM at its share of HBM.)  T 8192, K 7168, R 32: 26 us, 4.5 TB/s, of which some 7 are the
+// caps an SM at its share of HBM.)  T 8192, K 7168, R 32: 27 us, 4.3 TB/s, of which some 7 are the
 // start behind the plan and the join.  What stands in the rows past the tile's only reaches
 // accumulator rows that nobody reads.  Rows that TMA cannot address, of odd lengths, are staged
 // by the threads.
@@ -664,8 +666,8 @@ __device__ __forceinline__ float dot8(uint4 u, uint4 v, float acc) {
 // of K (its warps R / 8 ranks each), the partial h meet in distributed shared memory in rank
 // order, then each CTA takes a slice of the columns, a row of B per group of LPR lanes.  The
 // first rows of B are requested before the cluster meets.  Bound by the latency of one pass
-// over an adapter (360 KB at K 7168, N 4096, R 16: 7 us for one token, 10 us for 64), which tokens
-// on the same adapter find in L2.
+// over an adapter (360 KB at K 7168, N 4096, R 16: 7 us for one token, 10 us for 64 where L2 holds
+// the bank, 13 and 18 us where it has to be read), which tokens on the same adapter find in L2.
 // TH threads; RW: ranks a warp; LPR: lanes a row of B, the power of two at or above R / 8.
 template <typename OT, int TH, int RW, int LPR>
 __global__ void __launch_bounds__(TH) k_lora_decode(const LoraDecode p) {
@@ -836,7 +838,7 @@ constexpr int LE_EPI_LD = 36;                     // floats of a transposition r
 // W and the parts, the others are three epilogues that take turns (one's turn is about 2500 cycles
 // a tile: two fell behind HBM).  Row-wise plain loads and stores, through a transposition in shared
 // memory, kept the load/store pipe busy for twice the time that HBM needs (135 us at T 8192, N
-// 14336, R 32, against 79 us now: 5.9 TB/s).  Rows that TMA cannot address (VEC false: odd lengths)
+// 14336, R 32, against 77 us now: 6.1 TB/s).  Rows that TMA cannot address (VEC false: odd lengths)
 // are still moved that way, by a kernel of their own (in one kernel its rows pushed the hot loop
 // out of the instruction cache).
 template <bool WMN, typename OT, bool VEC>
@@ -1322,8 +1324,8 @@ __device__ __forceinline__ void lora_wgrad_store(const LoraGradSide &sd, OT *out
 // 0-3 fetch v's rows (missing ones repeat one of the adapter's own, against zero rows of u) and
 // u's block, the stages dealt in turn to four of them, or to three where the ring has three stages
 // (see P); 4 issues the MMAs, 5-8 read TMEM; accumulators are
-// double-buffered, so an item's stores overlap the next one.  T 8192, K 7168, N 4096, R 64: 38 us,
-// 4.9 TB/s (pieces of 256 bytes a row, and u once for every 128 columns), and 7 us the join.
+// double-buffered, so an item's stores overlap the next one.  T 8192, K 7168, N 4096, R 64: 39 us,
+// 4.7 TB/s (pieces of 256 bytes a row, and u once for every 128 columns), and 7 us the join.
 template <typename OT, int S>
 __global__ void __launch_bounds__(LG_THREADS, S == 6 || S == 3 ? 1 : 2) k_lora_wgrad(
     const __grid_constant__ LoraWgradMaps maps, const LoraWgrad a) {

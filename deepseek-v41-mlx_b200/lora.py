@@ -11,6 +11,11 @@ gives the gradients of x, a and b for training them beside frozen weights.  ``Lo
 an object; the layers of ``linear`` take one (``FP8Linear(...)(x, lora=bank, lora_ids=ids)``).
 The rank is a multiple of 8 up to 128 (pad a and b with zeros to mix ranks in one bank), K a
 multiple of 8.  Ids at or past n count as none and raise bit 1 of ``dsv41_device_status``.
+
+Tensors are taken as values: a result has no autograd history, even where an input requires a
+gradient; ``lora_backward`` is the gradient.  x, a, b, dy and h must start on 16 bytes (views that
+do not are refused); base, out and dx_base may start anywhere.  An infinity in x, a, b or dy makes
+the elements whose sums it enters infinite or NaN, and no others.
 """
 
 from __future__ import annotations

@@ -132,7 +132,9 @@ def balance_loss(logits, indices, offsets=None, mask=None, score_func="sqrtsoftp
     which is 1 for a balanced router with equal scores.  ``dlogits`` (given ``grad_loss``, a
     number or float32 [S], or ``dweights``, float32 [..., topk]) is the gradient of
     sum(grad_loss * loss) with the counts held constant, plus that of sum(dweights * weights)
-    for the routing weights that ``Gate`` gives for these logits and indices."""
+    for the routing weights that ``Gate`` gives for these logits and indices.  Tensors are taken
+    as values: the results have no autograd history.  A NaN among a live token's logits makes its
+    sequence's loss and its own gradient NaN."""
     t = _torch()
     z = L.cuda_tensor(logits, "logits")
     if z.dtype not in (t.float32, t.bfloat16):

@@ -195,18 +195,22 @@ int dsv41_gemv_affine(const void *x, int64_t M, int64_t K, const uint32_t *wq,
  * token (negative: none).  With i = ids[t]:
  *   h[t] = x[t] . a[i]^T          y[t] = base[t] + scaling[i] * (h[t] . b[i]^T)
  * base (may be NULL, may be y itself) and y [T, N] of out_dtype (F32 or BF16); rows without an
- * adapter get base (zeros when it is NULL).  h_out, if not NULL, receives h f32 [T, R] (zero
- * rows without an adapter) for the backward pass.  Sums are fp32, h is not rounded below 16
- * bits of mantissa, y is rounded once.  K a multiple of 8, R a multiple of 8 up to 128, n <=
- * 8192, T <= 2^30, N any; every tensor but y, the base, ids and scaling 16-byte aligned, and the
- * workspace.  An id at or past n counts as none and raises bit 1 of dsv41_device_status.
+ * adapter get base bit for bit (zeros when it is NULL).  h_out, if not NULL, receives h f32 [T, R]
+ * (zero rows without an adapter) for the backward pass.  Sums are fp32 and y is rounded once;
+ * scaling * h (and g below) enters its products with 17 significant bits or more for bf16 results
+ * and with all 24 for fp32 ones (magnitudes below 2^-110 with fewer).  An infinity in x, a, b or dy
+ * makes the elements whose sums it enters infinite or NaN, and no others.  K a multiple of 8, R a
+ * multiple of 8 up to 128, n <= 8192, T <= 2^30, N any; every tensor but y, the base, ids and
+ * scaling 16-byte aligned, and the workspace.  An id at or past n counts as none and raises bit 1
+ * of dsv41_device_status.
  *
  * dsv41_lora_backward: from dy bf16 [T, N], x and h of the forward pass, with g[t] =
  * scaling[i] * (dy[t] . b[i]):
  *   dx[t] = dx_base[t] + g[t] . a[i]    da[i] = sum_t g[t]^T x[t]
  *   db[i] = scaling[i] sum_t dy[t]^T h[t]
- * dx_base (may be NULL, may be dx) and dx [T, K] of dx_dtype; da [n, R, K] and db [n, N, R] of
- * grad_dtype, written whole (zeros for an adapter without tokens).  The same bits every time.
+ * dx_base (may be NULL, may be dx) and dx [T, K] of dx_dtype, rows without an adapter as above; da
+ * [n, R, K] and db [n, N, R] of grad_dtype, written whole (zeros for an adapter without tokens).
+ * The same bits every time.
  * The workspace may be NULL where its size is 0 (forward calls of few tokens: one launch). */
 size_t dsv41_lora_workspace_size(int64_t T, int64_t K, int64_t N, int64_t n, int64_t R,
                                  int backward);
@@ -247,7 +251,8 @@ int dsv41_moe_logits(const void *x, int64_t T, int64_t D, const void *gate_w, in
  * sum dweights * w over the unmasked tokens (dweights f32 [T, topk], NULL: left out), w the
  * routing weights of dsv41_moe_route for these logits and indices.  Masked tokens and tokens of
  * no sequence count nowhere, whatever they hold, and get zero gradients.  A row whose scores
- * are all zero (logits of -inf) adds nothing and gets a zero gradient from the loss.  loss f32
+ * are all zero (logits of -inf) adds nothing and gets a zero gradient from the loss; a NaN in a live
+ * row makes its sequence's loss and its own gradient NaN.  dlogits is no part of logits.  loss f32
  * [S], counts int32 [S, E].  1 <= E <= 1024, 1 <= topk <= min(64, E).  An index at or past E
  * counts as no choice and raises bit 1 of dsv41_device_status.  The same bits every time.
  * T, S <= 2^30.  The workspace (8-byte aligned) may be NULL where its size is 0. */
