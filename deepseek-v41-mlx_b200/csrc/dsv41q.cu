@@ -1056,8 +1056,8 @@ cudaError_t lora_decode_kernel(int64_t R, F &&f) {
 }
 
 // Clusters of c CTAs (2, 4 or 8) of k_lora_decode that the device holds at once, asked once a
-// device: fewer than its SMs over c, since a cluster stays within a part of the chip (of 8: 48 up to
-// R 32, 15 above, where the SMs alone would make 55 and 18).
+// device: fewer than its SMs over c, since a cluster stays within a part of the chip (of 8, on the
+// B200 that was asked: 48 up to R 32, 15 above, where the SMs alone would make 55 and 18).
 int64_t lora_decode_clusters(int64_t R, unsigned c, int dev, int sms) {
   static std::atomic<int> known[16][5][3];
   int n = 0;
