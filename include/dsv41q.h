@@ -196,7 +196,8 @@ int dsv41_gemv_affine(const void *x, int64_t M, int64_t K, const uint32_t *wq,
  *   h[t] = x[t] . a[i]^T          y[t] = base[t] + scaling[i] * (h[t] . b[i]^T)
  * base (may be NULL, may be y itself) and y [T, N] of out_dtype (F32 or BF16); rows without an
  * adapter get base bit for bit (zeros when it is NULL).  h_out, if not NULL, receives h f32 [T, R]
- * (zero rows without an adapter) for the backward pass.  Sums are fp32 and y is rounded once;
+ * (zero rows without an adapter) for the backward pass.  Sums are fp32 (those of the tensor cores
+ * truncate: m terms of one sign are off by up to m 2^-27 of their sum) and y is rounded once;
  * scaling * h (and g below) enters its products with 17 significant bits or more for bf16 results
  * and with all 24 for fp32 ones (magnitudes below 2^-110 with fewer).  An infinity in x, a, b or dy
  * makes the elements whose sums it enters infinite or NaN, and no others.  K a multiple of 8, R a
